@@ -1,0 +1,309 @@
+// Matrices in four bits (w4.h): into the form, out of it, and rows of it as token embeddings.
+#include "w4.h"
+
+#define W4_THREADS 256
+
+// Rounds a positive finite float to five significant bits, to nearest, ties to even.
+__device__ __forceinline__ float round5(float a) {
+  unsigned u = __float_as_uint(a);
+  u += 0x3ffffu + ((u >> 19) & 1u);
+  return __uint_as_float(u & 0xfff80000u);
+}
+
+// A group's scale from its largest and smallest element: an eighth of the largest magnitude, in five significant bits,
+// negative where that magnitude is a positive element's (so that the extreme is level -8, not the missing +8).  Below the
+// normal numbers: 0, the group is zeros.  Not above 31 * 2^120: 8 s has to stay finite.  NaN where an element is not finite.
+__device__ __forceinline__ float group_scale(float hi, float lo, bool finite) {
+  if (!finite) return __uint_as_float(0x7fc00000u);
+  const float a = fmaxf(hi, -lo) * 0.125f;
+  float s = fminf(round5(a), __uint_as_float(0x7df80000u));
+  if (s < 1.1754943508222875e-38f) s = 0.f;
+  return hi > -lo ? -s : s;
+}
+// The level of w under scale s, 0..15 = level + 8: w / s rounded to the nearest whole number, ties to even, EXACTLY.  The
+// quotient's own rounding may carry it onto or over a half; the remainder w - q s is exact in one fused operation (q s has
+// at most nine bits, and what is left of w is below s), and it says which side w lies on.
+__device__ __forceinline__ unsigned level_of(float w, float s) {
+  if (!(s != 0.f) || s != s) return 8u;
+  float q = rintf(w / s);
+  const float left = fmaf(-q, s, w), half = 0.5f * fabsf(s);
+  if (fabsf(left) > half) q += ((left > 0.f) == (s > 0.f)) ? 1.f : -1.f;
+  q = fminf(fmaxf(q, -8.f), 7.f);
+  return (unsigned)((int)q + 8);
+}
+
+// What lane (g, c) keeps of two chunks: rows g, g + 8 x quarters of 32 elements x its eight.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, bool row_ok, int k, int K, bool vec, float* v) {
+  if (!row_ok) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    return;
+  }
+  if (vec && k + 8 <= K) {
+    if (sizeof(T) == 2) {
+      const uint4 x = *(const uint4*)((const bf16*)row + k);
+      const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else {
+      const float4 x = *(const float4*)((const float*)row + k), y = *(const float4*)((const float*)row + k + 4);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f(row[k + i]) : 0.f;
+}
+// Two rows' eight levels (0..15 each) of a half chunk -> the two words of w4.h.
+__device__ __forceinline__ unsigned pack_word(const unsigned* a, const unsigned* b) {
+  return a[0] | b[0] << 4 | a[2] << 8 | b[2] << 12 | a[1] << 16 | b[1] << 20 | a[3] << 24 | b[3] << 28;
+}
+
+struct W4Out { uint4* q; unsigned* s; int N, K, chunks, groups, gshift; };
+
+// A warp a slab x 128 elements.  Bound by the matrix's bytes: every element is read once, by loads of 16 bytes whose four
+// neighbouring lanes take 64 (128 where T is float) consecutive bytes of a row.
+template <typename T>
+__global__ void __launch_bounds__(W4_THREADS) quantize_w4_kernel(const T* w, long long ldw, int vec, W4Out o) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int pairs = (o.chunks + 1) / 2;
+  const long long unit = (long long)blockIdx.x * (W4_THREADS / 32) + (threadIdx.x >> 5);
+  const int slab = (int)(unit / pairs), pair = (int)(unit % pairs);
+  if (slab * W4_SLAB >= o.N) return;
+  float v[2][4][8];
+  float hi[2][4], lo[2][4];
+  bool fin[2][4];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int n = slab * W4_SLAB + g + 8 * r;
+    const T* row = w + (size_t)n * ldw;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) load8(row, n < o.N, pair * 128 + h * 32 + c * 8, o.K, vec != 0, v[r][h]);
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      float a = v[r][h][0], b = a;
+      bool ok = true;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { a = fmaxf(a, v[r][h][i]); b = fminf(b, v[r][h][i]); ok = ok && fabsf(v[r][h][i]) <= 3.4028234663852886e38f; }
+#pragma unroll
+      for (int x = 1; x < 4; x <<= 1) {
+        a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
+        b = fminf(b, __shfl_xor_sync(0xffffffffu, b, x));
+        ok = __shfl_xor_sync(0xffffffffu, (int)ok, x) && ok;
+      }
+      hi[r][h] = a; lo[r][h] = b; fin[r][h] = ok;
+    }
+  // groups of 64 and 128: the quarters' extremes put together
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int step = 1; step <= 2; step <<= 1) {
+      if ((32 * step) >> o.gshift) continue;               // (this distance is between groups already)
+#pragma unroll
+      for (int h = 0; h < 4; ++h) if (!(h & step)) {
+        const float a = fmaxf(hi[r][h], hi[r][h | step]), b = fminf(lo[r][h], lo[r][h | step]);
+        const bool ok = fin[r][h] && fin[r][h | step];
+        hi[r][h] = hi[r][h | step] = a; lo[r][h] = lo[r][h | step] = b; fin[r][h] = fin[r][h | step] = ok;
+      }
+    }
+  float s[2][4];
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int h = 0; h < 4; ++h) s[r][h] = group_scale(hi[r][h], lo[r][h], fin[r][h]);
+#pragma unroll
+  for (int ch = 0; ch < 2; ++ch) {
+    if (2 * pair + ch >= o.chunks) break;
+    unsigned word[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      unsigned a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { a[i] = level_of(v[0][2 * ch + h][i], s[0][2 * ch + h]); b[i] = level_of(v[1][2 * ch + h][i], s[1][2 * ch + h]); }
+      word[2 * h] = pack_word(a, b); word[2 * h + 1] = pack_word(a + 4, b + 4);
+    }
+    o.q[((size_t)slab * o.chunks + 2 * pair + ch) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+  }
+  // quarter c's scales by lane c (a group's first quarter only)
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    if (c != h || ((h << 5) & ((1 << o.gshift) - 1))) continue;
+    const int grp = (pair * 128 + h * 32) >> o.gshift;
+    if (grp < o.groups) {
+      const unsigned lo16 = __float_as_uint(s[0][h]) >> 16, hi16 = __float_as_uint(s[1][h]) & 0xffff0000u;
+      o.s[((size_t)slab * o.groups + grp) * 8 + g] = lo16 | hi16;
+    }
+  }
+}
+
+// Levels and scales that exist already -> the layout.  bad: 1 a level outside -8..7, 2 a scale that is not finite, has more
+// than five significant bits or is so large that 8 s is not finite.
+__global__ void __launch_bounds__(W4_THREADS) pack_w4_kernel(const signed char* lv, long long ldl, const bf16* sc, long long lds, W4Out o, int groups_in, int* bad) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const long long unit = (long long)blockIdx.x * (W4_THREADS / 32) + (threadIdx.x >> 5);
+  const int slab = (int)(unit / o.chunks), chunk = (int)(unit % o.chunks);
+  if (slab * W4_SLAB >= o.N) return;
+  unsigned word[4];
+  bool wrong = false;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    unsigned u[2][8];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int n = slab * W4_SLAB + g + 8 * r, k = chunk * W4_CHUNK + h * 32 + c * 8;
+      const signed char* p = lv + (size_t)n * ldl + k;
+      signed char b[8];
+      const bool row_ok = n < o.N;
+      if (row_ok && k + 8 <= o.K && ((uintptr_t)p & 7) == 0) *(uint2*)b = *(const uint2*)p;
+      else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = row_ok && k + i < o.K ? p[i] : (signed char)0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { wrong = wrong || b[i] < -8 || b[i] > 7; u[r][i] = (unsigned)(b[i] + 8) & 15u; }
+    }
+    word[2 * h] = pack_word(u[0], u[1]); word[2 * h + 1] = pack_word(u[0] + 4, u[1] + 4);
+  }
+  if (wrong) atomicOr(bad, 1);
+  o.q[((size_t)slab * o.chunks + chunk) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+  // the groups that start in this chunk: lane c the c-th (a chunk starts two of 32, one of 64, every other one of 128)
+  const int first = (chunk * W4_CHUNK + (1 << o.gshift) - 1) >> o.gshift, end = ((chunk + 1) * W4_CHUNK + (1 << o.gshift) - 1) >> o.gshift;
+  const int grp = first + c;
+  if (grp < end && grp < o.groups) {
+    unsigned half[2];
+    bool odd = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int n = slab * W4_SLAB + g + 8 * r;
+      half[r] = n < o.N && grp < groups_in ? (unsigned)*(const unsigned short*)(sc + (size_t)n * lds + grp) : 0u;
+      const unsigned mag = half[r] & 0x7fffu;
+      odd = odd || (half[r] & 7u) || mag > 0x7df8u || (mag && mag < 0x80u);
+    }
+    if (odd) atomicOr(bad, 2);
+    o.s[((size_t)slab * o.groups + grp) * 8 + g] = half[0] | half[1] << 16;
+  }
+}
+
+// The eight elements of row `row` from k on (k a multiple of 8, in the padded width).
+__device__ __forceinline__ void row8(const W4Ref& m, int row, int k, float* v) {
+  const int slab = row / W4_SLAB, r = row % W4_SLAB, g = r & 7, chunk = k / W4_CHUNK, h = (k / 32) & 1, c = (k / 8) & 3;
+  const uint2 w = *((const uint2*)(m.q + ((size_t)slab * m.chunks + chunk) * 32 + 4 * g + c) + h);
+  const unsigned sw = m.s[((size_t)slab * m.groups + (k >> m.gshift)) * 8 + g];
+  const float s = r < 8 ? w4_scale_lo(sw) : w4_scale_hi(sw);
+  const int sh = r < 8 ? 0 : 4;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const unsigned u = (i ? w.y : w.x) >> sh;
+    v[4 * i + 0] = s * (float)((int)(u & 15u) - 8);
+    v[4 * i + 1] = s * (float)((int)(u >> 16 & 15u) - 8);
+    v[4 * i + 2] = s * (float)((int)(u >> 8 & 15u) - 8);
+    v[4 * i + 3] = s * (float)((int)(u >> 24 & 15u) - 8);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* v, int left, bool vec) {
+  if (vec && left >= 8) {
+    if (sizeof(T) == 2) {
+      unsigned w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); w[i] = *(unsigned*)&b; }
+      *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+      *(float4*)((float*)p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) if (i < left) p[i] = from_f<T>(v[i]);
+}
+
+// A thread eight elements: the values themselves (exact in either type).
+template <typename T>
+__global__ void __launch_bounds__(W4_THREADS) dequantize_w4_kernel(W4Ref m, T* out, long long ldo, int vec) {
+  const int pieces = (m.K + 7) / 8;
+  const long long i = (long long)blockIdx.x * W4_THREADS + threadIdx.x;
+  const int row = (int)(i / pieces), k = (int)(i % pieces) * 8;
+  if (row >= m.N) return;
+  float v[8];
+  row8(m, row, k, v);
+  store8(out + (size_t)row * ldo + k, v, m.K - k, vec != 0);
+}
+
+// A thread eight elements of a token's row, times `scale`.  A token outside the table: zeros and *status = 1.
+__global__ void __launch_bounds__(W4_THREADS) embed_rows_w4_kernel(const int* tokens, W4Ref m, float* out, int T, int vec, int* status, float scale) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int pieces = (m.K + 7) / 8;
+  const long long i = (long long)blockIdx.x * W4_THREADS + threadIdx.x;
+  const long long t = i / pieces;
+  const int k = (int)(i % pieces) * 8;
+  if (t >= T) return;
+  const int tok = tokens[t];
+  float v[8];
+  if (tok < 0 || tok >= m.N) {
+    if (status && k == 0) atomicExch(status, 1);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  } else {
+    row8(m, tok, k, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= scale;
+  }
+  store8(out + (size_t)t * m.K + k, v, m.K - k, vec != 0);
+}
+
+static int check_sizes(int N, int K, int chunks, int groups, int gshift) {
+  if (N < 1 || K < 1 || gshift < 5 || gshift > 7 || chunks != ceil_div(K, W4_CHUNK)) return FELLM_ERR_SIZE;
+  if (groups != (int)(((long long)chunks * W4_CHUNK + (1 << gshift) - 1) >> gshift)) return FELLM_ERR_SIZE;
+  return 0;
+}
+static bool grid_ok(long long blocks) { return blocks > 0 && blocks < (1ll << 31); }
+
+FELLM_API int fellm_quantize_w4(const void* w, int w_bf16, long long ldw, void* q, void* s, int N, int K, int chunks, int groups, int gshift, cudaStream_t stream) {
+  if (!w || !q || !s) return FELLM_ERR_ARG;
+  if (int e = check_sizes(N, K, chunks, groups, gshift)) return e;
+  const W4Out o = {(uint4*)q, (unsigned*)s, N, K, chunks, groups, gshift};
+  const long long units = (long long)ceil_div(N, W4_SLAB) * ((chunks + 1) / 2), blocks = (units + W4_THREADS / 32 - 1) / (W4_THREADS / 32);
+  if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
+  if (w_bf16) quantize_w4_kernel<bf16><<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const bf16*)w, ldw, ldw % 8 == 0 && ((uintptr_t)w & 15) == 0, o);
+  else quantize_w4_kernel<float><<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const float*)w, ldw, ldw % 4 == 0 && ((uintptr_t)w & 15) == 0, o);
+  return launch_status();
+}
+FELLM_API int fellm_pack_w4(const void* levels, long long ldl, const void* scales, long long lds, int groups_in, void* q, void* s, int N, int K,
+                            int chunks, int groups, int gshift, int* bad, cudaStream_t stream) {
+  if (!levels || !scales || !q || !s || !bad) return FELLM_ERR_ARG;
+  if (int e = check_sizes(N, K, chunks, groups, gshift)) return e;
+  const W4Out o = {(uint4*)q, (unsigned*)s, N, K, chunks, groups, gshift};
+  const long long units = (long long)ceil_div(N, W4_SLAB) * chunks, blocks = (units + W4_THREADS / 32 - 1) / (W4_THREADS / 32);
+  if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
+  pack_w4_kernel<<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const signed char*)levels, ldl, (const bf16*)scales, lds, o, groups_in, bad);
+  return launch_status();
+}
+FELLM_API int fellm_dequantize_w4(const void* q, const void* s, void* out, int out_bf16, long long ldo, int N, int K, int chunks, int groups, int gshift,
+                                  cudaStream_t stream) {
+  if (!q || !s || !out) return FELLM_ERR_ARG;
+  if (int e = check_sizes(N, K, chunks, groups, gshift)) return e;
+  const W4Ref m = {(const uint4*)q, (const unsigned*)s, N, K, chunks, groups, gshift};
+  const long long blocks = ((long long)N * ceil_div(K, 8) + W4_THREADS - 1) / W4_THREADS;
+  if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
+  const int vec = ldo % (out_bf16 ? 8 : 4) == 0 && ((uintptr_t)out & 15) == 0;
+  if (out_bf16) dequantize_w4_kernel<bf16><<<(unsigned)blocks, W4_THREADS, 0, stream>>>(m, (bf16*)out, ldo, vec);
+  else dequantize_w4_kernel<float><<<(unsigned)blocks, W4_THREADS, 0, stream>>>(m, (float*)out, ldo, vec);
+  return launch_status();
+}
+FELLM_API int fellm_embed_rows_w4(const int* tokens, const void* q, const void* s, void* out, int T, int N, int K, int chunks, int groups, int gshift,
+                                  int* status, float scale, cudaStream_t stream) {
+  if (T <= 0) return 0;
+  if (!tokens || !q || !s || !out) return FELLM_ERR_ARG;
+  if (int e = check_sizes(N, K, chunks, groups, gshift)) return e;
+  const W4Ref m = {(const uint4*)q, (const unsigned*)s, N, K, chunks, groups, gshift};
+  const long long blocks = ((long long)T * ceil_div(K, 8) + W4_THREADS - 1) / W4_THREADS;
+  if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
+  return launch_k_class(launch_class_for_rows(T, 2), embed_rows_w4_kernel, dim3((unsigned)blocks, 1, 1), dim3(W4_THREADS, 1, 1), 0, stream, 1,
+                        tokens, m, (float*)out, T, (int)(K % 4 == 0 && ((uintptr_t)out & 15) == 0), status, scale);
+}

@@ -1,0 +1,39 @@
+// A matrix [N, K] in four bits, as every kernel that reads one finds it.
+//
+// w[n, k] = q[n, k] s[n, k / G]: levels q of -8..7, a scale for every G (32, 64 or 128) consecutive elements of a row.  A
+// scale has at most five significant bits, a level at most four of which -8 needs one: their product has at most eight, so
+// it is a bfloat16 number EXACTLY, and the matrix means the same numbers to a kernel that scales its sums of x q group by
+// group and to one that feeds bfloat16 weights to the tensor cores.
+//
+// Levels: slabs of 16 rows x chunks of 64 k, 512 bytes each, slab after slab and in it chunk after chunk; a warp reads a
+// chunk in one load of 16 bytes a lane.  Lane 4 g + c has rows g and g + 8, and of the chunk's two halves the elements
+// 8 c .. 8 c + 7: word j is half j / 2, elements 4 (j % 2) .. + 3 of those eight.  In a word, four bits each, q + 8:
+//   bits  0 row g element 0,   4 row g+8 element 0,   8 row g element 2,  12 row g+8 element 2,
+//   bits 16 row g element 1,  20 row g+8 element 1,  24 row g element 3,  28 row g+8 element 3,
+// so that word >> 4 r, masked with 0x000f000f, is the r-th operand register of an mma.m16n8k16 whose k slots {2c, 2c+1,
+// 2c+8, 2c+9} are taken for elements {0, 1, 2, 3} (a sum does not ask in which order).
+// Scales: bfloat16 pairs (row g, row g + 8), eight of them for each slab and group.
+// Rows behind N are levels 0 under scales 0, elements behind K levels 0.
+#pragma once
+#include "common.cuh"
+
+#define W4_SLAB 16
+#define W4_CHUNK 64
+
+struct W4Ref {
+  const uint4* q;            // [slabs][chunks][32]
+  const unsigned* s;         // [slabs][groups][8]
+  int N, K, chunks, groups;  // groups: as many as cover chunks * 64 elements
+  int gshift;                // log2 of the group: 5, 6 or 7
+};
+
+// 128 + q + 8 in both halves is 0x4300 | (q + 8): the four bits are the lowest of bfloat16's mantissa at exponent 7.
+__device__ __forceinline__ unsigned w4_pair_biased(unsigned word, int r) { return ((word >> (4 * r)) & 0x000f000fu) | 0x43004300u; }
+// minus 136: the levels themselves, exactly.
+__device__ __forceinline__ unsigned w4_pair(unsigned word, int r) {
+  const unsigned b = w4_pair_biased(word, r), off = 0x43084308u;
+  __nv_bfloat162 v = __hsub2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&off);
+  return *(unsigned*)&v;
+}
+__device__ __forceinline__ float w4_scale_lo(unsigned s) { return __uint_as_float(s << 16); }
+__device__ __forceinline__ float w4_scale_hi(unsigned s) { return __uint_as_float(s & 0xffff0000u); }

@@ -1974,6 +1974,181 @@ def interleave_gate_up(gate, up):
     return torch.stack([gate.reshape(F // 8, 8, K), up.reshape(F // 8, 8, K)], dim=1).reshape(2 * F, K).contiguous()
 
 
+# ------------------------------------------------------------------------------ matrices in four bits
+
+W4_GROUPS = (32, 64, 128)
+
+
+class W4:
+    """A matrix [N, K] in four bits: w[n, k] = level[n, k] * scale[n, k // group], levels -8..7, scales of at most five
+    significant bits (level * scale is a bfloat16 number exactly, so every kernel that reads the matrix multiplies with the
+    same numbers).  Made by quantize_w4 or pack_w4, which return when it is laid out: any stream may read it, and a product
+    may ask for it before the kernel in front has ended.  q, scales: the kernels' layout (csrc/w4.h); nothing writes them again."""
+    dtype = "int4"                          # (of no torch dtype: what asks a matrix for bfloat16 leaves it alone)
+    is_cuda = True
+
+    def __init__(self, q, scales, N: int, K: int, group: int):
+        self.q, self.scales, self.shape, self.group = q, scales, (N, K), group
+        self._sizes = (N, K, q.shape[1], scales.shape[1], group.bit_length() - 1)        # as the launchers take them
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def nbytes(self) -> int:
+        return 4 * (self.q.numel() + self.scales.numel())
+
+    def data_ptr(self) -> int:
+        return self.q.data_ptr()
+
+
+def _w4_dev(*tensors):
+    """Everything on the current device: its stream is the one that is launched on."""
+    _dev(*tensors)
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"a tensor on {t.device}, but the current device is cuda:{here}")
+
+
+def _w4_room(N: int, K: int, group: int, device):
+    if group not in W4_GROUPS:
+        raise KernelError(f"a group of {group}: four-bit matrices have groups of {', '.join(map(str, W4_GROUPS))}")
+    if N < 1 or K < 1 or N > 2 ** 30 or K > 2 ** 30:
+        raise KernelError(f"a matrix of {N} x {K} cannot be held in four bits")
+    slabs, chunks = -(-N // 16), -(-K // 64)
+    return (torch.empty((slabs, chunks, 128), dtype=torch.int32, device=device),
+            torch.empty((slabs, -(-chunks * 64 // group), 8), dtype=torch.int32, device=device))
+
+
+def _w4_matrix(w, what: str):
+    if w.dim() != 2 or (w.shape[1] > 1 and w.stride(1) != 1):
+        raise KernelError(f"{what}: a matrix [N, K] whose rows are contiguous, not {list(w.shape)} with strides {list(w.stride())}")
+
+
+def _w4_laid_out(what: str):
+    if torch.cuda.is_current_stream_capturing():
+        raise KernelError(f"{what} waits for its result and cannot be captured into a CUDA graph")
+
+
+def quantize_w4(w, group: int = 64) -> W4:
+    """w [N, K] bfloat16 or float32 (row stride free) in four bits.  A group's scale is an eighth of its largest magnitude in
+    five significant bits, negative where that is a positive element's, so that the extreme becomes level -8; a level is
+    w / scale rounded to the nearest, ties to even.  A group with an element that is not finite becomes NaN."""
+    _w4_matrix(w, "quantize_w4")
+    q, s = _w4_room(w.shape[0], w.shape[1], group, w.device)
+    _w4_dev(w)
+    _w4_laid_out("quantize_w4")
+    out = W4(q, s, w.shape[0], w.shape[1], group)
+    f = _fn("w4", "fellm_quantize_w4", [_c_p, _c_int, _c_ll, _c_p, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p])
+    _check(f(_p(w), _is_bf16(w), w.stride(0), _p(q), _p(s), *out._sizes, _stream()), "quantize_w4")
+    torch.cuda.current_stream().synchronize()
+    return out
+
+
+def pack_w4(levels, scales, group: int) -> W4:
+    """A matrix whose levels (int8 [N, K], -8..7) and scales ([N, ceil(K / group)], bfloat16 or float32) are known.
+    Refuses levels outside their range and scales that have more than five significant bits, are not finite or too near
+    either end of bfloat16's range: their products with a level would not be bfloat16 numbers."""
+    _w4_matrix(levels, "pack_w4")
+    N, K = levels.shape
+    q, s = _w4_room(N, K, group, levels.device)
+    if levels.dtype != torch.int8:
+        raise KernelError(f"pack_w4: levels are int8, not {levels.dtype}")
+    if tuple(scales.shape) != (N, -(-K // group)):
+        raise KernelError(f"pack_w4: scales of {list(scales.shape)} for a matrix of {N} x {K} in groups of {group}")
+    _is_bf16(scales)
+    _w4_dev(levels, scales)
+    _w4_laid_out("pack_w4")
+    kept = scales.to(torch.bfloat16)
+    if scales.dtype == torch.float32 and not torch.equal(kept.float(), scales):
+        raise KernelError("pack_w4: scales of more than five significant bits")
+    kept = kept.contiguous()
+    out = W4(q, s, N, K, group)
+    bad = torch.zeros(1, dtype=torch.int32, device=levels.device)
+    f = _fn("w4", "fellm_pack_w4", [_c_p, _c_ll, _c_p, _c_ll, _c_int, _c_p, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p])
+    _check(f(_p(levels), levels.stride(0), _p(kept), kept.stride(0), kept.shape[1], _p(q), _p(s), *out._sizes, _p(bad), _stream()), "pack_w4")
+    code = int(bad.item())
+    if code & 1:
+        raise KernelError("pack_w4: levels outside -8..7")
+    if code:
+        raise KernelError("pack_w4: scales that are not finite, of more than five significant bits or at the ends of bfloat16's range")
+    return out
+
+
+def dequantize_w4(w: W4, out_dtype=torch.bfloat16, out=None):
+    """The matrix's values [N, K], exact in bfloat16 as in float32."""
+    if out is None:
+        out = torch.empty(w.shape, dtype=out_dtype, device=w.device)
+    _w4_matrix(out, "dequantize_w4")
+    if tuple(out.shape) != w.shape:
+        raise KernelError(f"dequantize_w4: a matrix of {list(w.shape)} does not fit {list(out.shape)}")
+    _w4_dev(w.q, out)
+    N, K, chunks, groups, gshift = w._sizes
+    f = _fn("w4", "fellm_dequantize_w4", [_c_p, _c_p, _c_p, _c_int, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p])
+    _check(f(_p(w.q), _p(w.scales), _p(out), _is_bf16(out), out.stride(0), N, K, chunks, groups, gshift, _stream()), "dequantize_w4")
+    return out
+
+
+def embed_rows_w4(tokens, table: W4, out, status=None, scale: float = 1.0):
+    """out[t, :] = table[tokens[t], :] * scale, float32.  A token outside the table writes zeros and sets status to 1."""
+    _i32(tokens, "tokens")
+    T = tokens.numel()
+    if out.dtype != torch.float32 or not out.is_contiguous() or tuple(out.shape) != (T, table.shape[1]):
+        raise KernelError(f"embed_rows_w4: out must be contiguous float32 [{T}, {table.shape[1]}]")
+    _w4_dev(tokens, table.q, out, status)
+    f = _fn("w4", "fellm_embed_rows_w4", [_c_p, _c_p, _c_p, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_f, _c_p])
+    _check(f(_p(tokens), _p(table.q), _p(table.scales), _p(out), T, *table._sizes, _p(status), float(scale), _stream()), "embed_rows_w4")
+    return out
+
+
+def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, swiglu=False, act=None):
+    """out = x[M, K] @ w[N, K]^T (+ bias), w in four bits, x bfloat16 or float32 (row stride free), float32 sums; the result is
+    bfloat16 for bfloat16 x unless out or out_dtype says float32, and float32 for float32 x.
+    accumulate: out (float32 [M, N]) += ; swiglu: w's rows are interleaved in blocks of 8 gate / 8 up (interleave_gate_up)
+    and the result [M, N/2] is silu(gate) * up; act="relu2": the result is max(., 0)^2."""
+    if x.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise KernelError(f"gemm_w4: x is {list(x.shape)} but w is {list(w.shape)}")
+    M, K = x.shape
+    N = w.shape[0]
+    x_bf16 = _is_bf16(x)
+    if K > 1 and x.stride(1) != 1:
+        raise KernelError(f"gemm_w4: x's rows must be contiguous, its strides are {list(x.stride())}")
+    if accumulate + swiglu + (act is not None) > 1:
+        raise KernelError("gemm_w4: one of accumulate, swiglu and act")
+    if act not in (None, "relu2"):
+        raise KernelError(f"gemm_w4: unknown activation {act!r}")
+    if swiglu and N % 16:
+        raise KernelError(f"gemm_w4: the gate/up matrix needs a multiple of 16 rows, got {N}")
+    if accumulate and out is None:
+        raise KernelError("gemm_w4: accumulate needs the tensor to add into")
+    cols = N // 2 if swiglu else N
+    if out is None:
+        out = torch.empty((M, cols), dtype=out_dtype or x.dtype, device=x.device)
+    if out.dim() != 2 or out.shape[0] != M or out.shape[1] != cols or (cols > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < cols):
+        raise KernelError(f"gemm_w4: the result is [{M}, {cols}] with contiguous rows, not {list(out.shape)} with strides {list(out.stride())}")
+    out_bf16 = _is_bf16(out)
+    if out_dtype is not None and out.dtype != out_dtype:
+        raise KernelError(f"gemm_w4: out is {out.dtype}, out_dtype {out_dtype}")
+    if out_bf16 and (accumulate or not x_bf16):
+        raise KernelError("gemm_w4: sums are added to float32, and float32 rows do not round down to a bfloat16 result")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != N or not bias.is_contiguous()):
+        raise KernelError(f"gemm_w4: the bias is contiguous float32 [{N}]")
+    _w4_dev(x, w.q, bias, out)
+    if accumulate:
+        residual_written(out)
+    if M == 0:
+        return out
+    epi = _EPI_ACC if accumulate else _EPI_SWIGLU if swiglu else _EPI_RELU2 if act else _EPI_STORE
+    f = _fn("gemm_w4", "fellm_gemm_w4", _GEMM_W4_ARGS)
+    _check(f(_p(x), x_bf16, x.stride(0) if M > 1 else 0, _p(w.q), _p(w.scales), _p(bias), _p(out), out_bf16, out.stride(0) if M > 1 else 0, epi, M,
+             *w._sizes, _stream()), "gemm_w4")
+    return out
+
+
+_GEMM_W4_ARGS = [_c_p, _c_int, _c_ll, _c_p, _c_p, _c_p, _c_p, _c_int, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p]
+
+
 # ------------------------------------------------------------------------------ attention dispatch
 
 _decode_scratch = {}

@@ -1,0 +1,261 @@
+"""Matrices in four bits on the GPU, against plain forms in 64 bits."""
+from __future__ import annotations
+
+import zlib
+
+import pytest
+import torch
+
+import w4_util
+
+DEV = "cuda"
+SIZES = [(16, 64, 32), (1, 1, 32), (17, 33, 32), (40, 200, 64), (129, 130, 128), (1003, 1357, 32), (256, 1024, 64), (272, 2056, 128), (2064, 64, 64),
+         (48, 8200, 128)]
+
+
+def _gen(*seed):
+    return torch.Generator(device=DEV).manual_seed(zlib.crc32(repr(seed).encode()))
+
+
+def _room(x, w, bias, out_bf16):
+    """K products summed in float32 in any order, each addition truncating: at most 1.25 K 2^-23 of the sum of magnitudes (17
+    terms aligned in an MMA of 16 products), half a step of the output's type."""
+    K = x.shape[1]
+    mags = x.double().abs() @ w.abs().T + (bias.double().abs() if bias is not None else 0.0)
+    return 1.25 * K * 2.0 ** -23 * mags, (2.0 ** -8 if out_bf16 else 2.0 ** -24) * 1.001
+
+
+# ---------------------------------------------------------------------------------------------- into the form and out of it
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,group", SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantized_values(N, K, group, dtype):
+    from fellm_b200 import ops
+    g = _gen(N, K, group)
+    held = torch.randn(N, K + 5, generator=g, device=DEV) * torch.exp(3 * torch.randn(N, 1, generator=g, device=DEV))
+    w = held.to(dtype)[:, :K]                                    # (rows that start anywhere)
+    for t in (w, w.contiguous()):
+        got = ops.quantize_w4(t, group)
+        q, s = w4_util.plain_quantize(t, group)
+        want = w4_util.plain_values(q, s, group)
+        assert got.shape == (N, K) and got.group == group
+        assert torch.equal(ops.dequantize_w4(got).double(), want)
+        assert torch.equal(ops.dequantize_w4(got, torch.float32).double(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_halves_ties_and_ends(group):
+    """Elements on and next to every half step, groups of zeros, extremes of both signs and equal, tiny and huge magnitudes."""
+    from fellm_b200 import ops
+    rows = []
+    for unit in (1.0, 2.0 ** -7 * 17, 2.0 ** -60 * 31, 2.0 ** 100):
+        for sign in (1.0, -1.0):
+            base = torch.zeros(group)
+            base[0] = -8 * sign * unit                            # the scale: sign * unit
+            half = torch.arange(-15, 15, dtype=torch.float32) / 2 * unit
+            base[1:31] = half
+            up, down = base.clone(), base.clone()
+            up[1:31] = torch.nextafter(half, torch.full_like(half, float("inf")))
+            down[1:31] = torch.nextafter(half, torch.full_like(half, -float("inf")))
+            rows += [base, up, down]
+    rows += [torch.zeros(group), torch.full((group,), 3.0), torch.full((group,), -3.0), torch.full((group,), 2.0 ** -149), torch.full((group,), 2.0 ** -123),
+             torch.full((group,), 2.0 ** -122), torch.full((group,), 3.4028234663852886e38), -torch.full((group,), 3.4028234663852886e38)]
+    both = torch.zeros(group); both[3], both[9] = 5.0, -5.0
+    rows.append(both)
+    w = torch.stack(rows).to(DEV)
+    w = torch.cat([w, w.flip(0)], 1)
+    q, s = w4_util.plain_quantize(w, group)
+    got = ops.quantize_w4(w, group)
+    assert torch.equal(ops.dequantize_w4(got, torch.float32).double(), w4_util.plain_values(q, s, group))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_group_with_an_element_that_is_not_finite_is_nan(bad, dtype):
+    from fellm_b200 import ops
+    w = torch.randn(40, 200, generator=_gen(1), device=DEV).to(dtype)
+    w[21, 70] = bad
+    out = ops.dequantize_w4(ops.quantize_w4(w, 64))
+    assert out[21, 64:128].isnan().all()
+    out[21, 64:128] = 0
+    assert out.isfinite().all()
+    y = ops.gemm_w4(torch.zeros(2, 200, device=DEV, dtype=torch.bfloat16), ops.quantize_w4(w, 64))
+    assert y[:, 21].isnan().all() and y[:, :21].isfinite().all() and y[:, 22:].isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,group", SIZES)
+def test_packed_levels_come_back(N, K, group):
+    from fellm_b200 import ops
+    levels, scales = w4_util.random_matrix(N, K, group, _gen(N, K), DEV)
+    want = w4_util.plain_values(levels, scales, group)
+    wide = torch.zeros(N, K + 3, dtype=torch.int8, device=DEV)
+    wide[:, :K] = levels
+    for lv, sc in ((levels, scales), (wide[:, :K], scales.float()), (levels, scales.T.contiguous().T)):
+        assert torch.equal(ops.dequantize_w4(ops.pack_w4(lv, sc, group)).double(), want)
+    out = torch.full((N, K + 3), 7.0, device=DEV)
+    ops.dequantize_w4(ops.pack_w4(levels, scales, group), out=out[:, :K])
+    assert torch.equal(out[:, :K].double(), want) and (out[:, K:] == 7).all()
+
+
+@pytest.mark.gpu
+def test_levels_and_scales_that_are_refused():
+    from fellm_b200 import ops
+    from fellm_b200.config.errors import KernelError
+    levels, scales = w4_util.random_matrix(33, 100, 32, _gen(5), DEV)
+    for v in (-9, 8, 127, -128):
+        lv = levels.clone(); lv[32, 99] = v
+        with pytest.raises(KernelError, match="levels"):
+            ops.pack_w4(lv, scales, 32)
+    for v in (33 / 32, 257 / 256, float("inf"), float("nan"), 2.0 ** 125, 2.0 ** -127):
+        sc = scales.float(); sc[32, 3] = v
+        with pytest.raises(KernelError, match="scales"):
+            ops.pack_w4(levels, sc, 32)
+    for v in (0.0, -0.0, 31 * 2.0 ** 120, 2.0 ** -126, -1.9375):
+        sc = scales.float(); sc[32, 3] = v
+        assert torch.equal(ops.dequantize_w4(ops.pack_w4(levels, sc, 32)).double(), w4_util.plain_values(levels, sc, 32))
+
+
+# ------------------------------------------------------------------------------------------------------------ embedding
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,group", SIZES)
+@pytest.mark.parametrize("T", [1, 5, 300])
+def test_embedding_rows(N, K, group, T):
+    from fellm_b200 import ops
+    g = _gen(N, K, T)
+    levels, scales = w4_util.random_matrix(N, K, group, g, DEV)
+    table = ops.pack_w4(levels, scales, group)
+    tokens = torch.randint(0, N, (T,), generator=g, device=DEV, dtype=torch.int32)
+    tokens[-1] = N - 1
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    held = torch.full((T + 1, K), 7.0, device=DEV)
+    ops.embed_rows_w4(tokens, table, held[:T], status, 0.25)
+    assert torch.equal(held[:T].double(), w4_util.plain_values(levels, scales, group)[tokens.long()] * 0.25)
+    assert (held[T:] == 7).all() and int(status) == 0
+    if T > 1:
+        tokens[0], tokens[2] = N, -1
+        ops.embed_rows_w4(tokens, table, held[:T], status, 0.25)
+        assert int(status) == 1 and (held[[0, 2]] == 0).all()
+        assert torch.equal(held[3:T].double(), w4_util.plain_values(levels, scales, group)[tokens[3:].long()] * 0.25)
+
+
+@pytest.mark.gpu
+def test_no_tokens_and_no_rows():
+    from fellm_b200 import ops
+    w = ops.quantize_w4(torch.randn(32, 64, device=DEV), 32)
+    assert ops.embed_rows_w4(torch.zeros(0, dtype=torch.int32, device=DEV), w, torch.empty(0, 64, device=DEV)).shape == (0, 64)
+    assert ops.gemm_w4(torch.zeros(0, 64, device=DEV, dtype=torch.bfloat16), w).shape == (0, 32)
+
+
+# ------------------------------------------------------------------------------------------------------------- products
+
+ROWS = [1, 2, 5, 8, 9, 16, 17, 31, 33, 64, 65, 128, 130, 256, 300, 521]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,group", SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M", ROWS)
+def test_whole_numbers_come_out_exactly(N, K, group, dtype, M):
+    """Sums that are float32 numbers in every order: any element left out, doubled or in a wrong place shows."""
+    from fellm_b200 import ops
+    g = _gen(N, K, M)
+    levels, scales = w4_util.random_matrix(N, K, group, g, DEV)
+    x = w4_util.whole_rows(M, K, dtype, g, DEV)
+    got = ops.gemm_w4(x, ops.pack_w4(levels, scales, group), out_dtype=torch.float32)
+    ops.check_umma_status(DEV)
+    assert torch.equal(got.double(), w4_util.plain_product(x, w4_util.plain_values(levels, scales, group)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,group", [(16, 16, 32), (1008, 136, 32), (272, 1024, 64), (2064, 72, 128), (144, 4104, 128), (16, 333, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M", [1, 3, 8, 16, 23, 48, 100, 129, 400])
+@pytest.mark.parametrize("epi", ["store", "f32", "acc", "relu2", "swiglu"])
+def test_products(N, K, group, dtype, M, epi):
+    """Every epilogue, with a bias, from rows that lie apart into rows that lie apart, beside what has to stay."""
+    from fellm_b200 import ops
+    g = _gen(N, K, M, epi)
+    levels, scales = w4_util.random_matrix(N, K, group, g, DEV)
+    w4, w = ops.pack_w4(levels, scales, group), w4_util.plain_values(levels, scales, group)
+    for shift, pad in ((0, 0), (3, 7), (8, 8)):
+        xs = torch.randn(shift + M * (K + pad), generator=g, device=DEV).to(dtype)
+        x = xs[shift:].view(M, K + pad)[:, :K]
+        bias = torch.randn(N, generator=g, device=DEV) if pad else None
+        out_bf16 = dtype == torch.bfloat16 and epi not in ("f32", "acc")
+        cols = N // 2 if epi == "swiglu" else N
+        held = torch.randn(shift + (M + 1) * (cols + pad), generator=g, device=DEV).to(torch.bfloat16 if out_bf16 else torch.float32)
+        before = held.clone()
+        view = lambda t: t[shift:shift + M * (cols + pad)].view(M, cols + pad)[:, :cols]  # noqa: E731,B023
+        ops.gemm_w4(x, w4, bias, out=view(held), accumulate=epi == "acc", swiglu=epi == "swiglu", act="relu2" if epi == "relu2" else None)
+        ops.check_umma_status(DEV)
+        sums, step = _room(x, w, bias, out_bf16)
+        want = w4_util.plain_product(x, w, bias, epi if epi in ("relu2", "swiglu") else "store")
+        if epi == "acc":
+            want = want + view(before).double()
+            room = sums + 2.0 ** -23 * (view(before).double().abs() + want.abs())
+        elif epi == "relu2":
+            y = w4_util.plain_product(x, w, bias)
+            room = (2 * y.abs() + sums) * sums + (step + 2.0 ** -24) * want.abs()
+        elif epi == "swiglu":
+            y = w4_util.plain_product(x, w, bias).reshape(M, -1, 2, 8)
+            gate, up = y[:, :, 0].reshape(M, -1), y[:, :, 1].reshape(M, -1)
+            es = sums.reshape(M, -1, 2, 8)
+            eg, eu = es[:, :, 0].reshape(M, -1), es[:, :, 1].reshape(M, -1)
+            # |silu'| <= 1.1; the exponential, the sum, the quotient and the product: 8 roundings of float32 at most
+            room = 1.1 * eg * (up.abs() + eu) + gate.abs() * eu + (step + 8 * 2.0 ** -24) * want.abs() + 2.0 ** -126
+        else:
+            room = sums + step * want.abs()
+        off = (view(held).double() - want).abs()
+        assert (off <= room).all(), float((off / room.clamp(min=1e-300)).max())
+        view(held).copy_(view(before))
+        assert torch.equal(held, before), "something beside the product's rows was written"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 4, 20, 200])
+def test_float32_rows_keep_all_their_bits(M):
+    """One element a row, so that nothing is summed: x q s in float32, correctly rounded twice at most."""
+    from fellm_b200 import ops
+    g = _gen(M)
+    levels, scales = w4_util.random_matrix(40, 200, 64, g, DEV)
+    x = torch.zeros(M, 200, device=DEV)
+    at = torch.randint(0, 200, (M, 1), generator=g, device=DEV)
+    x.scatter_(1, at, torch.randn(M, 1, generator=g, device=DEV) * torch.exp(8 * torch.randn(M, 1, generator=g, device=DEV)))
+    got = ops.gemm_w4(x, ops.pack_w4(levels, scales, 64))
+    want = x.double() @ w4_util.plain_values(levels, scales, 64).T
+    assert ((got.double() - want).abs() <= 2.0 ** -22 * want.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M", [2, 33, 300])
+def test_infinities_stay_in_their_rows(dtype, M):
+    from fellm_b200 import ops
+    g = _gen(M, 9)
+    levels, scales = w4_util.random_matrix(144, 136, 32, g, DEV)
+    levels[levels == 0] = 1
+    x = torch.randn(M, 136, generator=g, device=DEV).to(dtype)
+    w4 = ops.pack_w4(levels, scales, 32)
+    clean = ops.gemm_w4(x, w4)
+    x[0, 77], x[1, 5] = float("inf"), float("nan")
+    got = ops.gemm_w4(x, w4)
+    w = w4_util.plain_values(levels, scales, 32)
+    assert torch.equal(got[0].double(), w[:, 77].sign() * float("inf")) and got[1].isnan().all()
+    assert torch.equal(got[2:], clean[2:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 8, 16, 40, 128, 300])
+def test_the_same_bits_every_time(M):
+    from fellm_b200 import ops
+    g = _gen(M, 2)
+    w4 = ops.quantize_w4(torch.randn(1024, 2048, generator=g, device=DEV), 64)
+    x = torch.randn(M, 2048, generator=g, device=DEV).bfloat16()
+    first = ops.gemm_w4(x, w4, out_dtype=torch.float32)
+    for _ in range(5):
+        assert torch.equal(ops.gemm_w4(x, w4, out_dtype=torch.float32), first)
