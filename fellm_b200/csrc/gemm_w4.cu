@@ -27,14 +27,6 @@ __device__ __forceinline__ void mma_bf16(float* d, const unsigned* a, unsigned b
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void split3(float v, unsigned& a, unsigned& b, unsigned& c) {
-  const unsigned u = __float_as_uint(v);
-  a = u & 0xffff0000u;
-  const float r = (u & 0x7f800000u) == 0x7f800000u ? 0.f : v - __uint_as_float(a);        // (an infinity or NaN is the first piece alone)
-  b = __float_as_uint(r) & 0xffff0000u;
-  c = __float_as_uint(r - __uint_as_float(b)) & 0xffff0000u;
-  if ((u & 0x7f800000u) == 0x7f800000u && (u & 0x7fffffu)) a |= 0x400000u;                 // a NaN whose high bits are those of an infinity
-}
 // Eight elements of a row of x from k on as operand registers [part][4].
 template <int XT> struct XParts { static constexpr int N = XT == X_F32 ? 3 : 1; };
 template <int XT>
@@ -59,8 +51,8 @@ __device__ __forceinline__ void load_x8(const GwArgs& a, int m, int k, unsigned 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       unsigned lo[3], hi[3];
-      split3(k + 2 * i < a.w.K ? p[2 * i] : 0.f, lo[0], lo[1], lo[2]);
-      split3(k + 2 * i + 1 < a.w.K ? p[2 * i + 1] : 0.f, hi[0], hi[1], hi[2]);
+      w4_split3(k + 2 * i < a.w.K ? p[2 * i] : 0.f, lo[0], lo[1], lo[2]);
+      w4_split3(k + 2 * i + 1 < a.w.K ? p[2 * i + 1] : 0.f, hi[0], hi[1], hi[2]);
 #pragma unroll
       for (int q = 0; q < P; ++q) b[q][i] = lo[q] >> 16 | hi[q];
     }

@@ -1,0 +1,445 @@
+// y = x W^T of a matrix in four bits (w4.h) for more than a handful of rows, on tcgen05: D[n, t] = sum_k W[n, k] x[t, k], the
+// MMA's 128 rows are weight rows, its 16 to 256 columns are rows of x.
+//
+// The weights become bfloat16 on their way into shared memory: level * scale is a bfloat16 number exactly (w4.h), so this
+// rounds nothing, and K may be summed in one accumulator whatever the groups.  Eight warps take a slab of 16 rows each:
+// 16 bytes a lane from memory, several chunks ahead in registers, are 32 weights, four 16-byte pieces of the tile in the
+// 128-byte swizzle that the MMA reads.  (16 + level + 8) is a shift and an and-or away (the four bits at the top of bfloat16's
+// mantissa at exponent 4), and one fused multiply-add makes (that) * s - 24 s: both 24 s and the result are bfloat16 numbers.
+// x comes by TMA, one thread issues the MMAs, four warps store what is finished: lane = weight row, so a row of the result
+// leaves in pieces of 32 neighbouring columns.
+//
+// Persistent over tiles with two accumulators in tensor memory; where there are too few tiles for the SMs, the K range of a
+// tile is shared out over a cluster of 2, 4 or 8 CTAs, whose sums are put together through distributed shared memory, in
+// rank order, each rank finishing its share of the columns.
+//
+// Roles in a CTA of 448 threads: warp 0 TMA of x (one lane), warp 1 MMA issuer (one lane) and owner of tensor memory, warps
+// 2-9 weights, warps 10-13 epilogue (tensor memory lanes 32 (warp % 4) ..).  Every wait on an mbarrier is bounded: after a
+// second a role records itself in `status` (141 x, 142 MMA, 143 weights, 144 epilogue, 145 accumulator) and all roles fall
+// through to the common exit, where tensor memory is freed.
+#include <cuda.h>
+#include "w4.h"
+
+#define W4U_THREADS 448
+#define W4U_DEQ_WARPS 8
+#define W4U_AHEAD 8                    // chunks a warp holds in registers ahead of the one it unpacks: 4 KB a warp, 32 KB an SM
+#define W4U_SPIN_LIMIT (1u << 26)
+#define W4U_WAIT_NS 1000000000ull
+#define W4U_A_BYTES (128 * 128)        // 128 weight rows x 64 k
+
+enum { EPI_STORE = 0, EPI_ACC = 1, EPI_SWIGLU = 2, EPI_RELU2 = 6 };
+
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(unsigned bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_expect_tx(unsigned bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity) {
+  unsigned ok;
+  asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ unsigned long long global_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, int* status, int code) {
+  if (mbar_try(bar, parity)) return true;
+  const unsigned long long t0 = global_ns();
+  for (unsigned i = 0; i < W4U_SPIN_LIMIT; ++i) {
+    if (mbar_try(bar, parity)) return true;
+    if ((i & 63) == 63 && global_ns() - t0 > W4U_WAIT_NS) break;
+  }
+  if (status) atomicExch(status, code);
+  return false;
+}
+__device__ __forceinline__ void tma_load_2d(unsigned dst, const CUtensorMap* map, int c0, int c1, unsigned bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+// K-major operand tile, rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ unsigned long long umma_desc(unsigned smem_addr) {
+  return (unsigned long long)((smem_addr & 0x3FFFF) >> 4) | (unsigned long long)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// kind::f16: D float32, A and B bfloat16, both K-major.
+__device__ __forceinline__ unsigned umma_idesc(int m, int n) { return 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)(n >> 3) << 17 | (unsigned)(m >> 4) << 24; }
+__device__ __forceinline__ void umma_f16(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit(unsigned bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(unsigned taddr, float* v) {
+  unsigned* r = reinterpret_cast<unsigned*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r)); return r; }
+__device__ __forceinline__ unsigned mapa(unsigned addr, unsigned rank) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void st_cluster(unsigned addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
+struct W4uArgs {
+  W4Ref w;
+  const float* bias; void* out; int* status;
+  long long ldo;
+  int M, epi, out_bf16;
+  int bn;                    // rows of x a tile, a multiple of 16, <= 256
+  int parts;                 // 1: x as it is; 3: every 64 columns of x are three times 64, whose sum they are
+  int stages, splits, tmem_cols;
+};
+
+// The four words of a lane (rows g and g + 8, 16 elements each) -> its pieces of the tile.  Neighbouring even and odd rows
+// are written half a row apart, so that eight lanes of a store meet every bank once.
+__device__ __forceinline__ unsigned w4_value(unsigned word, int r, unsigned s2, unsigned off2) {
+  // nibble r of both halves at bits 3..6: 16 + level + 8 at exponent 4
+  const unsigned moved = r == 0 ? word << 3 : word >> (4 * r - 3);
+  const unsigned b = (moved & 0x00780078u) | 0x41804180u;
+  __nv_bfloat162 v = __hfma2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&s2, *(const __nv_bfloat162*)&off2);
+  return *(unsigned*)&v;
+}
+__device__ __forceinline__ unsigned times_minus_24(unsigned s2) {
+  const unsigned c = 0xc1c0c1c0u;                                    // -24, -24
+  __nv_bfloat162 v = __hmul2(*(const __nv_bfloat162*)&s2, *(const __nv_bfloat162*)&c);
+  return *(unsigned*)&v;
+}
+__device__ __forceinline__ void st_shared_v4(unsigned addr, unsigned a, unsigned b, unsigned c, unsigned d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ void put(const W4uArgs& a, int m, int n, float v) {
+  const size_t o = (size_t)m * a.ldo + n;
+  if (a.out_bf16) ((bf16*)a.out)[o] = __float2bfloat16_rn(v);
+  else ((float*)a.out)[o] = v;
+}
+// 16 finished columns (rows of x from m on, `rows` of them count) of weight row n, a warp's lanes neighbouring weight rows.
+__device__ __forceinline__ void finish16(const W4uArgs& a, float* v, int m, int rows, int n, float bias) {
+  const int lane = threadIdx.x & 31;
+  const bool in = n < a.w.N;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] += bias;
+  if (a.epi == EPI_SWIGLU) {
+    // lanes 8..15 and 24..31 hold what the eight before them are multiplied with: those take the even columns, these the odd
+    const bool gate = !(lane & 8);
+    const int f = ((n & ~15) >> 1) + (lane & 7);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float other = __shfl_xor_sync(0xffffffffu, gate ? v[j + 1] : v[j], 8);
+      const float z = gate ? glu_act(v[j], other, 0.f, 1.f) : glu_act(other, v[j + 1], 0.f, 1.f);
+      const int t = gate ? j : j + 1;
+      if (in && t < rows) put(a, m + t, f, z);
+    }
+    return;
+  }
+  if (!in) return;
+  if (a.epi == EPI_ACC) {
+    float old[16];
+    float* o = (float*)a.out + (size_t)m * a.ldo + n;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) if (j < rows) old[j] = o[(size_t)j * a.ldo];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) if (j < rows) o[(size_t)j * a.ldo] = old[j] + v[j];
+    return;
+  }
+  if (a.epi == EPI_RELU2) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) { v[j] = fmaxf(v[j], 0.f); v[j] *= v[j]; }
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) if (j < rows) put(a, m + j, n, v[j]);
+}
+
+template <bool SPLIT>
+__global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];           // full[8], empty[8], acc_full[2], acc_empty[2]
+  __shared__ unsigned tmem_base_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const unsigned stage_bytes = W4U_A_BYTES + (unsigned)a.bn * 128u;
+  const unsigned full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[8]), accfull0 = smem_u32(&bars[16]), accempty0 = smem_u32(&bars[18]);
+  const int m_tiles = (a.M + a.bn - 1) / a.bn, n_tiles = (a.w.N + 127) / 128, total = m_tiles * n_tiles;
+  const int rank = SPLIT ? (int)cluster_rank() : 0;
+  const int first = SPLIT ? (int)blockIdx.x / a.splits : (int)blockIdx.x, step = SPLIT ? total : (int)gridDim.x;
+  // this CTA's chunks of K
+  const int c_lo = SPLIT ? (int)((long long)a.w.chunks * rank / a.splits) : 0, c_hi = SPLIT ? (int)((long long)a.w.chunks * (rank + 1) / a.splits) : a.w.chunks;
+  const int blocks = (c_hi - c_lo) * a.parts;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) { mbar_init(full0 + 8 * s, 1 + W4U_DEQ_WARPS); mbar_init(empty0 + 8 * s, 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(accfull0 + 8 * b, 1); mbar_init(accempty0 + 8 * b, 4); }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_base_s)), "r"(a.tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const unsigned tmem_base = tmem_base_s, acc_cols = (unsigned)a.tmem_cols / 2;
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      pdl_wait();                                            // x is the output of the kernel before this one
+      unsigned it = 0;
+      bool ok = true;
+      for (int t = first; t < total && ok; t += step) {
+        const int m0 = (t % m_tiles) * a.bn;
+        for (int b = 0; b < blocks; ++b, ++it) {
+          const unsigned s = it % a.stages;
+          if (it >= (unsigned)a.stages && !mbar_wait(empty0 + 8 * s, (it / a.stages - 1) & 1, a.status, 141)) { ok = false; break; }
+          mbar_expect_tx(full0 + 8 * s, (unsigned)a.bn * 128u);
+          tma_load_2d(tiles + s * stage_bytes + W4U_A_BYTES, &map_x, (c_lo * a.parts + b) * W4_CHUNK, m0, full0 + 8 * s);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const unsigned idesc = umma_idesc(128, a.bn);
+      unsigned it = 0, use = 0;
+      bool ok = true;
+      for (int t = first; t < total && ok; t += step, ++use) {
+        const unsigned acc = use & 1, d = tmem_base + acc * acc_cols;
+        if (use >= 2) {
+          ok = mbar_wait(accempty0 + 8 * acc, ((use >> 1) - 1) & 1, a.status, 145);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        }
+        for (int b = 0; b < blocks; ++b, ++it) {
+          const unsigned s = it % a.stages;
+          ok = mbar_wait(full0 + 8 * s, (it / a.stages) & 1, a.status, 142);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          const unsigned sa = tiles + s * stage_bytes;
+          const unsigned long long da = umma_desc(sa), db = umma_desc(sa + W4U_A_BYTES);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_f16(d, da + 2 * k, db + 2 * k, idesc, (b | k) ? 1u : 0u);
+          umma_commit(empty0 + 8 * s);
+        }
+        if (ok) umma_commit(accfull0 + 8 * acc);
+      }
+    }
+  } else if (warp < 2 + W4U_DEQ_WARPS) {
+    // weights: nothing in front of this kernel writes them, so they need not wait for it
+    const int sl = warp - 2, g = lane >> 2, c = lane & 3, slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB;
+    unsigned it = 0;
+    bool ok = true;
+    // byte offsets of the lane's pieces in the tile: row 16 sl + g (and + 8: the same swizzle), pieces c and 4 + c
+    const unsigned row = (unsigned)(16 * sl + g) * 128u, p0 = (unsigned)(c ^ g) * 16u, p1 = (unsigned)((c + 4) ^ g) * 16u;
+    const bool flip = g & 1;
+    for (int t = first; t < total && ok; t += step) {
+      const int slab = (t / m_tiles) * 8 + sl;
+      const bool have = slab < slabs;
+      const uint4* q = a.w.q + ((size_t)(have ? slab : 0) * a.w.chunks + c_lo) * 32 + lane;
+      const unsigned* sc = a.w.s + (size_t)(have ? slab : 0) * a.w.groups * 8 + g;
+      uint4 qv[W4U_AHEAD];
+      unsigned sv[W4U_AHEAD][2];
+      auto fetch = [&](int b, int u) {
+        const int ch = a.parts == 3 ? b / 3 : b;
+        if (b < blocks && have) {
+          qv[u] = __ldg(q + (size_t)ch * 32);
+          const int k = (c_lo + ch) * W4_CHUNK;
+          sv[u][0] = __ldg(sc + (size_t)(k >> a.w.gshift) * 8);
+          sv[u][1] = a.w.gshift == 5 ? __ldg(sc + (size_t)((k + 32) >> 5) * 8) : sv[u][0];
+        } else { qv[u] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u); sv[u][0] = sv[u][1] = 0u; }
+      };
+#pragma unroll
+      for (int u = 0; u < W4U_AHEAD; ++u) fetch(u, u);
+      for (int b0 = 0; b0 < blocks && ok; b0 += W4U_AHEAD) {
+#pragma unroll
+        for (int u = 0; u < W4U_AHEAD; ++u) {
+          if (b0 + u < blocks && ok) {
+            const unsigned s = it % a.stages;
+            if (it >= (unsigned)a.stages) ok = mbar_wait(empty0 + 8 * s, (it / a.stages - 1) & 1, a.status, 143);
+            const unsigned dst = tiles + s * stage_bytes + row;
+            const unsigned w[4] = {qv[u].x, qv[u].y, qv[u].z, qv[u].w};
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {                     // rows g, g + 8
+              const unsigned s2a = __byte_perm(sv[u][0], 0, r ? 0x3232 : 0x1010), s2b = __byte_perm(sv[u][1], 0, r ? 0x3232 : 0x1010);
+              const unsigned oa = times_minus_24(s2a), ob = times_minus_24(s2b);
+              unsigned lo[4], hi[4];
+              lo[0] = w4_value(w[0], r, s2a, oa); lo[1] = w4_value(w[0], r + 2, s2a, oa); lo[2] = w4_value(w[1], r, s2a, oa); lo[3] = w4_value(w[1], r + 2, s2a, oa);
+              hi[0] = w4_value(w[2], r, s2b, ob); hi[1] = w4_value(w[2], r + 2, s2b, ob); hi[2] = w4_value(w[3], r, s2b, ob); hi[3] = w4_value(w[3], r + 2, s2b, ob);
+              const unsigned at = dst + r * 1024u;            // eight rows further on
+              st_shared_v4(at + (flip ? p1 : p0), flip ? hi[0] : lo[0], flip ? hi[1] : lo[1], flip ? hi[2] : lo[2], flip ? hi[3] : lo[3]);
+              st_shared_v4(at + (flip ? p0 : p1), flip ? lo[0] : hi[0], flip ? lo[1] : hi[1], flip ? lo[2] : hi[2], flip ? lo[3] : hi[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full0 + 8 * s);
+            ++it;
+            fetch(b0 + u + W4U_AHEAD, u);
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (!SPLIT && warp >= 2 + W4U_DEQ_WARPS) {
+    pdl_wait();
+    const int quarter = warp & 3;
+    unsigned use = 0;
+    for (int t = first; t < total; t += step, ++use) {
+      const unsigned acc = use & 1;
+      const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + quarter * 32 + lane;
+      const float bias = a.bias && n < a.w.N ? a.bias[n] : 0.f;
+      if (!mbar_wait(accfull0 + 8 * acc, (use >> 1) & 1, a.status, 144)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      for (int c0 = 0; c0 < a.bn && m0 + c0 < a.M; c0 += 16) {
+        float v[16];
+        tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + acc * acc_cols + c0, v);
+        finish16(a, v, m0 + c0, a.M - m0 - c0, n, bias);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(accempty0 + 8 * acc);
+    }
+  }
+  if (SPLIT) {
+    // every rank sends the other ranks' columns of its sums to them: [sending rank][column][128 rows]
+    const int quarter = warp & 3, t = first;
+    const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + quarter * 32 + lane;
+    const int share = ((a.bn / 16 + a.splits - 1) / a.splits) * 16;               // columns a rank finishes, a multiple of 16
+    const unsigned recv = tiles + (unsigned)a.stages * stage_bytes;
+    const bool epi_warp = warp >= 2 + W4U_DEQ_WARPS;
+    bool ok = true;
+    cluster_sync();                                                               // (every rank of the cluster has started: its memory is there)
+    if (epi_warp) {
+      pdl_wait();
+      ok = mbar_wait(accfull0, 0, a.status, 144);
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      for (int c0 = 0; ok && c0 < a.bn && m0 + c0 < a.M; c0 += 16) {
+        const int owner = c0 / share;
+        if (owner == rank) continue;
+        float v[16];
+        tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c0, v);
+        const unsigned dst = mapa(recv + (unsigned)(((rank * share + c0 - owner * share) * 128 + quarter * 32 + lane) * 4), (unsigned)owner);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) st_cluster(dst + j * 512, v[j]);
+      }
+    }
+    cluster_sync();
+    if (epi_warp && ok) {
+      const float bias = a.bias && n < a.w.N ? a.bias[n] : 0.f;
+      const float* mine = reinterpret_cast<const float*>(smem_raw + (recv - smem_u32(smem_raw))) + quarter * 32 + lane;
+      for (int c0 = rank * share; c0 < a.bn && c0 < (rank + 1) * share && m0 + c0 < a.M; c0 += 16) {
+        float own[16], v[16];
+        tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c0, own);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = 0.f;
+        for (int r = 0; r < a.splits; ++r) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] += r == rank ? own[j] : mine[(size_t)(r * share + c0 - rank * share + j) * 128];
+        }
+        finish16(a, v, m0 + c0, a.M - m0 - c0, n, bias);
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(a.tmem_cols) : "memory");
+  }
+}
+
+// Rows that TMA cannot read as they are: bfloat16 rows on no 16-byte boundary or of a K that is no multiple of 8 (copied,
+// zeros up to whole chunks), and float32 rows, every 64 elements of which become three times 64 bfloat16 whose sum they are.
+__global__ void __launch_bounds__(256) w4_rows_kernel(const void* x, int x_bf16, long long ldx, unsigned short* out, int M, int K, int chunks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int width = chunks * W4_CHUNK;
+  const int m = (int)(i / width), k = (int)(i % width);
+  if (m >= M) return;
+  if (x_bf16) {
+    out[i] = k < K ? ((const unsigned short*)x)[(size_t)m * ldx + k] : (unsigned short)0;
+    return;
+  }
+  unsigned a, b, c;
+  w4_split3(k < K ? ((const float*)x)[(size_t)m * ldx + k] : 0.f, a, b, c);
+  unsigned short* o = out + (size_t)m * 3 * width + (size_t)(k / W4_CHUNK) * 3 * W4_CHUNK + k % W4_CHUNK;
+  o[0] = (unsigned short)(c >> 16); o[W4_CHUNK] = (unsigned short)(b >> 16); o[2 * W4_CHUNK] = (unsigned short)(a >> 16);      // (the smallest first)
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (EncodeTiledFn)p;
+  }
+  return fn;
+}
+
+// Bytes of scratch the product wants for rows TMA cannot read (0: it reads x itself).
+FELLM_API long long fellm_gemm_w4_umma_scratch(const void* x, int x_bf16, long long ldx, int M, int K) {
+  if (x_bf16 && K % 8 == 0 && (M == 1 || (ldx % 8 == 0 && ldx >= K)) && ((uintptr_t)x & 15) == 0) return 0;
+  return (long long)M * ceil_div(K, W4_CHUNK) * W4_CHUNK * (x_bf16 ? 2 : 6);
+}
+
+FELLM_API int fellm_gemm_w4_umma(const void* x, int x_bf16, long long ldx, const void* q, const void* s, const float* bias, void* out, int out_bf16,
+                                 long long ldo, int epi, int M, int N, int K, int chunks, int groups, int gshift, void* scratch, int* status,
+                                 cudaStream_t stream) {
+  if (M <= 0) return 0;
+  if (!x || !q || !s || !out || !status) return FELLM_ERR_ARG;
+  if (N < 1 || K < 1 || gshift < 5 || gshift > 7 || chunks != ceil_div(K, W4_CHUNK)) return FELLM_ERR_SIZE;
+  if (groups != (int)(((long long)chunks * W4_CHUNK + (1 << gshift) - 1) >> gshift)) return FELLM_ERR_SIZE;
+  if (epi != EPI_STORE && epi != EPI_ACC && epi != EPI_SWIGLU && epi != EPI_RELU2) return FELLM_ERR_ARG;
+  if (epi == EPI_SWIGLU && N % W4_SLAB) return FELLM_ERR_SIZE;
+  const bool copied = fellm_gemm_w4_umma_scratch(x, x_bf16, ldx, M, K) != 0;
+  const int parts = x_bf16 ? 1 : 3;
+  if (copied) {
+    if (!scratch || ((uintptr_t)scratch & 15)) return FELLM_ERR_ARG;
+    const long long n = (long long)M * chunks * W4_CHUNK, b = (n + 255) / 256;
+    if (b >= (1ll << 31)) return FELLM_ERR_SIZE;
+    if (int e = launch_k_class(launch_class_for_rows(M, 0), w4_rows_kernel, dim3((unsigned)b, 1, 1), dim3(256, 1, 1), 0, stream, 1, x, x_bf16, ldx,
+                               (unsigned short*)scratch, M, K, chunks)) return e;
+    x = scratch; ldx = (long long)parts * chunks * W4_CHUNK;
+  }
+  W4uArgs a = {{(const uint4*)q, (const unsigned*)s, N, K, chunks, groups, gshift}, bias, out, status, ldo, M, epi, out_bf16};
+  a.parts = parts;
+  const int n_sm = fellm_sm_count(), n_tiles = ceil_div(N, 128);
+  // columns of a tile: all rows in one where they fit, else as few tiles as 256 allow, equally wide
+  const int wide = n_tiles * ceil_div(M, 256) >= n_sm ? 256 : 128;
+  a.bn = ceil_div(ceil_div(M, ceil_div(M, wide)), 16) * 16;
+  const int total = n_tiles * ceil_div(M, a.bn);
+  a.splits = 1;
+  while (a.splits < 8 && total * a.splits * 2 <= n_sm && chunks >= a.splits * 2 * 4 && a.bn <= 128) a.splits *= 2;
+  const int stage = W4U_A_BYTES + a.bn * 128;
+  const int share = ceil_div(a.bn / 16, a.splits) * 16, recv = a.splits > 1 ? a.splits * share * 512 : 0;
+  a.stages = (220 * 1024 - recv) / stage;
+  if (a.stages > 8) a.stages = 8;
+  a.tmem_cols = 32;
+  while (a.tmem_cols < 2 * a.bn) a.tmem_cols *= 2;
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return FELLM_ERR_ARG;
+  CUtensorMap map;
+  cuuint64_t dims[2] = {(cuuint64_t)(copied ? parts * chunks * W4_CHUNK : K), (cuuint64_t)M};
+  cuuint64_t strides[1] = {(cuuint64_t)(M == 1 && !copied ? (long long)ceil_div(K, 8) * 8 : ldx) * 2};
+  cuuint32_t box[2] = {W4_CHUNK, (cuuint32_t)a.bn}, estr[2] = {1, 1};
+  const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return 1000 + (int)r;
+  const size_t smem = (size_t)a.stages * stage + recv + 1024;
+  auto kern = a.splits > 1 ? gemm_w4_umma_kernel<true> : gemm_w4_umma_kernel<false>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
+  return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
+}

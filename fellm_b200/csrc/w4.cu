@@ -12,11 +12,12 @@ __device__ __forceinline__ float round5(float a) {
 
 // A group's scale from its largest and smallest element: an eighth of the largest magnitude, in five significant bits,
 // negative where that magnitude is a positive element's (so that the extreme is level -8, not the missing +8).  Below the
-// normal numbers: 0, the group is zeros.  Not above 31 * 2^120: 8 s has to stay finite.  NaN where an element is not finite.
+// normal numbers: 0, the group is zeros.  Not above 31 * 2^118: 24 s has to stay
+// finite, with which the weights are made bfloat16 numbers.  NaN where an element is not finite.
 __device__ __forceinline__ float group_scale(float hi, float lo, bool finite) {
   if (!finite) return __uint_as_float(0x7fc00000u);
   const float a = fmaxf(hi, -lo) * 0.125f;
-  float s = fminf(round5(a), __uint_as_float(0x7df80000u));
+  float s = fminf(round5(a), __uint_as_float(0x7cf80000u));
   if (s < 1.1754943508222875e-38f) s = 0.f;
   return hi > -lo ? -s : s;
 }
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(W4_THREADS) quantize_w4_kernel(const T* w, lon
 }
 
 // Levels and scales that exist already -> the layout.  bad: 1 a level outside -8..7, 2 a scale that is not finite, has more
-// than five significant bits or is so large that 8 s is not finite.
+// than five significant bits or is above 31 * 2^118 or not a normal number.
 __global__ void __launch_bounds__(W4_THREADS) pack_w4_kernel(const signed char* lv, long long ldl, const bf16* sc, long long lds, W4Out o, int groups_in, int* bad) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const long long unit = (long long)blockIdx.x * (W4_THREADS / 32) + (threadIdx.x >> 5);
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(W4_THREADS) pack_w4_kernel(const signed char* 
       const int n = slab * W4_SLAB + g + 8 * r;
       half[r] = n < o.N && grp < groups_in ? (unsigned)*(const unsigned short*)(sc + (size_t)n * lds + grp) : 0u;
       const unsigned mag = half[r] & 0x7fffu;
-      odd = odd || (half[r] & 7u) || mag > 0x7df8u || (mag && mag < 0x80u);
+      odd = odd || (half[r] & 7u) || mag > 0x7cf8u || (mag && mag < 0x80u);
     }
     if (odd) atomicOr(bad, 2);
     o.s[((size_t)slab * o.groups + grp) * 8 + g] = half[0] | half[1] << 16;

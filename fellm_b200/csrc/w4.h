@@ -37,3 +37,13 @@ __device__ __forceinline__ unsigned w4_pair(unsigned word, int r) {
 }
 __device__ __forceinline__ float w4_scale_lo(unsigned s) { return __uint_as_float(s << 16); }
 __device__ __forceinline__ float w4_scale_hi(unsigned s) { return __uint_as_float(s & 0xffff0000u); }
+// A float32 number as three bfloat16 ones (in the upper halves), a + b + c = v exactly: 8 bits of its mantissa each (as far
+// down as bfloat16 reaches, 2^-133).  An infinity or NaN is the first piece alone.
+__device__ __forceinline__ void w4_split3(float v, unsigned& a, unsigned& b, unsigned& c) {
+  const unsigned u = __float_as_uint(v);
+  a = u & 0xffff0000u;
+  const float r = (u & 0x7f800000u) == 0x7f800000u ? 0.f : v - __uint_as_float(a);
+  b = __float_as_uint(r) & 0xffff0000u;
+  c = __float_as_uint(r - __uint_as_float(b)) & 0xffff0000u;
+  if ((u & 0x7f800000u) == 0x7f800000u && (u & 0x7fffffu)) a |= 0x400000u;                 // a NaN whose high bits are those of an infinity
+}

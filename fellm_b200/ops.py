@@ -1594,7 +1594,8 @@ def check_umma_status(device):
                     "the tcgen05 prefill attention" if 311 <= code <= 317 else
                     "the tcgen05 product of few rows" if 111 <= code <= 113 else
                     "the tcgen05 product on CTA pairs" if 121 <= code <= 124 else
-                    "the tcgen05 product with K over two CTAs" if 131 <= code <= 134 else "the tcgen05 product")
+                    "the tcgen05 product with K over two CTAs" if 131 <= code <= 134 else
+                    "the tcgen05 product of four-bit weights" if 141 <= code <= 145 else "the tcgen05 product")
             raise KernelError(f"{what} gave up waiting on a barrier (role {code})")
 
 
@@ -1977,6 +1978,7 @@ def interleave_gate_up(gate, up):
 # ------------------------------------------------------------------------------ matrices in four bits
 
 W4_GROUPS = (32, 64, 128)
+W4_FEW_ROWS = 16                         # up to so many rows: mma.sync, a warp a slab of 16 weight rows; more: tcgen05
 
 
 class W4:
@@ -2140,6 +2142,15 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
     if M == 0:
         return out
     epi = _EPI_ACC if accumulate else _EPI_SWIGLU if swiglu else _EPI_RELU2 if act else _EPI_STORE
+    if M > W4_FEW_ROWS:
+        need = _fn("gemm_w4_umma", "fellm_gemm_w4_umma_scratch", [_c_p, _c_int, _c_ll, _c_int, _c_int])
+        need.restype = _c_ll
+        room = need(_p(x), x_bf16, x.stride(0), M, K)
+        scratch = torch.empty(room, dtype=torch.uint8, device=x.device) if room else None
+        f = _fn("gemm_w4_umma", "fellm_gemm_w4_umma", _GEMM_W4_ARGS[:-1] + [_c_p, _c_p, _c_p])
+        _check(f(_p(x), x_bf16, x.stride(0), _p(w.q), _p(w.scales), _p(bias), _p(out), out_bf16, out.stride(0), epi, M, *w._sizes, _p(scratch),
+                 _p(umma_status(x.device)), _stream()), "gemm_w4_umma")
+        return out
     f = _fn("gemm_w4", "fellm_gemm_w4", _GEMM_W4_ARGS)
     _check(f(_p(x), x_bf16, x.stride(0) if M > 1 else 0, _p(w.q), _p(w.scales), _p(bias), _p(out), out_bf16, out.stride(0) if M > 1 else 0, epi, M,
              *w._sizes, _stream()), "gemm_w4")

@@ -8,7 +8,7 @@ def plain_scale(piece):
     """The scale of one group [N, <= G] (float64), [N, 1]."""
     big = piece.abs().amax(1, keepdim=True)
     mant, expo = torch.frexp(big / 8)
-    s = torch.ldexp(torch.round(mant * 32), expo - 5).clamp(max=31 * 2.0 ** 120)
+    s = torch.ldexp(torch.round(mant * 32), expo - 5).clamp(max=31 * 2.0 ** 118)
     s = torch.where(s < 2.0 ** -126, torch.zeros_like(s), s)
     return torch.where(piece.amax(1, keepdim=True) > -piece.amin(1, keepdim=True), -s, s)
 
