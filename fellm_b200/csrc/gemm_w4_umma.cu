@@ -13,16 +13,20 @@
 // tile is shared out over a cluster of 2, 4 or 8 CTAs, whose sums are put together through distributed shared memory, in
 // rank order, each rank finishing its share of the columns.
 //
-// Roles in a CTA of 448 threads: warp 0 TMA of x (one lane), warp 1 MMA issuer (one lane) and owner of tensor memory, warps
-// 2-9 weights, warps 10-13 epilogue (tensor memory lanes 32 (warp % 4) ..).  Every wait on an mbarrier is bounded: after a
+// Roles in a CTA: warp 0 TMA of x (one lane), warp 1 MMA issuer (one lane) and owner of tensor memory, warps 2-17 weights
+// (two sets of eight), warps 18-21 epilogue (tensor memory lanes 32 (warp % 4) ..).  Every wait on an mbarrier is bounded: after a
 // second a role records itself in `status` (141 x, 142 MMA, 143 weights, 144 epilogue, 145 accumulator) and all roles fall
 // through to the common exit, where tensor memory is freed.
 #include <cuda.h>
 #include "w4.h"
 
-#define W4U_THREADS 448
-#define W4U_DEQ_WARPS 8
-#define W4U_AHEAD 8                    // chunks a warp holds in registers ahead of the one it unpacks: 4 KB a warp, 32 KB an SM
+#ifndef W4U_SETS
+#define W4U_SETS 2                     // sets of eight warps that make weights, each every other stage
+#endif
+#define W4U_THREADS (32 * (2 + 8 * W4U_SETS + 4))
+#ifndef W4U_AHEAD
+#define W4U_AHEAD 4                    // chunks a warp holds in registers ahead of the one it unpacks
+#endif
 #define W4U_SPIN_LIMIT (1u << 26)
 #define W4U_WAIT_NS 1000000000ull
 #define W4U_A_BYTES (128 * 128)        // 128 weight rows x 64 k
@@ -160,6 +164,14 @@ __device__ __forceinline__ void finish16(const W4uArgs& a, float* v, int m, int 
   for (int j = 0; j < 16; ++j) if (j < rows) put(a, m + j, n, v[j]);
 }
 
+// A role's place in the ring of stages, and how often it has been round (its parity).  A role that fills stages waits for the
+// parity before its own: of a new barrier that is complete.
+struct Ring {
+  unsigned stage = 0, parity = 0;
+  __device__ __forceinline__ void add(unsigned n, unsigned stages) { stage += n; if (stage >= stages) { stage -= stages; parity ^= 1u; } }        // n <= stages
+  __device__ __forceinline__ void add_many(unsigned n, unsigned stages) { stage += n; parity ^= (stage / stages) & 1u; stage %= stages; }
+};
+
 template <bool SPLIT>
 __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   const int blocks = (c_hi - c_lo) * a.parts;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; ++s) { mbar_init(full0 + 8 * s, 1 + W4U_DEQ_WARPS); mbar_init(empty0 + 8 * s, 1); }
+    for (int s = 0; s < a.stages; ++s) { mbar_init(full0 + 8 * s, 1 + 8); mbar_init(empty0 + 8 * s, 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(accfull0 + 8 * b, 1); mbar_init(accempty0 + 8 * b, 4); }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -194,13 +206,13 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   if (warp == 0) {
     if (lane == 0) {
       pdl_wait();                                            // x is the output of the kernel before this one
-      unsigned it = 0;
+      Ring ring;
       bool ok = true;
       for (int t = first; t < total && ok; t += step) {
         const int m0 = (t % m_tiles) * a.bn;
-        for (int b = 0; b < blocks; ++b, ++it) {
-          const unsigned s = it % a.stages;
-          if (it >= (unsigned)a.stages && !mbar_wait(empty0 + 8 * s, (it / a.stages - 1) & 1, a.status, 141)) { ok = false; break; }
+        for (int b = 0; b < blocks; ++b, ring.add(1, a.stages)) {
+          const unsigned s = ring.stage;
+          if (!mbar_wait(empty0 + 8 * s, ring.parity ^ 1u, a.status, 141)) { ok = false; break; }
           mbar_expect_tx(full0 + 8 * s, (unsigned)a.bn * 128u);
           tma_load_2d(tiles + s * stage_bytes + W4U_A_BYTES, &map_x, (c_lo * a.parts + b) * W4_CHUNK, m0, full0 + 8 * s);
         }
@@ -209,7 +221,8 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   } else if (warp == 1) {
     if (lane == 0) {
       const unsigned idesc = umma_idesc(128, a.bn);
-      unsigned it = 0, use = 0;
+      unsigned use = 0;
+      Ring ring;
       bool ok = true;
       for (int t = first; t < total && ok; t += step, ++use) {
         const unsigned acc = use & 1, d = tmem_base + acc * acc_cols;
@@ -218,9 +231,9 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         }
-        for (int b = 0; b < blocks; ++b, ++it) {
-          const unsigned s = it % a.stages;
-          ok = mbar_wait(full0 + 8 * s, (it / a.stages) & 1, a.status, 142);
+        for (int b = 0; b < blocks; ++b, ring.add(1, a.stages)) {
+          const unsigned s = ring.stage;
+          ok = mbar_wait(full0 + 8 * s, ring.parity, a.status, 142);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           const unsigned sa = tiles + s * stage_bytes;
@@ -232,14 +245,17 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         if (ok) umma_commit(accfull0 + 8 * acc);
       }
     }
-  } else if (warp < 2 + W4U_DEQ_WARPS) {
+  } else if (warp < 2 + 8 * W4U_SETS) {
     // weights: nothing in front of this kernel writes them, so they need not wait for it
-    const int sl = warp - 2, g = lane >> 2, c = lane & 3, slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB;
-    unsigned it = 0;
+    const int sl = (warp - 2) & 7, set = (warp - 2) >> 3, g = lane >> 2, c = lane & 3, slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB;
+    Ring base;
     bool ok = true;
-    // byte offsets of the lane's pieces in the tile: row 16 sl + g (and + 8: the same swizzle), pieces c and 4 + c
-    const unsigned row = (unsigned)(16 * sl + g) * 128u, p0 = (unsigned)(c ^ g) * 16u, p1 = (unsigned)((c + 4) ^ g) * 16u;
+    // where the lane's pieces lie in the tile: row 16 sl + g (and + 8: the same swizzle), pieces c and 4 + c of its eight.  Odd rows
+    // are written the far piece first, so that eight lanes of a store meet every bank once.
     const bool flip = g & 1;
+    const unsigned row = (unsigned)(16 * sl + g) * 128u, near = (unsigned)(c ^ g) * 16u, far = (unsigned)((c + 4) ^ g) * 16u;
+    const unsigned p0 = row + (flip ? far : near), p1 = row + (flip ? near : far);
+    const bool two_scales = a.w.gshift == 5;
     for (int t = first; t < total && ok; t += step) {
       const int slab = (t / m_tiles) * 8 + sl;
       const bool have = slab < slabs;
@@ -247,48 +263,56 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       const unsigned* sc = a.w.s + (size_t)(have ? slab : 0) * a.w.groups * 8 + g;
       uint4 qv[W4U_AHEAD];
       unsigned sv[W4U_AHEAD][2];
-      auto fetch = [&](int b, int u) {
-        const int ch = a.parts == 3 ? b / 3 : b;
-        if (b < blocks && have) {
-          qv[u] = __ldg(q + (size_t)ch * 32);
-          const int k = (c_lo + ch) * W4_CHUNK;
-          sv[u][0] = __ldg(sc + (size_t)(k >> a.w.gshift) * 8);
-          sv[u][1] = a.w.gshift == 5 ? __ldg(sc + (size_t)((k + 32) >> 5) * 8) : sv[u][0];
-        } else { qv[u] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u); sv[u][0] = sv[u][1] = 0u; }
+      // This set's blocks of the tile: set, set + SETS, ...; `ahead`: the next one to be fetched.  Always a load, the last
+      // chunk's again behind the end: a register that is loaded or set would have to wait for the load at once.
+      int ahead = set;
+      auto fetch = [&](int u) {
+        const int ch = min(a.parts == 1 ? ahead : ahead / 3, c_hi - c_lo - 1);
+        qv[u] = __ldg(q + (size_t)(unsigned)ch * 32);
+        const unsigned* at = sc + (size_t)((unsigned)((c_lo + ch) * W4_CHUNK) >> a.w.gshift) * 8;
+        sv[u][0] = __ldg(at);
+        sv[u][1] = __ldg(at + (two_scales ? 8 : 0));
+        ahead += W4U_SETS;
       };
+      Ring ring = base;
+      ring.add(set, a.stages);
 #pragma unroll
-      for (int u = 0; u < W4U_AHEAD; ++u) fetch(u, u);
-      for (int b0 = 0; b0 < blocks && ok; b0 += W4U_AHEAD) {
+      for (int u = 0; u < W4U_AHEAD; ++u) fetch(u);
+      for (int b0 = set; b0 < blocks && ok; b0 += W4U_SETS * W4U_AHEAD) {
 #pragma unroll
         for (int u = 0; u < W4U_AHEAD; ++u) {
-          if (b0 + u < blocks && ok) {
-            const unsigned s = it % a.stages;
-            if (it >= (unsigned)a.stages) ok = mbar_wait(empty0 + 8 * s, (it / a.stages - 1) & 1, a.status, 143);
-            const unsigned dst = tiles + s * stage_bytes + row;
-            const unsigned w[4] = {qv[u].x, qv[u].y, qv[u].z, qv[u].w};
+          if (b0 + u * W4U_SETS < blocks && ok) {
+            const unsigned sa = have ? sv[u][0] : 0u, sb = have ? sv[u][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
+            const unsigned w[4] = {flip ? qv[u].z : qv[u].x, flip ? qv[u].w : qv[u].y, flip ? qv[u].x : qv[u].z, flip ? qv[u].y : qv[u].w};
+            unsigned v[2][2][4];                              // [row g, g + 8][piece][..]
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {                     // rows g, g + 8
-              const unsigned s2a = __byte_perm(sv[u][0], 0, r ? 0x3232 : 0x1010), s2b = __byte_perm(sv[u][1], 0, r ? 0x3232 : 0x1010);
-              const unsigned oa = times_minus_24(s2a), ob = times_minus_24(s2b);
-              unsigned lo[4], hi[4];
-              lo[0] = w4_value(w[0], r, s2a, oa); lo[1] = w4_value(w[0], r + 2, s2a, oa); lo[2] = w4_value(w[1], r, s2a, oa); lo[3] = w4_value(w[1], r + 2, s2a, oa);
-              hi[0] = w4_value(w[2], r, s2b, ob); hi[1] = w4_value(w[2], r + 2, s2b, ob); hi[2] = w4_value(w[3], r, s2b, ob); hi[3] = w4_value(w[3], r + 2, s2b, ob);
-              const unsigned at = dst + r * 1024u;            // eight rows further on
-              st_shared_v4(at + (flip ? p1 : p0), flip ? hi[0] : lo[0], flip ? hi[1] : lo[1], flip ? hi[2] : lo[2], flip ? hi[3] : lo[3]);
-              st_shared_v4(at + (flip ? p0 : p1), flip ? lo[0] : hi[0], flip ? lo[1] : hi[1], flip ? lo[2] : hi[2], flip ? lo[3] : hi[3]);
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
+                v[r][h][0] = w4_value(w[2 * h], r, s2, off); v[r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
+                v[r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
+              }
+            fetch(u);
+            ok = mbar_wait(empty0 + 8 * ring.stage, ring.parity ^ 1u, a.status, 143);
+            const unsigned dst = tiles + ring.stage * stage_bytes;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {                     // (row g + 8: eight rows of 128 bytes further on)
+              st_shared_v4(dst + p0 + r * 1024u, v[r][0][0], v[r][0][1], v[r][0][2], v[r][0][3]);
+              st_shared_v4(dst + p1 + r * 1024u, v[r][1][0], v[r][1][1], v[r][1][2], v[r][1][3]);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(full0 + 8 * s);
-            ++it;
-            fetch(b0 + u + W4U_AHEAD, u);
+            if (lane == 0) mbar_arrive(full0 + 8 * ring.stage);
+            ring.add(W4U_SETS, a.stages);
           }
         }
       }
+      base.add_many(blocks, a.stages);
     }
   }
   __syncwarp();
-  if (!SPLIT && warp >= 2 + W4U_DEQ_WARPS) {
+  if (!SPLIT && warp >= 2 + 8 * W4U_SETS) {
     pdl_wait();
     const int quarter = warp & 3;
     unsigned use = 0;
@@ -314,7 +338,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + quarter * 32 + lane;
     const int share = ((a.bn / 16 + a.splits - 1) / a.splits) * 16;               // columns a rank finishes, a multiple of 16
     const unsigned recv = tiles + (unsigned)a.stages * stage_bytes;
-    const bool epi_warp = warp >= 2 + W4U_DEQ_WARPS;
+    const bool epi_warp = warp >= 2 + 8 * W4U_SETS;
     bool ok = true;
     cluster_sync();                                                               // (every rank of the cluster has started: its memory is there)
     if (epi_warp) {
