@@ -13,22 +13,16 @@
 // tile is shared out over a cluster of 2, 4 or 8 CTAs, whose sums are put together through distributed shared memory, in
 // rank order, each rank finishing its share of the columns.
 //
-// Roles in a CTA: warp 0 TMA of x (one lane), warp 1 MMA issuer (one lane) and owner of tensor memory, warps 2-17 weights
-// (two sets of eight), warps 18-21 epilogue (tensor memory lanes 32 (warp % 4) ..).  Every wait on an mbarrier is bounded: after a
+// Roles in a CTA: warp 0 TMA of x (one lane), warp 1 MMA issuer (one lane) and owner of tensor memory, then one or two sets of
+// eight warps for weights, the last four warps epilogue (tensor memory lanes 32 (warp % 4) ..).  Every wait on an mbarrier is bounded: after a
 // second a role records itself in `status` (141 x, 142 MMA, 143 weights, 144 epilogue, 145 accumulator) and all roles fall
 // through to the common exit, where tensor memory is freed.
 #include <cuda.h>
 #include "w4.h"
 
-#ifndef W4U_SETS
-#define W4U_SETS 2                     // sets of eight warps that make weights, each every other stage
-#endif
-#define W4U_THREADS (32 * (2 + 8 * W4U_SETS + 4))
-#ifndef W4U_AHEAD
-#define W4U_AHEAD 4                    // chunks a warp holds in registers ahead of the one it unpacks
-#endif
+// SETS: sets of eight warps that make weights, each every SETS-th stage
+constexpr int w4u_threads(int sets) { return 32 * (2 + 8 * sets + 4); }
 #define W4U_SPIN_LIMIT (1u << 26)
-#define W4U_WAIT_NS 1000000000ull
 #define W4U_A_BYTES (128 * 128)        // 128 weight rows x 64 k
 
 enum { EPI_STORE = 0, EPI_ACC = 1, EPI_SWIGLU = 2, EPI_RELU2 = 6 };
@@ -44,34 +38,58 @@ __device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity) {
   asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ unsigned long long global_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
-  return t;
-}
+// Bounded wait: false (and *status set) after some 2^31 cycles, a second.  (By the SM's own clock: reading the global timer
+// takes longer than most waits here.)
 __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, int* status, int code) {
   if (mbar_try(bar, parity)) return true;
-  const unsigned long long t0 = global_ns();
+  const long long t0 = clock64();
   for (unsigned i = 0; i < W4U_SPIN_LIMIT; ++i) {
     if (mbar_try(bar, parity)) return true;
-    if ((i & 63) == 63 && global_ns() - t0 > W4U_WAIT_NS) break;
+    if ((i & 63) == 63 && clock64() - t0 > (1ll << 31)) break;
   }
   if (status) atomicExch(status, code);
   return false;
+}
+// The epilogue's wait for a finished accumulator, most of a tile's time: one warp asks, now and then (four that ask all the time
+// took a third of the issue slots), the others sleep at a barrier.  False for all four if it ran out.
+__device__ __forceinline__ bool epilogue_wait(unsigned bar, unsigned parity, int* status, int* gave_up, bool asks) {
+  if (asks && !mbar_try(bar, parity)) {
+    const long long t0 = clock64();
+    bool ok = false;
+    for (unsigned i = 0; i < W4U_SPIN_LIMIT && !ok; ++i) {
+      __nanosleep(64);
+      ok = mbar_try(bar, parity);
+      if (clock64() - t0 > (1ll << 31)) break;
+    }
+    if (!ok) { *gave_up = 1; if (status) atomicExch(status, 144); }
+  }
+  asm volatile("bar.sync 1, 128;\n" ::: "memory");
+  return *(volatile int*)gave_up == 0;
 }
 __device__ __forceinline__ void tma_load_2d(unsigned dst, const CUtensorMap* map, int c0, int c1, unsigned bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
                ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
 }
-// K-major operand tile, rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ unsigned long long umma_desc(unsigned smem_addr) {
-  return (unsigned long long)((smem_addr & 0x3FFFF) >> 4) | (unsigned long long)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
+// K-major operand tile, rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart: the descriptor's upper word, and its
+// lower one from the address (a further piece of 32 bytes of K is 2 more).
+#define W4U_DESC_HI ((1024u >> 4) | 1u << 14 | 2u << 29)
+__device__ __forceinline__ unsigned umma_desc_lo(unsigned smem_addr) { return (smem_addr & 0x3FFFF) >> 4; }
 // kind::f16: D float32, A and B bfloat16, both K-major.
 __device__ __forceinline__ unsigned umma_idesc(int m, int n) { return 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)(n >> 3) << 17 | (unsigned)(m >> 4) << 24; }
-__device__ __forceinline__ void umma_f16(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// The four MMAs of a stage's 64 k.
+__device__ __forceinline__ void umma_stage(unsigned d, unsigned a_lo, unsigned b_lo, unsigned idesc, unsigned accumulate) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    asm volatile("{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.b32 p, %4, 0;\nmov.b64 da, {%1, %5};\nmov.b64 db, {%2, %5};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n"
+                 ::"r"(d), "r"(a_lo + 2 * k), "r"(b_lo + 2 * k), "r"(idesc), "r"(k ? 1u : accumulate), "r"(W4U_DESC_HI) : "memory");
+}
+// One lane of a converged warp, the same one every time.  (A role's loop runs in the whole warp, so that its counters and
+// descriptors are uniform; a loop inside `if (lane == 0)` took some 800 cycles a stage for its scalar arithmetic.)
+__device__ __forceinline__ bool elect_one() {
+  unsigned p;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
 }
 __device__ __forceinline__ void umma_commit(unsigned bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
@@ -94,13 +112,13 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
+// PARTS 1: x as it is; 3: every 64 columns of x are three times 64, whose sum they are.
 struct W4uArgs {
   W4Ref w;
   const float* bias; void* out; int* status;
   long long ldo;
   int M, epi, out_bf16;
   int bn;                    // rows of x a tile, a multiple of 16, <= 256
-  int parts;                 // 1: x as it is; 3: every 64 columns of x are three times 64, whose sum they are
   int stages, splits, tmem_cols;
 };
 
@@ -172,11 +190,13 @@ struct Ring {
   __device__ __forceinline__ void add_many(unsigned n, unsigned stages) { stage += n; parity ^= (stage / stages) & 1u; stage %= stages; }
 };
 
-template <bool SPLIT>
-__global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
+template <bool SPLIT, int PARTS, int SETS>
+__global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
+  constexpr int AHEAD = 4;               // chunks a warp holds in registers ahead of the one it unpacks
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];           // full[8], empty[8], acc_full[2], acc_empty[2]
   __shared__ unsigned tmem_base_s;
+  __shared__ int gave_up;                // the epilogue has
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const unsigned stage_bytes = W4U_A_BYTES + (unsigned)a.bn * 128u;
@@ -186,9 +206,10 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   const int first = SPLIT ? (int)blockIdx.x / a.splits : (int)blockIdx.x, step = SPLIT ? total : (int)gridDim.x;
   // this CTA's chunks of K
   const int c_lo = SPLIT ? (int)((long long)a.w.chunks * rank / a.splits) : 0, c_hi = SPLIT ? (int)((long long)a.w.chunks * (rank + 1) / a.splits) : a.w.chunks;
-  const int blocks = (c_hi - c_lo) * a.parts;
+  const int blocks = (c_hi - c_lo) * PARTS;
 
   if (threadIdx.x == 0) {
+    gave_up = 0;
     for (int s = 0; s < a.stages; ++s) { mbar_init(full0 + 8 * s, 1 + 8); mbar_init(empty0 + 8 * s, 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(accfull0 + 8 * b, 1); mbar_init(accempty0 + 8 * b, 4); }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -200,119 +221,115 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-  const unsigned tmem_base = tmem_base_s, acc_cols = (unsigned)a.tmem_cols / 2;
+  const unsigned tmem_base = tmem_base_s, acc_cols = SPLIT ? 0u : (unsigned)a.tmem_cols / 2;
   pdl_launch_dependents();
 
   if (warp == 0) {
-    if (lane == 0) {
-      pdl_wait();                                            // x is the output of the kernel before this one
-      Ring ring;
-      bool ok = true;
-      for (int t = first; t < total && ok; t += step) {
-        const int m0 = (t % m_tiles) * a.bn;
-        for (int b = 0; b < blocks; ++b, ring.add(1, a.stages)) {
-          const unsigned s = ring.stage;
-          if (!mbar_wait(empty0 + 8 * s, ring.parity ^ 1u, a.status, 141)) { ok = false; break; }
-          mbar_expect_tx(full0 + 8 * s, (unsigned)a.bn * 128u);
-          tma_load_2d(tiles + s * stage_bytes + W4U_A_BYTES, &map_x, (c_lo * a.parts + b) * W4_CHUNK, m0, full0 + 8 * s);
+    pdl_wait();                                              // x is the output of the kernel before this one
+    Ring ring;
+    bool ok = true;
+    for (int t = first; t < total && ok; t += step) {
+      const int m0 = (t % m_tiles) * a.bn;
+      for (int b = 0; b < blocks && ok; ++b) {
+        ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * ring.stage, ring.parity ^ 1u, a.status, 141));
+        if (ok && elect_one()) {
+          mbar_expect_tx(full0 + 8 * ring.stage, (unsigned)a.bn * 128u);
+          tma_load_2d(tiles + ring.stage * stage_bytes + W4U_A_BYTES, &map_x, (c_lo * PARTS + b) * W4_CHUNK, m0, full0 + 8 * ring.stage);
         }
+        __syncwarp();
+        ring.add(1, a.stages);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const unsigned idesc = umma_idesc(128, a.bn);
-      unsigned use = 0;
-      Ring ring;
-      bool ok = true;
-      for (int t = first; t < total && ok; t += step, ++use) {
-        const unsigned acc = use & 1, d = tmem_base + acc * acc_cols;
-        if (use >= 2) {
-          ok = mbar_wait(accempty0 + 8 * acc, ((use >> 1) - 1) & 1, a.status, 145);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    const unsigned idesc = umma_idesc(128, a.bn), a_lo = umma_desc_lo(tiles);
+    unsigned use = 0;
+    Ring ring;
+    bool ok = true;
+    for (int t = first; t < total && ok; t += step, ++use) {
+      const unsigned acc = use & 1, d = tmem_base + acc * acc_cols;
+      if (use >= 2) {
+        ok = __all_sync(0xffffffffu, mbar_wait(accempty0 + 8 * acc, ((use >> 1) - 1) & 1, a.status, 145));
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      }
+      for (int b = 0; b < blocks && ok; ++b) {
+        ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * ring.stage, ring.parity, a.status, 142));
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const unsigned lo = a_lo + ring.stage * (stage_bytes >> 4);
+        if (ok && elect_one()) {
+          umma_stage(d, lo, lo + (W4U_A_BYTES >> 4), idesc, b ? 1u : 0u);
+          umma_commit(empty0 + 8 * ring.stage);
+          if (b == blocks - 1) umma_commit(accfull0 + 8 * acc);
         }
-        for (int b = 0; b < blocks; ++b, ring.add(1, a.stages)) {
-          const unsigned s = ring.stage;
-          ok = mbar_wait(full0 + 8 * s, ring.parity, a.status, 142);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          const unsigned sa = tiles + s * stage_bytes;
-          const unsigned long long da = umma_desc(sa), db = umma_desc(sa + W4U_A_BYTES);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(d, da + 2 * k, db + 2 * k, idesc, (b | k) ? 1u : 0u);
-          umma_commit(empty0 + 8 * s);
-        }
-        if (ok) umma_commit(accfull0 + 8 * acc);
+        __syncwarp();
+        ring.add(1, a.stages);
       }
     }
-  } else if (warp < 2 + 8 * W4U_SETS) {
+  } else if (warp < 2 + 8 * SETS) {
     // weights: nothing in front of this kernel writes them, so they need not wait for it
     const int sl = (warp - 2) & 7, set = (warp - 2) >> 3, g = lane >> 2, c = lane & 3, slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB;
     Ring base;
     bool ok = true;
     // where the lane's pieces lie in the tile: row 16 sl + g (and + 8: the same swizzle), pieces c and 4 + c of its eight.  Odd rows
     // are written the far piece first, so that eight lanes of a store meet every bank once.
-    const bool flip = g & 1;
-    const unsigned row = (unsigned)(16 * sl + g) * 128u, near = (unsigned)(c ^ g) * 16u, far = (unsigned)((c + 4) ^ g) * 16u;
+    const bool flip = g & 1, two_scales = a.w.gshift == 5;
+    const unsigned row = tiles + (unsigned)(16 * sl + g) * 128u, near = (unsigned)(c ^ g) * 16u, far = (unsigned)((c + 4) ^ g) * 16u;
     const unsigned p0 = row + (flip ? far : near), p1 = row + (flip ? near : far);
-    const bool two_scales = a.w.gshift == 5;
     for (int t = first; t < total && ok; t += step) {
       const int slab = (t / m_tiles) * 8 + sl;
       const bool have = slab < slabs;
       const uint4* q = a.w.q + ((size_t)(have ? slab : 0) * a.w.chunks + c_lo) * 32 + lane;
       const unsigned* sc = a.w.s + (size_t)(have ? slab : 0) * a.w.groups * 8 + g;
-      uint4 qv[W4U_AHEAD];
-      unsigned sv[W4U_AHEAD][2];
-      // This set's blocks of the tile: set, set + SETS, ...; `ahead`: the next one to be fetched.  Always a load, the last
-      // chunk's again behind the end: a register that is loaded or set would have to wait for the load at once.
-      int ahead = set;
+      uint4 qv[AHEAD];
+      unsigned sv[AHEAD][2];
+      // This set's blocks of the tile: set, set + SETS, ...; `ahead`: the next one to be fetched.  Behind the last one loads go on
+      // (into the next slab or the room behind the matrix): a load that may not happen would have to be waited for at once.
+      unsigned ahead = set;
       auto fetch = [&](int u) {
-        const int ch = min(a.parts == 1 ? ahead : ahead / 3, c_hi - c_lo - 1);
-        qv[u] = __ldg(q + (size_t)(unsigned)ch * 32);
-        const unsigned* at = sc + (size_t)((unsigned)((c_lo + ch) * W4_CHUNK) >> a.w.gshift) * 8;
+        const unsigned ch = PARTS == 1 ? ahead : ahead / 3;
+        qv[u] = __ldg(q + ch * 32u);
+        const unsigned* at = sc + ((((unsigned)c_lo + ch) * W4_CHUNK) >> a.w.gshift) * 8u;
         sv[u][0] = __ldg(at);
         sv[u][1] = __ldg(at + (two_scales ? 8 : 0));
-        ahead += W4U_SETS;
+        ahead += SETS;
       };
       Ring ring = base;
       ring.add(set, a.stages);
 #pragma unroll
-      for (int u = 0; u < W4U_AHEAD; ++u) fetch(u);
-      for (int b0 = set; b0 < blocks && ok; b0 += W4U_SETS * W4U_AHEAD) {
+      for (int u = 0; u < AHEAD; ++u) fetch(u);
+      for (int b0 = set; b0 < blocks && ok; b0 += SETS * AHEAD) {
 #pragma unroll
-        for (int u = 0; u < W4U_AHEAD; ++u) {
-          if (b0 + u * W4U_SETS < blocks && ok) {
-            const unsigned sa = have ? sv[u][0] : 0u, sb = have ? sv[u][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
-            const unsigned w[4] = {flip ? qv[u].z : qv[u].x, flip ? qv[u].w : qv[u].y, flip ? qv[u].x : qv[u].z, flip ? qv[u].y : qv[u].w};
-            unsigned v[2][2][4];                              // [row g, g + 8][piece][..]
+        for (int u = 0; u < AHEAD; ++u) {
+          if (b0 + u * SETS >= blocks) break;
+          const unsigned sa = have ? sv[u][0] : 0u, sb = have ? sv[u][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
+          const unsigned w[4] = {flip ? qv[u].z : qv[u].x, flip ? qv[u].w : qv[u].y, flip ? qv[u].x : qv[u].z, flip ? qv[u].y : qv[u].w};
+          unsigned v[2][2][4];                              // [row g, g + 8][piece][..]
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
-                v[r][h][0] = w4_value(w[2 * h], r, s2, off); v[r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
-                v[r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
-              }
-            fetch(u);
-            ok = mbar_wait(empty0 + 8 * ring.stage, ring.parity ^ 1u, a.status, 143);
-            const unsigned dst = tiles + ring.stage * stage_bytes;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {                     // (row g + 8: eight rows of 128 bytes further on)
-              st_shared_v4(dst + p0 + r * 1024u, v[r][0][0], v[r][0][1], v[r][0][2], v[r][0][3]);
-              st_shared_v4(dst + p1 + r * 1024u, v[r][1][0], v[r][1][1], v[r][1][2], v[r][1][3]);
+            for (int h = 0; h < 2; ++h) {
+              const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
+              v[r][h][0] = w4_value(w[2 * h], r, s2, off); v[r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
+              v[r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
             }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full0 + 8 * ring.stage);
-            ring.add(W4U_SETS, a.stages);
+          fetch(u);
+          ok = mbar_wait(empty0 + 8 * ring.stage, ring.parity ^ 1u, a.status, 143) && ok;
+          const unsigned at = ring.stage * stage_bytes;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {                     // (row g + 8: eight rows of 128 bytes further on)
+            st_shared_v4(at + p0 + r * 1024u, v[r][0][0], v[r][0][1], v[r][0][2], v[r][0][3]);
+            st_shared_v4(at + p1 + r * 1024u, v[r][1][0], v[r][1][1], v[r][1][2], v[r][1][3]);
           }
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full0 + 8 * ring.stage);
+          ring.add(SETS, a.stages);
         }
       }
       base.add_many(blocks, a.stages);
     }
   }
   __syncwarp();
-  if (!SPLIT && warp >= 2 + 8 * W4U_SETS) {
+  if (!SPLIT && warp >= 2 + 8 * SETS) {
     pdl_wait();
     const int quarter = warp & 3;
     unsigned use = 0;
@@ -320,7 +337,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       const unsigned acc = use & 1;
       const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + quarter * 32 + lane;
       const float bias = a.bias && n < a.w.N ? a.bias[n] : 0.f;
-      if (!mbar_wait(accfull0 + 8 * acc, (use >> 1) & 1, a.status, 144)) break;
+      if (!epilogue_wait(accfull0 + 8 * acc, (use >> 1) & 1, a.status, &gave_up, quarter == 2)) break;
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       for (int c0 = 0; c0 < a.bn && m0 + c0 < a.M; c0 += 16) {
         float v[16];
@@ -337,14 +354,17 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     const int quarter = warp & 3, t = first;
     const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + quarter * 32 + lane;
     const int share = ((a.bn / 16 + a.splits - 1) / a.splits) * 16;               // columns a rank finishes, a multiple of 16
-    const unsigned recv = tiles + (unsigned)a.stages * stage_bytes;
-    const bool epi_warp = warp >= 2 + 8 * W4U_SETS;
+    const unsigned recv = tiles;                                                  // (over the stages: they have been read when it is written)
+    const bool epi_warp = warp >= 2 + 8 * SETS;
     bool ok = true;
-    cluster_sync();                                                               // (every rank of the cluster has started: its memory is there)
     if (epi_warp) {
       pdl_wait();
-      ok = mbar_wait(accfull0, 0, a.status, 144);
+      ok = epilogue_wait(accfull0, 0, a.status, &gave_up, quarter == 2);
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    }
+    __syncwarp();
+    cluster_sync();                                                               // every rank's MMAs have read their stages
+    if (epi_warp) {
       for (int c0 = 0; ok && c0 < a.bn && m0 + c0 < a.M; c0 += 16) {
         const int owner = c0 / share;
         if (owner == rank) continue;
@@ -355,6 +375,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         for (int j = 0; j < 16; ++j) st_cluster(dst + j * 512, v[j]);
       }
     }
+    __syncwarp();
     cluster_sync();
     if (epi_warp && ok) {
       const float bias = a.bias && n < a.w.N ? a.bias[n] : 0.f;
@@ -437,20 +458,20 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, int x_bf16, long long ldx, const
     x = scratch; ldx = (long long)parts * chunks * W4_CHUNK;
   }
   W4uArgs a = {{(const uint4*)q, (const unsigned*)s, N, K, chunks, groups, gshift}, bias, out, status, ldo, M, epi, out_bf16};
-  a.parts = parts;
   const int n_sm = fellm_sm_count(), n_tiles = ceil_div(N, 128);
   // columns of a tile: all rows in one where they fit, else as few tiles as 256 allow, equally wide
   const int wide = n_tiles * ceil_div(M, 256) >= n_sm ? 256 : 128;
   a.bn = ceil_div(ceil_div(M, ceil_div(M, wide)), 16) * 16;
-  const int total = n_tiles * ceil_div(M, a.bn);
+  const int total = n_tiles * ceil_div(M, a.bn), sets = a.bn <= 128 ? 1 : 2;
   a.splits = 1;
-  while (a.splits < 8 && total * a.splits * 2 <= n_sm && chunks >= a.splits * 2 * 4 && a.bn <= 128) a.splits *= 2;
+  while (sets == 1 && a.splits < 8 && total * a.splits * 2 <= 2 * n_sm && chunks >= a.splits * 2 * 4) a.splits *= 2;
   const int stage = W4U_A_BYTES + a.bn * 128;
   const int share = ceil_div(a.bn / 16, a.splits) * 16, recv = a.splits > 1 ? a.splits * share * 512 : 0;
-  a.stages = (220 * 1024 - recv) / stage;
+  a.stages = (sets == 1 ? 110 : 220) * 1024 / stage;
   if (a.stages > 8) a.stages = 8;
   a.tmem_cols = 32;
-  while (a.tmem_cols < 2 * a.bn) a.tmem_cols *= 2;
+  while (a.tmem_cols < (a.splits > 1 ? 1 : 2) * a.bn) a.tmem_cols *= 2;
+  if (recv > a.stages * stage) return FELLM_ERR_SIZE;
   EncodeTiledFn fn = encode_fn();
   if (!fn) return FELLM_ERR_ARG;
   CUtensorMap map;
@@ -460,10 +481,17 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, int x_bf16, long long ldx, const
   const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return 1000 + (int)r;
-  const size_t smem = (size_t)a.stages * stage + recv + 1024;
-  auto kern = a.splits > 1 ? gemm_w4_umma_kernel<true> : gemm_w4_umma_kernel<false>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
-  const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
-  return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
+  const size_t smem = (size_t)a.stages * stage + 1024;
+  const int grid = a.splits > 1 ? total * a.splits : (total < (3 - sets) * n_sm ? total : (3 - sets) * n_sm);
+  auto go = [&](auto kern) -> int {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(w4u_threads(sets), 1, 1), smem, stream, a.splits, map, a);
+  };
+  if (parts == 1) {
+    if (sets == 2) return go(gemm_w4_umma_kernel<false, 1, 2>);
+    return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 1, 1>) : go(gemm_w4_umma_kernel<false, 1, 1>);
+  }
+  if (sets == 2) return go(gemm_w4_umma_kernel<false, 3, 2>);
+  return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 3, 1>) : go(gemm_w4_umma_kernel<false, 3, 1>);
 }

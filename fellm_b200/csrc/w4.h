@@ -13,12 +13,14 @@
 // so that word >> 4 r, masked with 0x000f000f, is the r-th operand register of an mma.m16n8k16 whose k slots {2c, 2c+1,
 // 2c+8, 2c+9} are taken for elements {0, 1, 2, 3} (a sum does not ask in which order).
 // Scales: bfloat16 pairs (row g, row g + 8), eight of them for each slab and group.
-// Rows behind N are levels 0 under scales 0, elements behind K levels 0.
+// Rows behind N are levels 0 under scales 0, elements behind K levels 0.  Behind the last slab there are W4_READ_AHEAD chunks (and
+// as many chunks' scales at groups of 32) of memory of no meaning: a kernel that fetches ahead need not ask where a row ends.
 #pragma once
 #include "common.cuh"
 
 #define W4_SLAB 16
 #define W4_CHUNK 64
+#define W4_READ_AHEAD 32
 
 struct W4Ref {
   const uint4* q;            // [slabs][chunks][32]

@@ -1978,6 +1978,7 @@ def interleave_gate_up(gate, up):
 # ------------------------------------------------------------------------------ matrices in four bits
 
 W4_GROUPS = (32, 64, 128)
+W4_READ_AHEAD = 32                       # chunks behind the end of a matrix that are there to be read (not used)
 W4_FEW_ROWS = 16                         # up to so many rows: mma.sync, a warp a slab of 16 weight rows; more: tcgen05
 
 
@@ -2014,13 +2015,18 @@ def _w4_dev(*tensors):
 
 
 def _w4_room(N: int, K: int, group: int, device):
+    """(levels [slabs, chunks, 128], scales [slabs, groups, 8]), each with room behind it that a kernel may read ahead into."""
     if group not in W4_GROUPS:
         raise KernelError(f"a group of {group}: four-bit matrices have groups of {', '.join(map(str, W4_GROUPS))}")
     if N < 1 or K < 1 or N > 2 ** 30 or K > 2 ** 30:
         raise KernelError(f"a matrix of {N} x {K} cannot be held in four bits")
     slabs, chunks = -(-N // 16), -(-K // 64)
-    return (torch.empty((slabs, chunks, 128), dtype=torch.int32, device=device),
-            torch.empty((slabs, -(-chunks * 64 // group), 8), dtype=torch.int32, device=device))
+    groups = -(-chunks * 64 // group)
+    made = []
+    for shape, behind in (((slabs, chunks, 128), W4_READ_AHEAD * 128), ((slabs, groups, 8), W4_READ_AHEAD * 16)):
+        n = shape[0] * shape[1] * shape[2]
+        made.append(torch.empty(n + behind, dtype=torch.int32, device=device)[:n].view(shape))
+    return tuple(made)
 
 
 def _w4_matrix(w, what: str):
