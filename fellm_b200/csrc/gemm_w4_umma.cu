@@ -190,23 +190,26 @@ struct Ring {
   __device__ __forceinline__ void add_many(unsigned n, unsigned stages) { stage += n; parity ^= (stage / stages) & 1u; stage %= stages; }
 };
 
-template <bool SPLIT, int PARTS, int SETS>
+// KB: chunks of K a stage.
+template <bool SPLIT, int PARTS, int SETS, int KB>
 __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
-  constexpr int AHEAD = 4;               // chunks a warp holds in registers ahead of the one it unpacks
+  constexpr int AHEAD = KB == 1 ? 4 : 2;                               // stages whose chunks a warp holds in registers ahead of the one it unpacks
+  constexpr unsigned A_BYTES = KB * W4U_A_BYTES;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];           // full[8], empty[8], acc_full[2], acc_empty[2]
   __shared__ unsigned tmem_base_s;
   __shared__ int gave_up;                // the epilogue has
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const unsigned stage_bytes = W4U_A_BYTES + (unsigned)a.bn * 128u;
+  const unsigned x_bytes = (unsigned)a.bn * 128u, stage_bytes = A_BYTES + KB * x_bytes;
   const unsigned full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[8]), accfull0 = smem_u32(&bars[16]), accempty0 = smem_u32(&bars[18]);
   const int m_tiles = (a.M + a.bn - 1) / a.bn, n_tiles = (a.w.N + 127) / 128, total = m_tiles * n_tiles;
   const int rank = SPLIT ? (int)cluster_rank() : 0;
   const int first = SPLIT ? (int)blockIdx.x / a.splits : (int)blockIdx.x, step = SPLIT ? total : (int)gridDim.x;
   // this CTA's chunks of K
-  const int c_lo = SPLIT ? (int)((long long)a.w.chunks * rank / a.splits) : 0, c_hi = SPLIT ? (int)((long long)a.w.chunks * (rank + 1) / a.splits) : a.w.chunks;
-  const int blocks = (c_hi - c_lo) * PARTS;
+  const int stages_of_k = (a.w.chunks + KB - 1) / KB;
+  const int c_lo = SPLIT ? (int)((long long)stages_of_k * rank / a.splits) * KB : 0, c_hi = SPLIT ? (int)((long long)stages_of_k * (rank + 1) / a.splits) * KB : stages_of_k * KB;
+  const int blocks = (c_hi - c_lo) / KB * PARTS;
 
   if (threadIdx.x == 0) {
     gave_up = 0;
@@ -233,8 +236,10 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
       for (int b = 0; b < blocks && ok; ++b) {
         ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * ring.stage, ring.parity ^ 1u, a.status, 141));
         if (ok && elect_one()) {
-          mbar_expect_tx(full0 + 8 * ring.stage, (unsigned)a.bn * 128u);
-          tma_load_2d(tiles + ring.stage * stage_bytes + W4U_A_BYTES, &map_x, (c_lo * PARTS + b) * W4_CHUNK, m0, full0 + 8 * ring.stage);
+          mbar_expect_tx(full0 + 8 * ring.stage, KB * x_bytes);
+#pragma unroll
+          for (int i = 0; i < KB; ++i)                       // (behind the end of K: zeros)
+            tma_load_2d(tiles + ring.stage * stage_bytes + A_BYTES + i * x_bytes, &map_x, (c_lo * PARTS + b * KB + i) * W4_CHUNK, m0, full0 + 8 * ring.stage);
         }
         __syncwarp();
         ring.add(1, a.stages);
@@ -256,7 +261,9 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         const unsigned lo = a_lo + ring.stage * (stage_bytes >> 4);
         if (ok && elect_one()) {
-          umma_stage(d, lo, lo + (W4U_A_BYTES >> 4), idesc, b ? 1u : 0u);
+#pragma unroll
+          for (int i = 0; i < KB; ++i)
+            umma_stage(d, lo + i * (W4U_A_BYTES >> 4), lo + (A_BYTES >> 4) + i * (x_bytes >> 4), idesc, (b | i) ? 1u : 0u);
           umma_commit(empty0 + 8 * ring.stage);
           if (b == blocks - 1) umma_commit(accfull0 + 8 * acc);
         }
@@ -279,17 +286,20 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
       const bool have = slab < slabs;
       const uint4* q = a.w.q + ((size_t)(have ? slab : 0) * a.w.chunks + c_lo) * 32 + lane;
       const unsigned* sc = a.w.s + (size_t)(have ? slab : 0) * a.w.groups * 8 + g;
-      uint4 qv[AHEAD];
-      unsigned sv[AHEAD][2];
+      uint4 qv[AHEAD][KB];
+      unsigned sv[AHEAD][KB][2];
       // This set's blocks of the tile: set, set + SETS, ...; `ahead`: the next one to be fetched.  Behind the last one loads go on
       // (into the next slab or the room behind the matrix): a load that may not happen would have to be waited for at once.
       unsigned ahead = set;
       auto fetch = [&](int u) {
-        const unsigned ch = PARTS == 1 ? ahead : ahead / 3;
-        qv[u] = __ldg(q + ch * 32u);
-        const unsigned* at = sc + ((((unsigned)c_lo + ch) * W4_CHUNK) >> a.w.gshift) * 8u;
-        sv[u][0] = __ldg(at);
-        sv[u][1] = __ldg(at + (two_scales ? 8 : 0));
+#pragma unroll
+        for (int i = 0; i < KB; ++i) {
+          const unsigned ch = PARTS == 1 ? ahead * KB + i : ahead / 3;
+          qv[u][i] = __ldg(q + ch * 32u);
+          const unsigned* at = sc + ((((unsigned)c_lo + ch) * W4_CHUNK) >> a.w.gshift) * 8u;
+          sv[u][i][0] = __ldg(at);
+          sv[u][i][1] = __ldg(at + (two_scales ? 8 : 0));
+        }
         ahead += SETS;
       };
       Ring ring = base;
@@ -300,25 +310,32 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
           if (b0 + u * SETS >= blocks) break;
-          const unsigned sa = have ? sv[u][0] : 0u, sb = have ? sv[u][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
-          const unsigned w[4] = {flip ? qv[u].z : qv[u].x, flip ? qv[u].w : qv[u].y, flip ? qv[u].x : qv[u].z, flip ? qv[u].y : qv[u].w};
-          unsigned v[2][2][4];                              // [row g, g + 8][piece][..]
+          unsigned v[KB][2][2][4];                          // [chunk][row g, g + 8][piece][..]
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+          for (int i = 0; i < KB; ++i) {
+            const bool in = have && (KB == 1 || i == 0 || c_lo + (b0 + u * SETS) * KB + i < a.w.chunks);
+            const uint4 x = qv[u][i];
+            const unsigned sa = in ? sv[u][i][0] : 0u, sb = in ? sv[u][i][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
+            const unsigned w[4] = {flip ? x.z : x.x, flip ? x.w : x.y, flip ? x.x : x.z, flip ? x.y : x.w};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
-              v[r][h][0] = w4_value(w[2 * h], r, s2, off); v[r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
-              v[r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
-            }
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
+                v[i][r][h][0] = w4_value(w[2 * h], r, s2, off); v[i][r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
+                v[i][r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[i][r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
+              }
+          }
           fetch(u);
           ok = mbar_wait(empty0 + 8 * ring.stage, ring.parity ^ 1u, a.status, 143) && ok;
           const unsigned at = ring.stage * stage_bytes;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {                     // (row g + 8: eight rows of 128 bytes further on)
-            st_shared_v4(at + p0 + r * 1024u, v[r][0][0], v[r][0][1], v[r][0][2], v[r][0][3]);
-            st_shared_v4(at + p1 + r * 1024u, v[r][1][0], v[r][1][1], v[r][1][2], v[r][1][3]);
-          }
+          for (int i = 0; i < KB; ++i)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {                   // (row g + 8: eight rows of 128 bytes further on)
+              st_shared_v4(at + p0 + i * W4U_A_BYTES + r * 1024u, v[i][r][0][0], v[i][r][0][1], v[i][r][0][2], v[i][r][0][3]);
+              st_shared_v4(at + p1 + i * W4U_A_BYTES + r * 1024u, v[i][r][1][0], v[i][r][1][1], v[i][r][1][2], v[i][r][1][3]);
+            }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
           __syncwarp();
           if (lane == 0) mbar_arrive(full0 + 8 * ring.stage);
@@ -465,9 +482,9 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, int x_bf16, long long ldx, const
   const int total = n_tiles * ceil_div(M, a.bn), sets = a.bn <= 128 ? 1 : 2;
   a.splits = 1;
   while (sets == 1 && a.splits < 8 && total * a.splits * 2 <= 2 * n_sm && chunks >= a.splits * 2 * 4) a.splits *= 2;
-  const int stage = W4U_A_BYTES + a.bn * 128;
+  const int kb = parts == 1 && a.bn <= 64 ? 2 : 1, stage = kb * (W4U_A_BYTES + a.bn * 128);
   const int share = ceil_div(a.bn / 16, a.splits) * 16, recv = a.splits > 1 ? a.splits * share * 512 : 0;
-  a.stages = (sets == 1 ? 110 : 220) * 1024 / stage;
+  a.stages = (sets == 1 ? 112 : 220) * 1024 / stage;
   if (a.stages > 8) a.stages = 8;
   a.tmem_cols = 32;
   while (a.tmem_cols < (a.splits > 1 ? 1 : 2) * a.bn) a.tmem_cols *= 2;
@@ -489,9 +506,10 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, int x_bf16, long long ldx, const
     return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(w4u_threads(sets), 1, 1), smem, stream, a.splits, map, a);
   };
   if (parts == 1) {
-    if (sets == 2) return go(gemm_w4_umma_kernel<false, 1, 2>);
-    return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 1, 1>) : go(gemm_w4_umma_kernel<false, 1, 1>);
+    if (sets == 2) return go(gemm_w4_umma_kernel<false, 1, 2, 1>);
+    if (kb == 2) return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 1, 1, 2>) : go(gemm_w4_umma_kernel<false, 1, 1, 2>);
+    return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 1, 1, 1>) : go(gemm_w4_umma_kernel<false, 1, 1, 1>);
   }
-  if (sets == 2) return go(gemm_w4_umma_kernel<false, 3, 2>);
-  return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 3, 1>) : go(gemm_w4_umma_kernel<false, 3, 1>);
+  if (sets == 2) return go(gemm_w4_umma_kernel<false, 3, 2, 1>);
+  return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 3, 1, 1>) : go(gemm_w4_umma_kernel<false, 3, 1, 1>);
 }
