@@ -125,14 +125,12 @@ struct W4uArgs {
 // The four words of a lane (rows g and g + 8, 16 elements each) -> its pieces of the tile.  Neighbouring even and odd rows
 // are written half a row apart, so that eight lanes of a store meet every bank once.
 __device__ __forceinline__ unsigned w4_value(unsigned word, int r, unsigned s2, unsigned off2) {
-  // nibble r of both halves at bits 3..6: 16 + level + 8 at exponent 4
-  const unsigned moved = r == 0 ? word << 3 : word >> (4 * r - 3);
-  const unsigned b = (moved & 0x00780078u) | 0x41804180u;
+  const unsigned b = w4_pair_biased(word, r);
   __nv_bfloat162 v = __hfma2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&s2, *(const __nv_bfloat162*)&off2);
   return *(unsigned*)&v;
 }
 __device__ __forceinline__ unsigned times_minus_24(unsigned s2) {
-  const unsigned c = 0xc1c0c1c0u;                                    // -24, -24
+  const unsigned c = W4_MINUS_24;
   __nv_bfloat162 v = __hmul2(*(const __nv_bfloat162*)&s2, *(const __nv_bfloat162*)&c);
   return *(unsigned*)&v;
 }

@@ -58,7 +58,8 @@ __device__ __forceinline__ void load8(const T* row, bool row_ok, int k, int K, b
 }
 // Two rows' eight levels (0..15 each) of a half chunk -> the two words of w4.h.
 __device__ __forceinline__ unsigned pack_word(const unsigned* a, const unsigned* b) {
-  return a[0] | b[0] << 4 | a[2] << 8 | b[2] << 12 | a[1] << 16 | b[1] << 20 | a[3] << 24 | b[3] << 28;
+  const unsigned w = a[0] | b[0] << 4 | a[2] << 8 | b[2] << 12 | a[1] << 16 | b[1] << 20 | a[3] << 24 | b[3] << 28;
+  return __funnelshift_l(w, w, 3);
 }
 
 struct W4Out { uint4* q; unsigned* s; int N, K, chunks, groups, gshift; };
@@ -198,7 +199,7 @@ __device__ __forceinline__ void row8(const W4Ref& m, int row, int k, float* v) {
   const int sh = r < 8 ? 0 : 4;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const unsigned u = (i ? w.y : w.x) >> sh;
+    const unsigned x = i ? w.y : w.x, u = __funnelshift_r(x, x, 3) >> sh;
     v[4 * i + 0] = s * (float)((int)(u & 15u) - 8);
     v[4 * i + 1] = s * (float)((int)(u >> 16 & 15u) - 8);
     v[4 * i + 2] = s * (float)((int)(u >> 8 & 15u) - 8);

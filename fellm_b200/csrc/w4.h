@@ -7,11 +7,13 @@
 //
 // Levels: slabs of 16 rows x chunks of 64 k, 512 bytes each, slab after slab and in it chunk after chunk; a warp reads a
 // chunk in one load of 16 bytes a lane.  Lane 4 g + c has rows g and g + 8, and of the chunk's two halves the elements
-// 8 c .. 8 c + 7: word j is half j / 2, elements 4 (j % 2) .. + 3 of those eight.  In a word, four bits each, q + 8:
+// 8 c .. 8 c + 7: word j is half j / 2, elements 4 (j % 2) .. + 3 of those eight.  In a word, turned left by three bits, four
+// bits each, q + 8:
 //   bits  0 row g element 0,   4 row g+8 element 0,   8 row g element 2,  12 row g+8 element 2,
 //   bits 16 row g element 1,  20 row g+8 element 1,  24 row g element 3,  28 row g+8 element 3,
-// so that word >> 4 r, masked with 0x000f000f, is the r-th operand register of an mma.m16n8k16 whose k slots {2c, 2c+1,
-// 2c+8, 2c+9} are taken for elements {0, 1, 2, 3} (a sum does not ask in which order).
+// so that the word turned right by 4 r and masked with 0x00780078 has at the top of bfloat16's mantissa what the r-th operand
+// register of an mma.m16n8k16 wants, whose k slots {2c, 2c+1, 2c+8, 2c+9} are taken for elements {0, 1, 2, 3} (a sum does not
+// ask in which order): or-ed with 0x41804180 it is the pair of 16 + (q + 8).
 // Scales: bfloat16 pairs (row g, row g + 8), eight of them for each slab and group.
 // Rows behind N are levels 0 under scales 0, elements behind K levels 0.  Behind the last slab there are W4_READ_AHEAD chunks (and
 // as many chunks' scales at groups of 32) of memory of no meaning: a kernel that fetches ahead need not ask where a row ends.
@@ -29,12 +31,12 @@ struct W4Ref {
   int gshift;                // log2 of the group: 5, 6 or 7
 };
 
-// 128 + q + 8 in both halves is 0x4300 | (q + 8): the four bits are the lowest of bfloat16's mantissa at exponent 7.
-__device__ __forceinline__ unsigned w4_pair_biased(unsigned word, int r) { return ((word >> (4 * r)) & 0x000f000fu) | 0x43004300u; }
-// minus 136: the levels themselves, exactly.
+__device__ __forceinline__ unsigned w4_pair_biased(unsigned word, int r) { return (__funnelshift_r(word, word, 4 * r) & 0x00780078u) | 0x41804180u; }
+// minus 24: the levels themselves, exactly.
+#define W4_MINUS_24 0xc1c0c1c0u
 __device__ __forceinline__ unsigned w4_pair(unsigned word, int r) {
-  const unsigned b = w4_pair_biased(word, r), off = 0x43084308u;
-  __nv_bfloat162 v = __hsub2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&off);
+  const unsigned b = w4_pair_biased(word, r), off = W4_MINUS_24;
+  __nv_bfloat162 v = __hadd2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&off);
   return *(unsigned*)&v;
 }
 __device__ __forceinline__ float w4_scale_lo(unsigned s) { return __uint_as_float(s << 16); }
