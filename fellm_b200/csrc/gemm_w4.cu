@@ -17,7 +17,7 @@
 #include "w4.h"
 
 #define GW_UNIT 4                      // chunks
-#define GW_DEPTH 3                     // units of a warp's ring: one is used, the others are on their way
+#define GW_DEPTH 4                     // units of a warp's ring: one is used, the others are on their way
 #define GW_SLOT (GW_UNIT * (512 + 64)) // a unit's levels, its groups' scales (eight at groups of 32)
 
 enum { EPI_STORE = 0, EPI_ACC = 1, EPI_SWIGLU = 2, EPI_F32 = 3, EPI_RELU2 = 6 };      // 6: max(v, 0)^2
@@ -28,7 +28,6 @@ struct GwArgs {
   const void* x; const float* bias; void* out;
   long long ldx, ldo;
   int M, epi, out_bf16;
-  int share;                 // warps that share a slab: a power of two, all of a block's warps in such groups
 };
 
 __device__ __forceinline__ void mma_bf16(float* d, const unsigned* a, unsigned b0, unsigned b1) {
@@ -37,31 +36,36 @@ __device__ __forceinline__ void mma_bf16(float* d, const unsigned* a, unsigned b
 }
 // Eight elements of a row of x from k on as operand registers [part][4].
 template <int XT> struct XParts { static constexpr int N = XT == X_F32 ? 3 : 1; };
-// `row` points to the row's element 0.  FULL: all eight are there.
+// Eight elements from p on, of which `left` are the row's.  FULL: all eight.
 template <int XT, bool FULL>
-__device__ __forceinline__ void load_x8(const void* row, int k, int K, unsigned (*b)[4]) {
+__device__ __forceinline__ void load_x8(const void* at, int left, unsigned (*b)[4]) {
   constexpr int P = XParts<XT>::N;
   if (XT == X_BF16) {
-    const uint4 v = FULL || k < K ? *(const uint4*)((const bf16*)row + k) : make_uint4(0u, 0u, 0u, 0u);
+    const uint4 v = FULL || left > 0 ? *(const uint4*)at : make_uint4(0u, 0u, 0u, 0u);
     b[0][0] = v.x; b[0][1] = v.y; b[0][2] = v.z; b[0][3] = v.w;
   } else if (XT == X_BF16_ANY) {
-    const unsigned short* p = (const unsigned short*)row + k;
+    const unsigned short* p = (const unsigned short*)at;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const unsigned lo = FULL || k + 2 * i < K ? p[2 * i] : 0, hi = FULL || k + 2 * i + 1 < K ? p[2 * i + 1] : 0;
+      const unsigned lo = FULL || 2 * i < left ? p[2 * i] : 0, hi = FULL || 2 * i + 1 < left ? p[2 * i + 1] : 0;
       b[0][i] = lo | hi << 16;
     }
   } else {
-    const float* p = (const float*)row + k;
+    const float* p = (const float*)at;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       unsigned lo[3], hi[3];
-      w4_split3(FULL || k + 2 * i < K ? p[2 * i] : 0.f, lo[0], lo[1], lo[2]);
-      w4_split3(FULL || k + 2 * i + 1 < K ? p[2 * i + 1] : 0.f, hi[0], hi[1], hi[2]);
+      w4_split3(FULL || 2 * i < left ? p[2 * i] : 0.f, lo[0], lo[1], lo[2]);
+      w4_split3(FULL || 2 * i + 1 < left ? p[2 * i + 1] : 0.f, hi[0], hi[1], hi[2]);
 #pragma unroll
       for (int q = 0; q < P; ++q) b[q][i] = lo[q] >> 16 | hi[q];
     }
   }
+}
+
+__device__ __forceinline__ void mma_bf16_first(float* d, const unsigned* a, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // One value of the result (two of the gated form's sums give one).
@@ -77,71 +81,104 @@ __device__ __forceinline__ void put(const GwArgs& a, int m, int n, float v) {
 
 struct TrueType { static constexpr bool value = true; };
 struct FalseType { static constexpr bool value = false; };
-__device__ __forceinline__ void cp_async16(unsigned dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+// (offsets as immediates: an addition for every copy and load is an instruction in thirty)
+template <int DST, int SRC> __device__ __forceinline__ void cp_async16(unsigned dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;\n" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
 }
+template <int OFF> __device__ __forceinline__ uint4 lds128(unsigned at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4 + %5];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at), "n"(OFF));
+  return v;
+}
+template <int OFF> __device__ __forceinline__ unsigned lds32(unsigned at) {
+  unsigned v;
+  asm volatile("ld.shared.b32 %0, [%1 + %2];\n" : "=r"(v) : "r"(at), "n"(OFF));
+  return v;
+}
+template <int I> struct Int { static constexpr int value = I; };
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
+// What a block's warps do next with the slabs that are left of its range: t slabs side by side, `share` = warps / t warps each, t a power
+// of two: whole rounds of a slab a warp (nothing to be put together), and the rest of the range by all warps too.
+struct Segment {
+  int slab, lo, hi;          // this warp's slab and its units of it
+  int t, share;
+};
+__device__ __forceinline__ Segment next_segment(int slab, int left, int warp, int warps, int units) {
+  Segment s;
+  const int log_w = 31 - __clz(warps), log_t = min(log_w, 31 - __clz(left)), log_share = log_w - log_t;        // (left >= 1)
+  s.t = 1 << log_t;
+  s.share = 1 << log_share;
+  const int sub = warp & (s.share - 1);
+  s.slab = slab + (warp >> log_share);
+  s.lo = (units * sub) >> log_share; s.hi = (units * (sub + 1)) >> log_share;
+  return s;
+}
+
 // XT: what x is.  NT: tiles of eight rows of x.  GS: log2 of the group.
 template <int XT, int NT, int GS>
-__global__ void __launch_bounds__(512) gemm_w4_rows_kernel(GwArgs a) {
-  constexpr int P = XParts<XT>::N, COLS = 8 * NT;
+__global__ void __maxnreg__(128) gemm_w4_rows_kernel(GwArgs a) {
+  constexpr int P = XParts<XT>::N, COLS = 8 * NT, XB = XT == X_F32 ? 4 : 2;      // XB: bytes of an element of x
   extern __shared__ __align__(16) unsigned char smem[];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB, m0 = blockIdx.y * COLS, cols = min(a.M - m0, COLS);
-  const int group = warp / a.share, sub = warp % a.share, groups = warps / a.share;
-  const int first = blockIdx.x * groups + group, step = gridDim.x * groups;
-  const unsigned char* ring = smem + (size_t)warp * GW_DEPTH * GW_SLOT;
-  const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring);
+  const int first = (int)((long long)slabs * blockIdx.x / gridDim.x), end = (int)((long long)slabs * (blockIdx.x + 1) / gridDim.x);
+  const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * GW_DEPTH * GW_SLOT;
   float* red = reinterpret_cast<float*>(smem + (size_t)warps * GW_DEPTH * GW_SLOT);      // [2][warps][COLS][17]
-  // this warp's units of every slab
-  const int units = (a.w.chunks + GW_UNIT - 1) / GW_UNIT, lo = units * sub / a.share, hi = units * (sub + 1) / a.share;
+  const int units = (a.w.chunks + GW_UNIT - 1) / GW_UNIT;
   constexpr int SCALES = 256 >> GS;                         // groups a unit
-  int f_slab = first, f_unit = lo;
-  unsigned f_at = ring_at;
-  const uint4* fq = a.w.q + ((size_t)f_slab * a.w.chunks + lo * GW_UNIT) * 32 + lane;
-  const unsigned* fs = a.w.s + ((size_t)f_slab * a.w.groups + lo * SCALES) * 8 + 4 * lane;
-  // (a unit that ends behind the slab's last chunk takes what lies behind it along)
+  // what is fetched next: of which segment, how many units are left of it (a unit that ends behind the slab's last chunk takes what lies
+  // behind it along)
+  int f_slab = first, f_left = 0;
+  unsigned f_at = ring + lane * 16;
+  const uint4* fq = a.w.q;
+  const unsigned* fs = a.w.s;
   auto fetch = [&]() {
-    if (f_slab < slabs && lo < hi) {
-#pragma unroll
-      for (int i = 0; i < GW_UNIT; ++i) cp_async16(f_at + i * 512 + lane * 16, fq + i * 32);
-      if (lane < 2 * SCALES) cp_async16(f_at + GW_UNIT * 512 + lane * 16, fs);
+    while (f_left == 0 && f_slab < end) {
+      const Segment n = next_segment(f_slab, end - f_slab, warp, warps, units);
+      f_slab += n.t;
+      f_left = n.hi - n.lo;
+      fq = a.w.q + ((size_t)n.slab * a.w.chunks + n.lo * GW_UNIT) * 32 + lane;
+      fs = a.w.s + ((size_t)n.slab * a.w.groups + n.lo * SCALES) * 8 + 4 * lane;
+    }
+    if (f_left > 0) {
+      cp_async16<0, 0>(f_at, fq); cp_async16<512, 512>(f_at, fq); cp_async16<1024, 1024>(f_at, fq); cp_async16<1536, 1536>(f_at, fq);
+      if (lane < 2 * SCALES) cp_async16<GW_UNIT * 512, 0>(f_at, fs);
       fq += GW_UNIT * 32; fs += SCALES * 8;
-      if (++f_unit == hi) {
-        f_unit = lo; f_slab += step;
-        fq = a.w.q + ((size_t)f_slab * a.w.chunks + lo * GW_UNIT) * 32 + lane;
-        fs = a.w.s + ((size_t)f_slab * a.w.groups + lo * SCALES) * 8 + 4 * lane;
-      }
+      --f_left;
     }
     cp_commit();
-    f_at = f_at == ring_at + (GW_DEPTH - 1) * GW_SLOT ? ring_at : f_at + GW_SLOT;
+    f_at = f_at == ring + lane * 16 + (GW_DEPTH - 1) * GW_SLOT ? ring + lane * 16 : f_at + GW_SLOT;
   };
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < GW_DEPTH - 1; ++i) fetch();          // (weights: nothing in front of this kernel writes them)
   pdl_launch_dependents();
   pdl_wait();
   const unsigned char* xrow[NT];                            // (columns behind the last row repeat it: nobody reads their sums)
 #pragma unroll
-  for (int t = 0; t < NT; ++t) xrow[t] = (const unsigned char*)a.x + (size_t)(m0 + min(8 * t + g, cols - 1)) * a.ldx * (XT == X_F32 ? 4 : 2);
-  const unsigned char* at = ring;
+  for (int t = 0; t < NT; ++t) xrow[t] = (const unsigned char*)a.x + (size_t)(m0 + min(8 * t + g, cols - 1)) * a.ldx * XB + c * 8 * XB;
+  unsigned at = ring;
   int turn = 0;
-  for (int slab = first; slab < slabs; slab += step, turn ^= 1) {
+  for (int next = first; next < end; turn ^= 1) {
+    const Segment seg = next_segment(next, end - next, warp, warps, units);
+    next += seg.t;
     float total[NT][4], part[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) total[t][i] = part[t][i] = 0.f;
-    auto chunk = [&](int i, int ch, auto full) {
+      for (int i = 0; i < 4; ++i) total[t][i] = 0.f;
+    // chunk i of unit u, whose elements of x lie from `xu` on
+    auto chunk = [&](auto idx, int u, const unsigned char* const* xu, auto full) {
+      constexpr int i = decltype(idx)::value;
       unsigned b[2][NT][P][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) load_x8<XT, decltype(full)::value>(xrow[t], ch * W4_CHUNK + h * 32 + c * 8, a.w.K, b[h][t]);
-      const uint4 qv = *(const uint4*)(at + i * 512 + lane * 16);
+        for (int t = 0; t < NT; ++t)
+          load_x8<XT, decltype(full)::value>(xu[t] + (i * W4_CHUNK + h * 32) * XB, a.w.K - (u * GW_UNIT + i) * W4_CHUNK - h * 32 - c * 8, b[h][t]);
+      const uint4 qv = lds128<i * 512>(at + lane * 16);
       const unsigned word[4] = {qv.x, qv.y, qv.z, qv.w};
-      const unsigned* sc = (const unsigned*)(at + GW_UNIT * 512) + g;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -152,35 +189,43 @@ __global__ void __launch_bounds__(512) gemm_w4_rows_kernel(GwArgs a) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
 #pragma unroll
-            for (int p = P - 1; p >= 0; --p) mma_bf16(part[t], w, b[h][t][p][2 * j], b[h][t][p][2 * j + 1]);
+            for (int p = P - 1; p >= 0; --p) {
+              if (j == 0 && p == P - 1 && (GS == 5 || (h == 0 && (GS == 6 || !(i & 1))))) mma_bf16_first(part[t], w, b[h][t][p][0], b[h][t][p][1]);
+              else mma_bf16(part[t], w, b[h][t][p][2 * j], b[h][t][p][2 * j + 1]);
+            }
           }
         }
-        if (GS == 5 || (h == 1 && (GS == 6 || (i & 1) || ch == a.w.chunks - 1))) {
-          const unsigned sv = sc[(GS == 5 ? 2 * i + h : GS == 6 ? i : i >> 1) * 8];
+        if (GS == 5 || (h == 1 && (GS == 6 || (i & 1) || (!decltype(full)::value && u * GW_UNIT + i == a.w.chunks - 1)))) {
+          const unsigned sv = GS == 5 ? (h ? lds32<GW_UNIT * 512 + (2 * i + 1) * 32>(at + g * 4) : lds32<GW_UNIT * 512 + 2 * i * 32>(at + g * 4))
+                                      : lds32<GW_UNIT * 512 + (GS == 6 ? i : i >> 1) * 32>(at + g * 4);
           const float s0 = w4_scale_lo(sv), s1 = w4_scale_hi(sv);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             total[t][0] = fmaf(s0, part[t][0], total[t][0]); total[t][1] = fmaf(s0, part[t][1], total[t][1]);
             total[t][2] = fmaf(s1, part[t][2], total[t][2]); total[t][3] = fmaf(s1, part[t][3], total[t][3]);
-            part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.f;
           }
         }
       }
     };
-    for (int u = lo; u < hi; ++u) {
+    for (int u = seg.lo; u < seg.hi; ++u) {
       cp_wait<GW_DEPTH - 2>();
       __syncwarp();                                          // every lane's copies have come, and every lane has read the unit before
       fetch();                                               // over that one
+      const unsigned char* xu[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) xu[t] = xrow[t] + (size_t)u * (GW_UNIT * W4_CHUNK * XB);
       if ((u + 1) * GW_UNIT * W4_CHUNK <= a.w.K) {
-#pragma unroll
-        for (int i = 0; i < GW_UNIT; ++i) chunk(i, u * GW_UNIT + i, TrueType());
+        chunk(Int<0>(), u, xu, TrueType()); chunk(Int<1>(), u, xu, TrueType());
+        chunk(Int<2>(), u, xu, TrueType()); chunk(Int<3>(), u, xu, TrueType());
       } else {
-#pragma unroll
-        for (int i = 0; i < GW_UNIT; ++i) if (u * GW_UNIT + i < a.w.chunks) chunk(i, u * GW_UNIT + i, FalseType());
+        chunk(Int<0>(), u, xu, FalseType());
+        if (u * GW_UNIT + 1 < a.w.chunks) chunk(Int<1>(), u, xu, FalseType());
+        if (u * GW_UNIT + 2 < a.w.chunks) chunk(Int<2>(), u, xu, FalseType());
+        if (u * GW_UNIT + 3 < a.w.chunks) chunk(Int<3>(), u, xu, FalseType());
       }
       at = at == ring + (GW_DEPTH - 1) * GW_SLOT ? ring : at + GW_SLOT;
     }
-    // the warps' shares together: two buffers in turn, so that one barrier a slab is enough
+    // the warps' shares together: two buffers in turn, so that one barrier is enough
     float* mine = red + ((size_t)(turn * warps + warp) * COLS) * 17;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -188,13 +233,14 @@ __global__ void __launch_bounds__(512) gemm_w4_rows_kernel(GwArgs a) {
       if (8 * t + 2 * c < cols) { p[0] = total[t][0]; p[8] = total[t][2]; }
       if (8 * t + 2 * c + 1 < cols) { p[17] = total[t][1]; p[25] = total[t][3]; }
     }
-    if (a.share == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "r"(32 * a.share) : "memory");
-    for (int i = 32 * sub + lane; i < ((cols + 1) & ~1) * W4_SLAB; i += 32 * a.share) {         // (a warp takes two rows of x)
-      const int t = i / W4_SLAB, r = i % W4_SLAB, m = m0 + t, n = slab * W4_SLAB + r;
-      const float* p = red + ((size_t)(turn * warps + group * a.share) * COLS + t) * 17 + r;
+    if (seg.share == 1) __syncwarp();
+    else __syncthreads();
+    const int sub = warp & (seg.share - 1);
+    for (int i = 32 * sub + lane; i < ((cols + 1) & ~1) * W4_SLAB; i += 32 * seg.share) {         // (a warp takes two rows of x)
+      const int t = i / W4_SLAB, r = i % W4_SLAB, m = m0 + t, slab = seg.slab, n = slab * W4_SLAB + r;
+      const float* p = red + ((size_t)(turn * warps + warp - sub) * COLS + t) * 17 + r;
       float v = 0.f;
-      for (int w = 0; w < a.share; ++w) v += p[w * COLS * 17];
+      for (int w = 0; w < seg.share; ++w) v += p[w * COLS * 17];
       if (a.bias && n < a.w.N) v += a.bias[n];
       if (a.epi == EPI_SWIGLU) {
         const float up = __shfl_down_sync(0xffffffffu, v, 8);
@@ -205,7 +251,7 @@ __global__ void __launch_bounds__(512) gemm_w4_rows_kernel(GwArgs a) {
 }
 
 template <int XT, int NT, int GS>
-static int launch_rows(GwArgs a, cudaStream_t stream) {
+static int launch_rows(const GwArgs& a, cudaStream_t stream) {
   const int slabs = ceil_div(a.w.N, W4_SLAB), units = ceil_div(a.w.chunks, GW_UNIT), n_sm = fellm_sm_count(), tiles = ceil_div(a.M, 8 * NT);
   auto kern = gemm_w4_rows_kernel<XT, NT, GS>;
   auto bytes = [](int warps) { return (size_t)warps * (GW_DEPTH * GW_SLOT + 2 * 8 * NT * 17 * 4); };
@@ -217,18 +263,10 @@ static int launch_rows(GwArgs a, cudaStream_t stream) {
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, 256, bytes(8)) != cudaSuccess || n < 1) n = 1;
     resident = n;
   }
-  // how many warps share a slab: the time of the busiest warp, in units and some three quarters of one for the end of a slab
-  const int most = resident * 8 * n_sm;
-  int best = 1;
-  double best_t = 1e30;
-  for (int share = 1; share <= 16 && share <= units; share *= 2) {
-    const double t = (double)ceil_div(slabs, most / share < 1 ? 1 : most / share) * (ceil_div(units, share) + 0.75);
-    if (t < best_t) { best_t = t; best = share; }
-  }
-  a.share = best;
-  const int warps = best == 16 ? 16 : slabs <= n_sm * (8 / best) ? best : 8;       // (few slabs: a block each)
-  const int groups = warps / best, want = ceil_div(slabs, groups), fit = resident * 8 / warps * n_sm;
-  const dim3 grid(want < fit ? want : (fit > 0 ? fit : n_sm), tiles, 1);
+  // Two blocks of eight warps an SM (what their rings leave room for), each a range of neighbouring slabs: every slot is filled before a block
+  // gets a second slab, since blocks are not spread over SMs evenly otherwise.  Few slabs: a block each, of sixteen warps where K is long
+  const int warps = slabs <= n_sm && units >= 16 ? 16 : 8, per = warps == 16 ? 1 : resident;
+  const dim3 grid(slabs < n_sm * per ? slabs : n_sm * per, tiles, 1);
   if (grid.y > 65535) return FELLM_ERR_SIZE;
   return launch_k_class(1, kern, grid, dim3(warps * 32, 1, 1), bytes(warps), stream, 1, a);
 }
@@ -246,7 +284,7 @@ FELLM_API int fellm_gemm_w4(const void* x, int x_bf16, long long ldx, const void
   if (groups != (int)(((long long)chunks * W4_CHUNK + (1 << gshift) - 1) >> gshift)) return FELLM_ERR_SIZE;
   if (epi != EPI_STORE && epi != EPI_ACC && epi != EPI_SWIGLU && epi != EPI_F32 && epi != EPI_RELU2) return FELLM_ERR_ARG;
   if (epi == EPI_SWIGLU && N % W4_SLAB) return FELLM_ERR_SIZE;
-  const GwArgs a = {{(const uint4*)q, (const unsigned*)s, N, K, chunks, groups, gshift}, x, bias, out, ldx, ldo, M, epi, out_bf16, 1};
+  const GwArgs a = {{(const uint4*)q, (const unsigned*)s, N, K, chunks, groups, gshift}, x, bias, out, ldx, ldo, M, epi, out_bf16};
   if (!x_bf16) return launch_rows_group<X_F32, 1>(a, stream);
   if (K % 8 || ldx % 8 || ((uintptr_t)x & 15)) return launch_rows_group<X_BF16_ANY, 1>(a, stream);
   return M <= 8 ? launch_rows_group<X_BF16, 1>(a, stream) : M <= 16 ? launch_rows_group<X_BF16, 2>(a, stream) : launch_rows_group<X_BF16, 4>(a, stream);

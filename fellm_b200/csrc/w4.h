@@ -31,7 +31,12 @@ struct W4Ref {
   int gshift;                // log2 of the group: 5, 6 or 7
 };
 
-__device__ __forceinline__ unsigned w4_pair_biased(unsigned word, int r) { return (__funnelshift_r(word, word, 4 * r) & 0x00780078u) | 0x41804180u; }
+// (One three-input operation: written as an and with a constant and an or with another it becomes two.)
+__device__ __forceinline__ unsigned w4_pair_biased(unsigned word, int r) {
+  unsigned v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(v) : "r"(__funnelshift_r(word, word, 4 * r)), "r"(0x00780078u), "r"(0x41804180u));
+  return v;
+}
 // minus 24: the levels themselves, exactly.
 #define W4_MINUS_24 0xc1c0c1c0u
 __device__ __forceinline__ unsigned w4_pair(unsigned word, int r) {
