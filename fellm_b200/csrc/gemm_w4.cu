@@ -16,11 +16,9 @@
 // nothing is rounded), which meet the same weights in three MMAs.
 #include "w4.h"
 
-#define GW_UNIT 4                      // chunks
 #define GW_DEPTH 4                     // units of a warp's ring: one is used, the others are on their way
-#define GW_SLOT (GW_UNIT * (512 + 64)) // a unit's levels, its groups' scales (eight at groups of 32)
+#define GW_SLOT (4 * (512 + 64))       // a unit: four chunks' levels, their groups' scales (eight at groups of 32)
 
-enum { EPI_STORE = 0, EPI_ACC = 1, EPI_SWIGLU = 2, EPI_F32 = 3, EPI_RELU2 = 6 };      // 6: max(v, 0)^2
 enum { X_BF16 = 0, X_BF16_ANY = 1, X_F32 = 2 };       // rows on 16 bytes and K a multiple of 8; any bfloat16; float32
 
 struct GwArgs {
@@ -71,9 +69,9 @@ __device__ __forceinline__ void mma_bf16_first(float* d, const unsigned* a, unsi
 // One value of the result (two of the gated form's sums give one).
 __device__ __forceinline__ void put(const GwArgs& a, int m, int n, float v) {
   const size_t o = (size_t)m * a.ldo + n;
-  if (a.epi == EPI_ACC) ((float*)a.out)[o] += v;
+  if (a.epi == W4_ACC) ((float*)a.out)[o] += v;
   else {
-    if (a.epi == EPI_RELU2) { v = fmaxf(v, 0.f); v *= v; }
+    if (a.epi == W4_RELU2) { v = fmaxf(v, 0.f); v *= v; }
     if (a.out_bf16) ((bf16*)a.out)[o] = __float2bfloat16_rn(v);
     else ((float*)a.out)[o] = v;
   }
@@ -116,36 +114,48 @@ __device__ __forceinline__ Segment next_segment(int slab, int left, int warp, in
   return s;
 }
 
-// XT: what x is.  NT: tiles of eight rows of x.  GS: log2 of the group.
-template <int XT, int NT, int GS>
+// Buffers for the warps' shares: two in turn, so that one barrier is enough, or one and a barrier more (two blocks an SM have to fit).
+__host__ __device__ constexpr int rows_buffers(int nt) { return nt < 4 ? 2 : 1; }
+
+// XT: what x is.  NT: tiles of eight rows of x.  GS: log2 of the group.  R: neighbouring slabs a warp takes together (a "slab" below is
+// R of them, a unit 4 / R chunks of each): the same columns' operands for both.
+template <int XT, int NT, int GS, int R>
 __global__ void __maxnreg__(128) gemm_w4_rows_kernel(GwArgs a) {
-  constexpr int P = XParts<XT>::N, COLS = 8 * NT, XB = XT == X_F32 ? 4 : 2;      // XB: bytes of an element of x
+  constexpr int UNIT = 4 / R, ROWS = R * W4_SLAB, P = XParts<XT>::N, COLS = 8 * NT, XB = XT == X_F32 ? 4 : 2;      // XB: bytes of an element of x
   extern __shared__ __align__(16) unsigned char smem[];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB, m0 = blockIdx.y * COLS, cols = min(a.M - m0, COLS);
+  const int all_slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB, slabs = (all_slabs + R - 1) / R, m0 = blockIdx.y * COLS, cols = min(a.M - m0, COLS);
   const int first = (int)((long long)slabs * blockIdx.x / gridDim.x), end = (int)((long long)slabs * (blockIdx.x + 1) / gridDim.x);
   const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * GW_DEPTH * GW_SLOT;
-  float* red = reinterpret_cast<float*>(smem + (size_t)warps * GW_DEPTH * GW_SLOT);      // [2][warps][COLS][17]
-  const int units = (a.w.chunks + GW_UNIT - 1) / GW_UNIT;
-  constexpr int SCALES = 256 >> GS;                         // groups a unit
+  float* red = reinterpret_cast<float*>(smem + (size_t)warps * GW_DEPTH * GW_SLOT);      // [buffers][warps][COLS][ROWS + 1]
+  const int units = (a.w.chunks + UNIT - 1) / UNIT;
+  constexpr int SCALES = (UNIT * W4_CHUNK) >> GS;           // groups a unit
   // what is fetched next: of which segment, how many units are left of it (a unit that ends behind the slab's last chunk takes what lies
   // behind it along)
   int f_slab = first, f_left = 0;
   unsigned f_at = ring + lane * 16;
   const uint4* fq = a.w.q;
   const unsigned* fs = a.w.s;
+  size_t q2 = 0, s2 = 0;                                    // to the second slab
   auto fetch = [&]() {
     while (f_left == 0 && f_slab < end) {
       const Segment n = next_segment(f_slab, end - f_slab, warp, warps, units);
       f_slab += n.t;
       f_left = n.hi - n.lo;
-      fq = a.w.q + ((size_t)n.slab * a.w.chunks + n.lo * GW_UNIT) * 32 + lane;
-      fs = a.w.s + ((size_t)n.slab * a.w.groups + n.lo * SCALES) * 8 + 4 * lane;
+      fq = a.w.q + ((size_t)(R * n.slab) * a.w.chunks + n.lo * UNIT) * 32 + lane;
+      fs = a.w.s + ((size_t)(R * n.slab) * a.w.groups + n.lo * SCALES) * 8 + 4 * lane;
+      if (R == 2 && 2 * n.slab + 1 < all_slabs) { q2 = (size_t)a.w.chunks * 32; s2 = (size_t)a.w.groups * 8; }
+      else q2 = s2 = 0;                                      // (an odd slab's neighbour is itself)
     }
     if (f_left > 0) {
-      cp_async16<0, 0>(f_at, fq); cp_async16<512, 512>(f_at, fq); cp_async16<1024, 1024>(f_at, fq); cp_async16<1536, 1536>(f_at, fq);
-      if (lane < 2 * SCALES) cp_async16<GW_UNIT * 512, 0>(f_at, fs);
-      fq += GW_UNIT * 32; fs += SCALES * 8;
+      cp_async16<0, 0>(f_at, fq); cp_async16<512, 512>(f_at, fq);
+      if (R == 1) { cp_async16<1024, 1024>(f_at, fq); cp_async16<1536, 1536>(f_at, fq); }
+      else { cp_async16<1024, 0>(f_at, fq + q2); cp_async16<1536, 512>(f_at, fq + q2); }
+      if (lane < 2 * SCALES) {
+        cp_async16<2048, 0>(f_at, fs);
+        if (R == 2) cp_async16<2048 + 128, 0>(f_at, fs + s2);
+      }
+      fq += UNIT * 32; fs += SCALES * 8;
       --f_left;
     }
     cp_commit();
@@ -160,14 +170,16 @@ __global__ void __maxnreg__(128) gemm_w4_rows_kernel(GwArgs a) {
   for (int t = 0; t < NT; ++t) xrow[t] = (const unsigned char*)a.x + (size_t)(m0 + min(8 * t + g, cols - 1)) * a.ldx * XB + c * 8 * XB;
   unsigned at = ring;
   int turn = 0;
-  for (int next = first; next < end; turn ^= 1) {
+  for (int next = first; next < end; turn ^= rows_buffers(NT) - 1) {
     const Segment seg = next_segment(next, end - next, warp, warps, units);
     next += seg.t;
-    float total[NT][4], part[NT][4];
+    float total[R][NT][4], part[R][NT][4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int k = 0; k < R; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) total[t][i] = 0.f;
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) total[k][t][i] = 0.f;
     // chunk i of unit u, whose elements of x lie from `xu` on
     auto chunk = [&](auto idx, int u, const unsigned char* const* xu, auto full) {
       constexpr int i = decltype(idx)::value;
@@ -176,33 +188,38 @@ __global__ void __maxnreg__(128) gemm_w4_rows_kernel(GwArgs a) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          load_x8<XT, decltype(full)::value>(xu[t] + (i * W4_CHUNK + h * 32) * XB, a.w.K - (u * GW_UNIT + i) * W4_CHUNK - h * 32 - c * 8, b[h][t]);
-      const uint4 qv = lds128<i * 512>(at + lane * 16);
-      const unsigned word[4] = {qv.x, qv.y, qv.z, qv.w};
+          load_x8<XT, decltype(full)::value>(xu[t] + (i * W4_CHUNK + h * 32) * XB, a.w.K - (u * UNIT + i) * W4_CHUNK - h * 32 - c * 8, b[h][t]);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int k = 0; k < R; ++k) {
+        const uint4 qv = k ? lds128<i * 512 + 1024>(at + lane * 16) : lds128<i * 512>(at + lane * 16);
+        const unsigned word[4] = {qv.x, qv.y, qv.z, qv.w};
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          unsigned w[4];
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) w[r] = w4_pair(word[2 * h + j], r);
+          for (int j = 0; j < 2; ++j) {
+            unsigned w[4];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
+            for (int r = 0; r < 4; ++r) w[r] = w4_pair(word[2 * h + j], r);
 #pragma unroll
-            for (int p = P - 1; p >= 0; --p) {
-              if (j == 0 && p == P - 1 && (GS == 5 || (h == 0 && (GS == 6 || !(i & 1))))) mma_bf16_first(part[t], w, b[h][t][p][0], b[h][t][p][1]);
-              else mma_bf16(part[t], w, b[h][t][p][2 * j], b[h][t][p][2 * j + 1]);
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+              for (int p = P - 1; p >= 0; --p) {
+                if (j == 0 && p == P - 1 && (GS == 5 || (h == 0 && (GS == 6 || !(i & 1))))) mma_bf16_first(part[k][t], w, b[h][t][p][0], b[h][t][p][1]);
+                else mma_bf16(part[k][t], w, b[h][t][p][2 * j], b[h][t][p][2 * j + 1]);
+              }
             }
           }
-        }
-        if (GS == 5 || (h == 1 && (GS == 6 || (i & 1) || (!decltype(full)::value && u * GW_UNIT + i == a.w.chunks - 1)))) {
-          const unsigned sv = GS == 5 ? (h ? lds32<GW_UNIT * 512 + (2 * i + 1) * 32>(at + g * 4) : lds32<GW_UNIT * 512 + 2 * i * 32>(at + g * 4))
-                                      : lds32<GW_UNIT * 512 + (GS == 6 ? i : i >> 1) * 32>(at + g * 4);
-          const float s0 = w4_scale_lo(sv), s1 = w4_scale_hi(sv);
+          if (GS == 5 || (h == 1 && (GS == 6 || (i & 1) || (!decltype(full)::value && u * UNIT + i == a.w.chunks - 1)))) {
+            constexpr int S0 = 2048 + (GS == 5 ? 2 * i : GS == 6 ? i : i >> 1) * 32;
+            const unsigned sa = at + g * 4 + (k ? 128u : 0u), sv = GS == 5 && h ? lds32<S0 + 32>(sa) : lds32<S0>(sa);
+            const float s0 = w4_scale_lo(sv), s1 = w4_scale_hi(sv);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            total[t][0] = fmaf(s0, part[t][0], total[t][0]); total[t][1] = fmaf(s0, part[t][1], total[t][1]);
-            total[t][2] = fmaf(s1, part[t][2], total[t][2]); total[t][3] = fmaf(s1, part[t][3], total[t][3]);
+            for (int t = 0; t < NT; ++t) {
+              float* to = total[k][t];
+              const float* from = part[k][t];
+              to[0] = fmaf(s0, from[0], to[0]); to[1] = fmaf(s0, from[1], to[1]);
+              to[2] = fmaf(s1, from[2], to[2]); to[3] = fmaf(s1, from[3], to[3]);
+            }
           }
         }
       }
@@ -213,36 +230,39 @@ __global__ void __maxnreg__(128) gemm_w4_rows_kernel(GwArgs a) {
       fetch();                                               // over that one
       const unsigned char* xu[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) xu[t] = xrow[t] + (size_t)u * (GW_UNIT * W4_CHUNK * XB);
-      if ((u + 1) * GW_UNIT * W4_CHUNK <= a.w.K) {
+      for (int t = 0; t < NT; ++t) xu[t] = xrow[t] + (size_t)u * (UNIT * W4_CHUNK * XB);
+      if ((u + 1) * UNIT * W4_CHUNK <= a.w.K) {
         chunk(Int<0>(), u, xu, TrueType()); chunk(Int<1>(), u, xu, TrueType());
-        chunk(Int<2>(), u, xu, TrueType()); chunk(Int<3>(), u, xu, TrueType());
+        if (R == 1) { chunk(Int<2 / R>(), u, xu, TrueType()); chunk(Int<3 / R>(), u, xu, TrueType()); }
       } else {
         chunk(Int<0>(), u, xu, FalseType());
-        if (u * GW_UNIT + 1 < a.w.chunks) chunk(Int<1>(), u, xu, FalseType());
-        if (u * GW_UNIT + 2 < a.w.chunks) chunk(Int<2>(), u, xu, FalseType());
-        if (u * GW_UNIT + 3 < a.w.chunks) chunk(Int<3>(), u, xu, FalseType());
+        if (u * UNIT + 1 < a.w.chunks) chunk(Int<1>(), u, xu, FalseType());
+        if (R == 1 && u * UNIT + 2 < a.w.chunks) chunk(Int<2 / R>(), u, xu, FalseType());
+        if (R == 1 && u * UNIT + 3 < a.w.chunks) chunk(Int<3 / R>(), u, xu, FalseType());
       }
       at = at == ring + (GW_DEPTH - 1) * GW_SLOT ? ring : at + GW_SLOT;
     }
-    // the warps' shares together: two buffers in turn, so that one barrier is enough
-    float* mine = red + ((size_t)(turn * warps + warp) * COLS) * 17;
+    // the warps' shares together
+    if (rows_buffers(NT) == 1) __syncthreads();
+    float* mine = red + ((size_t)(turn * warps + warp) * COLS) * (ROWS + 1);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float* p = mine + (8 * t + 2 * c) * 17 + g;
-      if (8 * t + 2 * c < cols) { p[0] = total[t][0]; p[8] = total[t][2]; }
-      if (8 * t + 2 * c + 1 < cols) { p[17] = total[t][1]; p[25] = total[t][3]; }
-    }
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float* p = mine + (8 * t + 2 * c) * (ROWS + 1) + k * W4_SLAB + g;
+        if (8 * t + 2 * c < cols) { p[0] = total[k][t][0]; p[8] = total[k][t][2]; }
+        if (8 * t + 2 * c + 1 < cols) { p[ROWS + 1] = total[k][t][1]; p[ROWS + 9] = total[k][t][3]; }
+      }
     if (seg.share == 1) __syncwarp();
     else __syncthreads();
     const int sub = warp & (seg.share - 1);
-    for (int i = 32 * sub + lane; i < ((cols + 1) & ~1) * W4_SLAB; i += 32 * seg.share) {         // (a warp takes two rows of x)
-      const int t = i / W4_SLAB, r = i % W4_SLAB, m = m0 + t, slab = seg.slab, n = slab * W4_SLAB + r;
-      const float* p = red + ((size_t)(turn * warps + warp - sub) * COLS + t) * 17 + r;
+    for (int i = 32 * sub + lane; i < (R == 2 ? cols : (cols + 1) & ~1) * ROWS; i += 32 * seg.share) {      // (whole warps: one row of x or two)
+      const int t = i / ROWS, r = i % W4_SLAB, m = m0 + t, slab = R * seg.slab + (R == 2 ? (i / W4_SLAB) & 1 : 0), n = slab * W4_SLAB + r;
+      const float* p = red + ((size_t)(turn * warps + warp - sub) * COLS + t) * (ROWS + 1) + i % ROWS;
       float v = 0.f;
-      for (int w = 0; w < seg.share; ++w) v += p[w * COLS * 17];
+      for (int w = 0; w < seg.share; ++w) v += p[w * COLS * (ROWS + 1)];
       if (a.bias && n < a.w.N) v += a.bias[n];
-      if (a.epi == EPI_SWIGLU) {
+      if (a.epi == W4_SWIGLU) {
         const float up = __shfl_down_sync(0xffffffffu, v, 8);
         if (r < 8 && t < cols && n < a.w.N) put(a, m, slab * 8 + r, glu_act(v, up, 0.f, 1.f));
       } else if (t < cols && n < a.w.N) put(a, m, n, v);
@@ -250,11 +270,11 @@ __global__ void __maxnreg__(128) gemm_w4_rows_kernel(GwArgs a) {
   }
 }
 
-template <int XT, int NT, int GS>
+template <int XT, int NT, int GS, int R>
 static int launch_rows(const GwArgs& a, cudaStream_t stream) {
-  const int slabs = ceil_div(a.w.N, W4_SLAB), units = ceil_div(a.w.chunks, GW_UNIT), n_sm = fellm_sm_count(), tiles = ceil_div(a.M, 8 * NT);
-  auto kern = gemm_w4_rows_kernel<XT, NT, GS>;
-  auto bytes = [](int warps) { return (size_t)warps * (GW_DEPTH * GW_SLOT + 2 * 8 * NT * 17 * 4); };
+  const int slabs = ceil_div(ceil_div(a.w.N, W4_SLAB), R), units = ceil_div(a.w.chunks, 4 / R), n_sm = fellm_sm_count(), tiles = ceil_div(a.M, 8 * NT);
+  auto kern = gemm_w4_rows_kernel<XT, NT, GS, R>;
+  auto bytes = [](int warps) { return (size_t)warps * (GW_DEPTH * GW_SLOT + rows_buffers(NT) * 8 * NT * (R * W4_SLAB + 1) * 4); };
   static int resident = 0;                              // blocks of eight warps an SM holds, asked once
   if (!resident) {
     int n = 0;
@@ -270,22 +290,22 @@ static int launch_rows(const GwArgs& a, cudaStream_t stream) {
   if (grid.y > 65535) return FELLM_ERR_SIZE;
   return launch_k_class(1, kern, grid, dim3(warps * 32, 1, 1), bytes(warps), stream, 1, a);
 }
-template <int XT, int NT>
+template <int XT, int NT, int R>
 static int launch_rows_group(const GwArgs& a, cudaStream_t stream) {
-  return a.w.gshift == 5 ? launch_rows<XT, NT, 5>(a, stream) : a.w.gshift == 6 ? launch_rows<XT, NT, 6>(a, stream) : launch_rows<XT, NT, 7>(a, stream);
+  return a.w.gshift == 5 ? launch_rows<XT, NT, 5, R>(a, stream) : a.w.gshift == 6 ? launch_rows<XT, NT, 6, R>(a, stream) : launch_rows<XT, NT, 7, R>(a, stream);
 }
 
 // x [M, K] (x_bf16: bfloat16, else float32), out [M, N] ([M, N/2] for the gated form, whose rows are 8 gate, 8 up, ...).
-FELLM_API int fellm_gemm_w4(const void* x, int x_bf16, long long ldx, const void* q, const void* s, const float* bias, void* out, int out_bf16,
-                            long long ldo, int epi, int M, int N, int K, int chunks, int groups, int gshift, cudaStream_t stream) {
+FELLM_API int fellm_gemm_w4(const void* x, long long ldx, const W4Ref* w, const float* bias, void* out, long long ldo, int flags, int M, cudaStream_t stream) {
   if (M <= 0) return 0;
-  if (!x || !q || !s || !out) return FELLM_ERR_ARG;
-  if (N < 1 || K < 1 || gshift < 5 || gshift > 7 || chunks != ceil_div(K, W4_CHUNK)) return FELLM_ERR_SIZE;
-  if (groups != (int)(((long long)chunks * W4_CHUNK + (1 << gshift) - 1) >> gshift)) return FELLM_ERR_SIZE;
-  if (epi != EPI_STORE && epi != EPI_ACC && epi != EPI_SWIGLU && epi != EPI_F32 && epi != EPI_RELU2) return FELLM_ERR_ARG;
-  if (epi == EPI_SWIGLU && N % W4_SLAB) return FELLM_ERR_SIZE;
-  const GwArgs a = {{(const uint4*)q, (const unsigned*)s, N, K, chunks, groups, gshift}, x, bias, out, ldx, ldo, M, epi, out_bf16};
-  if (!x_bf16) return launch_rows_group<X_F32, 1>(a, stream);
-  if (K % 8 || ldx % 8 || ((uintptr_t)x & 15)) return launch_rows_group<X_BF16_ANY, 1>(a, stream);
-  return M <= 8 ? launch_rows_group<X_BF16, 1>(a, stream) : M <= 16 ? launch_rows_group<X_BF16, 2>(a, stream) : launch_rows_group<X_BF16, 4>(a, stream);
+  if (!x || !out) return FELLM_ERR_ARG;
+  if (int e = w4_check(w)) return e;
+  if (int e = w4_check_epi(flags, w->N)) return e;
+  const int x_bf16 = flags & W4_X_BF16, N = w->N, K = w->K;
+  const GwArgs a = {*w, x, bias, out, ldx, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0};
+  if (!x_bf16) return launch_rows_group<X_F32, 1, 1>(a, stream);
+  if (K % 8 || ldx % 8 || ((uintptr_t)x & 15)) return launch_rows_group<X_BF16_ANY, 1, 1>(a, stream);
+  if (M <= 8) return launch_rows_group<X_BF16, 1, 1>(a, stream);
+  if (M <= 16) return N <= 2048 ? launch_rows_group<X_BF16, 2, 1>(a, stream) : launch_rows_group<X_BF16, 2, 2>(a, stream);
+  return launch_rows_group<X_BF16, 4, 2>(a, stream);
 }

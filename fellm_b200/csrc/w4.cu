@@ -259,53 +259,43 @@ __global__ void __launch_bounds__(W4_THREADS) embed_rows_w4_kernel(const int* to
   store8(out + (size_t)t * m.K + k, v, m.K - k, vec != 0);
 }
 
-static int check_sizes(int N, int K, int chunks, int groups, int gshift) {
-  if (N < 1 || K < 1 || gshift < 5 || gshift > 7 || chunks != ceil_div(K, W4_CHUNK)) return FELLM_ERR_SIZE;
-  if (groups != (int)(((long long)chunks * W4_CHUNK + (1 << gshift) - 1) >> gshift)) return FELLM_ERR_SIZE;
-  return 0;
-}
 static bool grid_ok(long long blocks) { return blocks > 0 && blocks < (1ll << 31); }
 
-FELLM_API int fellm_quantize_w4(const void* w, int w_bf16, long long ldw, void* q, void* s, int N, int K, int chunks, int groups, int gshift, cudaStream_t stream) {
-  if (!w || !q || !s) return FELLM_ERR_ARG;
-  if (int e = check_sizes(N, K, chunks, groups, gshift)) return e;
-  const W4Out o = {(uint4*)q, (unsigned*)s, N, K, chunks, groups, gshift};
-  const long long units = (long long)ceil_div(N, W4_SLAB) * ((chunks + 1) / 2), blocks = (units + W4_THREADS / 32 - 1) / (W4_THREADS / 32);
+FELLM_API int fellm_quantize_w4(const void* w, int w_bf16, long long ldw, const W4Ref* m, cudaStream_t stream) {
+  if (!w) return FELLM_ERR_ARG;
+  if (int e = w4_check(m)) return e;
+  const W4Out o = {(uint4*)m->q, (unsigned*)m->s, m->N, m->K, m->chunks, m->groups, m->gshift};
+  const long long units = (long long)ceil_div(m->N, W4_SLAB) * ((m->chunks + 1) / 2), blocks = (units + W4_THREADS / 32 - 1) / (W4_THREADS / 32);
   if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
   if (w_bf16) quantize_w4_kernel<bf16><<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const bf16*)w, ldw, ldw % 8 == 0 && ((uintptr_t)w & 15) == 0, o);
   else quantize_w4_kernel<float><<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const float*)w, ldw, ldw % 4 == 0 && ((uintptr_t)w & 15) == 0, o);
   return launch_status();
 }
-FELLM_API int fellm_pack_w4(const void* levels, long long ldl, const void* scales, long long lds, int groups_in, void* q, void* s, int N, int K,
-                            int chunks, int groups, int gshift, int* bad, cudaStream_t stream) {
-  if (!levels || !scales || !q || !s || !bad) return FELLM_ERR_ARG;
-  if (int e = check_sizes(N, K, chunks, groups, gshift)) return e;
-  const W4Out o = {(uint4*)q, (unsigned*)s, N, K, chunks, groups, gshift};
-  const long long units = (long long)ceil_div(N, W4_SLAB) * chunks, blocks = (units + W4_THREADS / 32 - 1) / (W4_THREADS / 32);
+FELLM_API int fellm_pack_w4(const void* levels, long long ldl, const void* scales, long long lds, int groups_in, const W4Ref* m, int* bad, cudaStream_t stream) {
+  if (!levels || !scales || !bad) return FELLM_ERR_ARG;
+  if (int e = w4_check(m)) return e;
+  const W4Out o = {(uint4*)m->q, (unsigned*)m->s, m->N, m->K, m->chunks, m->groups, m->gshift};
+  const long long units = (long long)ceil_div(m->N, W4_SLAB) * m->chunks, blocks = (units + W4_THREADS / 32 - 1) / (W4_THREADS / 32);
   if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
   pack_w4_kernel<<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const signed char*)levels, ldl, (const bf16*)scales, lds, o, groups_in, bad);
   return launch_status();
 }
-FELLM_API int fellm_dequantize_w4(const void* q, const void* s, void* out, int out_bf16, long long ldo, int N, int K, int chunks, int groups, int gshift,
-                                  cudaStream_t stream) {
-  if (!q || !s || !out) return FELLM_ERR_ARG;
-  if (int e = check_sizes(N, K, chunks, groups, gshift)) return e;
-  const W4Ref m = {(const uint4*)q, (const unsigned*)s, N, K, chunks, groups, gshift};
-  const long long blocks = ((long long)N * ceil_div(K, 8) + W4_THREADS - 1) / W4_THREADS;
+FELLM_API int fellm_dequantize_w4(const W4Ref* m, void* out, int out_bf16, long long ldo, cudaStream_t stream) {
+  if (!out) return FELLM_ERR_ARG;
+  if (int e = w4_check(m)) return e;
+  const long long blocks = ((long long)m->N * ceil_div(m->K, 8) + W4_THREADS - 1) / W4_THREADS;
   if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
   const int vec = ldo % (out_bf16 ? 8 : 4) == 0 && ((uintptr_t)out & 15) == 0;
-  if (out_bf16) dequantize_w4_kernel<bf16><<<(unsigned)blocks, W4_THREADS, 0, stream>>>(m, (bf16*)out, ldo, vec);
-  else dequantize_w4_kernel<float><<<(unsigned)blocks, W4_THREADS, 0, stream>>>(m, (float*)out, ldo, vec);
+  if (out_bf16) dequantize_w4_kernel<bf16><<<(unsigned)blocks, W4_THREADS, 0, stream>>>(*m, (bf16*)out, ldo, vec);
+  else dequantize_w4_kernel<float><<<(unsigned)blocks, W4_THREADS, 0, stream>>>(*m, (float*)out, ldo, vec);
   return launch_status();
 }
-FELLM_API int fellm_embed_rows_w4(const int* tokens, const void* q, const void* s, void* out, int T, int N, int K, int chunks, int groups, int gshift,
-                                  int* status, float scale, cudaStream_t stream) {
+FELLM_API int fellm_embed_rows_w4(const int* tokens, const W4Ref* m, void* out, int T, int* status, float scale, cudaStream_t stream) {
   if (T <= 0) return 0;
-  if (!tokens || !q || !s || !out) return FELLM_ERR_ARG;
-  if (int e = check_sizes(N, K, chunks, groups, gshift)) return e;
-  const W4Ref m = {(const uint4*)q, (const unsigned*)s, N, K, chunks, groups, gshift};
-  const long long blocks = ((long long)T * ceil_div(K, 8) + W4_THREADS - 1) / W4_THREADS;
+  if (!tokens || !out) return FELLM_ERR_ARG;
+  if (int e = w4_check(m)) return e;
+  const long long blocks = ((long long)T * ceil_div(m->K, 8) + W4_THREADS - 1) / W4_THREADS;
   if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
   return launch_k_class(launch_class_for_rows(T, 2), embed_rows_w4_kernel, dim3((unsigned)blocks, 1, 1), dim3(W4_THREADS, 1, 1), 0, stream, 1,
-                        tokens, m, (float*)out, T, (int)(K % 4 == 0 && ((uintptr_t)out & 15) == 0), status, scale);
+                        tokens, *m, (float*)out, T, (int)(m->K % 4 == 0 && ((uintptr_t)out & 15) == 0), status, scale);
 }

@@ -24,6 +24,7 @@
 #define W4_CHUNK 64
 #define W4_READ_AHEAD 32
 
+// (the caller keeps one of these with the matrix and hands its address to the launchers)
 struct W4Ref {
   const uint4* q;            // [slabs][chunks][32]
   const unsigned* s;         // [slabs][groups][8]
@@ -55,4 +56,18 @@ __device__ __forceinline__ void w4_split3(float v, unsigned& a, unsigned& b, uns
   b = __float_as_uint(r) & 0xffff0000u;
   c = __float_as_uint(r - __uint_as_float(b)) & 0xffff0000u;
   if ((u & 0x7f800000u) == 0x7f800000u && (u & 0x7fffffu)) a |= 0x400000u;                 // a NaN whose high bits are those of an infinity
+}
+
+static inline int w4_check(const W4Ref* w) {
+  if (!w || !w->q || !w->s) return FELLM_ERR_ARG;
+  if (w->N < 1 || w->K < 1 || w->gshift < 5 || w->gshift > 7 || w->chunks != ceil_div(w->K, W4_CHUNK)) return FELLM_ERR_SIZE;
+  return w->groups == (int)(((long long)w->chunks * W4_CHUNK + (1 << w->gshift) - 1) >> w->gshift) ? 0 : FELLM_ERR_SIZE;
+}
+
+// What a product does with its sums, and the types beside it, as the launchers are told.
+enum { W4_STORE = 0, W4_ACC = 1, W4_SWIGLU = 2, W4_RELU2 = 6, W4_EPI = 0xff, W4_X_BF16 = 0x100, W4_OUT_BF16 = 0x200 };
+static inline int w4_check_epi(int flags, int N) {
+  const int epi = flags & W4_EPI;
+  if (epi != W4_STORE && epi != W4_ACC && epi != W4_SWIGLU && epi != W4_RELU2) return FELLM_ERR_ARG;
+  return epi == W4_SWIGLU && N % W4_SLAB ? FELLM_ERR_SIZE : 0;
 }

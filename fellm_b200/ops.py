@@ -1982,21 +1982,24 @@ W4_READ_AHEAD = 32                       # chunks behind the end of a matrix tha
 W4_FEW_ROWS = 16                         # up to so many rows: mma.sync, a warp a slab of 16 weight rows; more: tcgen05
 
 
+class _W4Ref(ctypes.Structure):
+    """csrc/w4.h W4Ref: what a launcher is told of a matrix, in one pointer."""
+    _fields_ = [("q", _c_p), ("s", _c_p), ("N", _c_int), ("K", _c_int), ("chunks", _c_int), ("groups", _c_int), ("gshift", _c_int)]
+
+
 class W4:
     """A matrix [N, K] in four bits: w[n, k] = level[n, k] * scale[n, k // group], levels -8..7, scales of at most five
     significant bits (level * scale is a bfloat16 number exactly, so every kernel that reads the matrix multiplies with the
     same numbers).  Made by quantize_w4 or pack_w4, which return when it is laid out: any stream may read it, and a product
     may ask for it before the kernel in front has ended.  q, scales: the kernels' layout (csrc/w4.h); nothing writes them again."""
     dtype = "int4"                          # (of no torch dtype: what asks a matrix for bfloat16 leaves it alone)
-    is_cuda = True
 
     def __init__(self, q, scales, N: int, K: int, group: int):
         self.q, self.scales, self.shape, self.group = q, scales, (N, K), group
-        self._sizes = (N, K, q.shape[1], scales.shape[1], group.bit_length() - 1)        # as the launchers take them
-
-    @property
-    def device(self):
-        return self.q.device
+        self.device, self.is_cuda = q.device, q.is_cuda
+        self._device = q.get_device()
+        self._ref = _W4Ref(q.data_ptr(), scales.data_ptr(), N, K, q.shape[1], scales.shape[1], group.bit_length() - 1)
+        self._at = ctypes.addressof(self._ref)
 
     def nbytes(self) -> int:
         return 4 * (self.q.numel() + self.scales.numel())
@@ -2048,8 +2051,8 @@ def quantize_w4(w, group: int = 64) -> W4:
     _w4_dev(w)
     _w4_laid_out("quantize_w4")
     out = W4(q, s, w.shape[0], w.shape[1], group)
-    f = _fn("w4", "fellm_quantize_w4", [_c_p, _c_int, _c_ll, _c_p, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p])
-    _check(f(_p(w), _is_bf16(w), w.stride(0), _p(q), _p(s), *out._sizes, _stream()), "quantize_w4")
+    f = _fn("w4", "fellm_quantize_w4", [_c_p, _c_int, _c_ll, _c_p, _c_p])
+    _check(f(_p(w), _is_bf16(w), w.stride(0), out._at, _stream()), "quantize_w4")
     torch.cuda.current_stream().synchronize()
     return out
 
@@ -2074,8 +2077,8 @@ def pack_w4(levels, scales, group: int) -> W4:
     kept = kept.contiguous()
     out = W4(q, s, N, K, group)
     bad = torch.zeros(1, dtype=torch.int32, device=levels.device)
-    f = _fn("w4", "fellm_pack_w4", [_c_p, _c_ll, _c_p, _c_ll, _c_int, _c_p, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p])
-    _check(f(_p(levels), levels.stride(0), _p(kept), kept.stride(0), kept.shape[1], _p(q), _p(s), *out._sizes, _p(bad), _stream()), "pack_w4")
+    f = _fn("w4", "fellm_pack_w4", [_c_p, _c_ll, _c_p, _c_ll, _c_int, _c_p, _c_p, _c_p])
+    _check(f(_p(levels), levels.stride(0), _p(kept), kept.stride(0), kept.shape[1], out._at, _p(bad), _stream()), "pack_w4")
     code = int(bad.item())
     if code & 1:
         raise KernelError("pack_w4: levels outside -8..7")
@@ -2092,9 +2095,8 @@ def dequantize_w4(w: W4, out_dtype=torch.bfloat16, out=None):
     if tuple(out.shape) != w.shape:
         raise KernelError(f"dequantize_w4: a matrix of {list(w.shape)} does not fit {list(out.shape)}")
     _w4_dev(w.q, out)
-    N, K, chunks, groups, gshift = w._sizes
-    f = _fn("w4", "fellm_dequantize_w4", [_c_p, _c_p, _c_p, _c_int, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p])
-    _check(f(_p(w.q), _p(w.scales), _p(out), _is_bf16(out), out.stride(0), N, K, chunks, groups, gshift, _stream()), "dequantize_w4")
+    f = _fn("w4", "fellm_dequantize_w4", [_c_p, _c_p, _c_int, _c_ll, _c_p])
+    _check(f(w._at, _p(out), _is_bf16(out), out.stride(0), _stream()), "dequantize_w4")
     return out
 
 
@@ -2105,8 +2107,8 @@ def embed_rows_w4(tokens, table: W4, out, status=None, scale: float = 1.0):
     if out.dtype != torch.float32 or not out.is_contiguous() or tuple(out.shape) != (T, table.shape[1]):
         raise KernelError(f"embed_rows_w4: out must be contiguous float32 [{T}, {table.shape[1]}]")
     _w4_dev(tokens, table.q, out, status)
-    f = _fn("w4", "fellm_embed_rows_w4", [_c_p, _c_p, _c_p, _c_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_f, _c_p])
-    _check(f(_p(tokens), _p(table.q), _p(table.scales), _p(out), T, *table._sizes, _p(status), float(scale), _stream()), "embed_rows_w4")
+    f = _fn("w4", "fellm_embed_rows_w4", [_c_p, _c_p, _c_p, _c_int, _c_p, _c_f, _c_p])
+    _check(f(_p(tokens), table._at, _p(out), T, _p(status), scale, _stream()), "embed_rows_w4")
     return out
 
 
@@ -2115,55 +2117,69 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
     bfloat16 for bfloat16 x unless out or out_dtype says float32, and float32 for float32 x.
     accumulate: out (float32 [M, N]) += ; swiglu: w's rows are interleaved in blocks of 8 gate / 8 up (interleave_gate_up)
     and the result [M, N/2] is silu(gate) * up; act="relu2": the result is max(., 0)^2."""
-    if x.dim() != 2 or x.shape[1] != w.shape[1]:
-        raise KernelError(f"gemm_w4: x is {list(x.shape)} but w is {list(w.shape)}")
-    M, K = x.shape
-    N = w.shape[0]
-    x_bf16 = _is_bf16(x)
-    if K > 1 and x.stride(1) != 1:
-        raise KernelError(f"gemm_w4: x's rows must be contiguous, its strides are {list(x.stride())}")
-    if accumulate + swiglu + (act is not None) > 1:
-        raise KernelError("gemm_w4: one of accumulate, swiglu and act")
-    if act not in (None, "relu2"):
-        raise KernelError(f"gemm_w4: unknown activation {act!r}")
-    if swiglu and N % 16:
-        raise KernelError(f"gemm_w4: the gate/up matrix needs a multiple of 16 rows, got {N}")
-    if accumulate and out is None:
-        raise KernelError("gemm_w4: accumulate needs the tensor to add into")
-    cols = N // 2 if swiglu else N
+    N, K = w.shape
+    size = x.shape
+    if len(size) != 2 or size[1] != K:
+        raise KernelError(f"gemm_w4: x is {list(size)} but w is {[N, K]}")
+    M, dt = size[0], x.dtype
+    x_bf16 = dt is torch.bfloat16
+    if not x_bf16:
+        _is_bf16(x)
+    ldx, step = x.stride()
+    if step != 1 and K > 1:
+        raise KernelError(f"gemm_w4: x's rows must be contiguous, its strides are {[ldx, step]}")
+    flags, cols = (_W4_X_BF16 if x_bf16 else 0), N
+    if accumulate or swiglu or act is not None:
+        if accumulate + swiglu + (act is not None) > 1:
+            raise KernelError("gemm_w4: one of accumulate, swiglu and act")
+        if act not in (None, "relu2"):
+            raise KernelError(f"gemm_w4: unknown activation {act!r}")
+        if swiglu and N % 16:
+            raise KernelError(f"gemm_w4: the gate/up matrix needs a multiple of 16 rows, got {N}")
+        if accumulate and out is None:
+            raise KernelError("gemm_w4: accumulate needs the tensor to add into")
+        flags |= _EPI_ACC if accumulate else _EPI_SWIGLU if swiglu else _EPI_RELU2
+        if swiglu:
+            cols = N // 2
     if out is None:
-        out = torch.empty((M, cols), dtype=out_dtype or x.dtype, device=x.device)
-    if out.dim() != 2 or out.shape[0] != M or out.shape[1] != cols or (cols > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < cols):
-        raise KernelError(f"gemm_w4: the result is [{M}, {cols}] with contiguous rows, not {list(out.shape)} with strides {list(out.stride())}")
-    out_bf16 = _is_bf16(out)
-    if out_dtype is not None and out.dtype != out_dtype:
-        raise KernelError(f"gemm_w4: out is {out.dtype}, out_dtype {out_dtype}")
-    if out_bf16 and (accumulate or not x_bf16):
-        raise KernelError("gemm_w4: sums are added to float32, and float32 rows do not round down to a bfloat16 result")
+        odt, ldo = out_dtype or dt, cols
+        if odt is not dt and (odt is not torch.float32):
+            raise KernelError(f"gemm_w4: rows of {dt} do not make a result of {odt}")
+        out = torch.empty((M, cols), dtype=odt, device=x.device)
+    else:
+        if out.dim() != 2 or out.shape[0] != M or out.shape[1] != cols or (cols > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < cols):
+            raise KernelError(f"gemm_w4: the result is {[M, cols]} with contiguous rows, not {list(out.shape)} with strides {list(out.stride())}")
+        odt, ldo = out.dtype, out.stride(0)
+        if out_dtype is not None and odt != out_dtype:
+            raise KernelError(f"gemm_w4: out is {odt}, out_dtype {out_dtype}")
+        if _is_bf16(out) and (accumulate or not x_bf16):
+            raise KernelError("gemm_w4: sums are added to float32, and float32 rows do not round down to a bfloat16 result")
+    if odt is torch.bfloat16:
+        flags |= _W4_OUT_BF16
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != N or not bias.is_contiguous()):
         raise KernelError(f"gemm_w4: the bias is contiguous float32 [{N}]")
-    _w4_dev(x, w.q, bias, out)
+    here = w._device
+    if here < 0 or x.get_device() != here or out.get_device() != here or torch.cuda.current_device() != here or bias is not None:
+        _w4_dev(x, w.q, bias, out)
     if accumulate:
         residual_written(out)
     if M == 0:
         return out
-    epi = _EPI_ACC if accumulate else _EPI_SWIGLU if swiglu else _EPI_RELU2 if act else _EPI_STORE
+    at = x.data_ptr()
     if M > W4_FEW_ROWS:
-        need = _fn("gemm_w4_umma", "fellm_gemm_w4_umma_scratch", [_c_p, _c_int, _c_ll, _c_int, _c_int])
-        need.restype = _c_ll
-        room = need(_p(x), x_bf16, x.stride(0), M, K)
-        scratch = torch.empty(room, dtype=torch.uint8, device=x.device) if room else None
+        scratch = None
+        if not x_bf16 or K % 8 or ldx % 8 or ldx < K or at % 16:       # (what TMA does not read)
+            scratch = torch.empty(M * -(-K // 64) * (64 if x_bf16 else 192), dtype=torch.bfloat16, device=x.device)
         f = _fn("gemm_w4_umma", "fellm_gemm_w4_umma", _GEMM_W4_ARGS[:-1] + [_c_p, _c_p, _c_p])
-        _check(f(_p(x), x_bf16, x.stride(0), _p(w.q), _p(w.scales), _p(bias), _p(out), out_bf16, out.stride(0), epi, M, *w._sizes, _p(scratch),
-                 _p(umma_status(x.device)), _stream()), "gemm_w4_umma")
+        _check(f(at, ldx, w._at, _p(bias), out.data_ptr(), ldo, flags, M, _p(scratch), _p(umma_status(x.device)), _stream()), "gemm_w4_umma")
         return out
     f = _fn("gemm_w4", "fellm_gemm_w4", _GEMM_W4_ARGS)
-    _check(f(_p(x), x_bf16, x.stride(0) if M > 1 else 0, _p(w.q), _p(w.scales), _p(bias), _p(out), out_bf16, out.stride(0) if M > 1 else 0, epi, M,
-             *w._sizes, _stream()), "gemm_w4")
+    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), out.data_ptr(), ldo, flags, M, _stream()), "gemm_w4")
     return out
 
 
-_GEMM_W4_ARGS = [_c_p, _c_int, _c_ll, _c_p, _c_p, _c_p, _c_p, _c_int, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p]
+_W4_X_BF16, _W4_OUT_BF16 = 0x100, 0x200
+_GEMM_W4_ARGS = [_c_p, _c_ll, _c_p, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_p]
 
 
 # ------------------------------------------------------------------------------ attention dispatch
