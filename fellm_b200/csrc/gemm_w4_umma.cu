@@ -13,15 +13,16 @@
 // tile is shared out over a cluster of 2, 4 or 8 CTAs, whose sums are put together through distributed shared memory, in
 // rank order, each rank finishing its share of the columns.
 //
-// Roles in a CTA: warp 0 TMA of x (one lane), warp 1 MMA issuer (one lane) and owner of tensor memory, then one or two sets of
+// Roles in a CTA: warp 0 TMA of x (one lane), warp 1 MMA issuer (one lane) and owner of tensor memory, then two sets of
 // eight warps for weights, the last four warps epilogue (tensor memory lanes 32 (warp % 4) ..).  Every wait on an mbarrier is bounded: after a
-// second a role records itself in `status` (141 x, 142 MMA, 143 weights, 144 epilogue, 145 accumulator) and all roles fall
+// second a role records itself in `status` (141 x, 142 MMA, 143 weights, 144 epilogue, 145 accumulator) and all roles run
 // through to the common exit, where tensor memory is freed.
 #include <cuda.h>
 #include "w4.h"
 
-// SETS: sets of eight warps that make weights, each every SETS-th stage
-constexpr int w4u_threads(int sets) { return 32 * (2 + 8 * sets + 4); }
+#define SETS 2                         // sets of eight warps that make weights, each every other stage (three took registers from one another)
+#define W4U_THREADS (32 * (2 + 8 * SETS + 4))
+#define AHEAD 4                        // stages whose chunks a warp holds in registers ahead of the one it unpacks
 #define W4U_SPIN_LIMIT (1u << 26)
 #define W4U_A_BYTES (128 * 128)        // 128 weight rows x 64 k
 
@@ -36,34 +37,28 @@ __device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity) {
   asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-// Bounded wait: false (and *status set) after some 2^31 cycles, a second.  (By the SM's own clock: reading the global timer
-// takes longer than most waits here.)
-__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, int* status, int code) {
-  if (mbar_try(bar, parity)) return true;
+// Bounded wait: after some 2^31 cycles, a second (by the SM's own clock: reading the global timer takes longer than most waits
+// here), it records `code` and sets `dead`, and from then on no wait of this CTA waits: all roles run through to the common exit,
+// the same way as ever (so that no role's loop has to carry a verdict; what they store is of no use, and the status word says so).
+__device__ __forceinline__ void wait_slow(unsigned bar, unsigned parity, int* status, int code, volatile int* dead, unsigned nap) {
   const long long t0 = clock64();
   for (unsigned i = 0; i < W4U_SPIN_LIMIT; ++i) {
-    if (mbar_try(bar, parity)) return true;
+    if (mbar_try(bar, parity) || *dead) return;
+    if (nap) __nanosleep(nap);
     if ((i & 63) == 63 && clock64() - t0 > (1ll << 31)) break;
   }
+  *dead = 1;
   if (status) atomicExch(status, code);
-  return false;
 }
+#define W4U_WAIT(bar, parity, code) \
+  do { if (!mbar_try(bar, parity)) wait_slow(bar, parity, a.status, code, &dead, 0); } while (0)
 // The epilogue's wait for a finished accumulator, most of a tile's time: one warp asks, now and then (four that ask all the time
-// took a third of the issue slots), the others sleep at a barrier.  False for all four if it ran out.
-__device__ __forceinline__ bool epilogue_wait(unsigned bar, unsigned parity, int* status, int* gave_up, bool asks) {
-  if (asks && !mbar_try(bar, parity)) {
-    const long long t0 = clock64();
-    bool ok = false;
-    for (unsigned i = 0; i < W4U_SPIN_LIMIT && !ok; ++i) {
-      __nanosleep(64);
-      ok = mbar_try(bar, parity);
-      if (clock64() - t0 > (1ll << 31)) break;
-    }
-    if (!ok) { *gave_up = 1; if (status) atomicExch(status, 144); }
-  }
-  asm volatile("bar.sync 1, 128;\n" ::: "memory");
-  return *(volatile int*)gave_up == 0;
-}
+// took a third of the issue slots), the others sleep at a barrier.
+#define W4U_WAIT_EPILOGUE(bar, parity) \
+  do { \
+    if (warp == 2 + 8 * SETS && !mbar_try(bar, parity)) wait_slow(bar, parity, a.status, 144, &dead, 64); \
+    asm volatile("bar.sync 1, 128;\n" ::: "memory"); \
+  } while (0)
 __device__ __forceinline__ void tma_load_2d(unsigned dst, const CUtensorMap* map, int c0, int c1, unsigned bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
                ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
@@ -201,29 +196,25 @@ struct Ring {
   __device__ __forceinline__ void add_many(unsigned n, unsigned stages) { stage += n; parity ^= (stage / stages) & 1u; stage %= stages; }
 };
 
-// KB: chunks of K a stage.
-template <bool SPLIT, int PARTS, int SETS, int KB>
-__global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
-  constexpr int AHEAD = KB == 1 ? 4 : 2;                               // stages whose chunks a warp holds in registers ahead of the one it unpacks
-  constexpr unsigned A_BYTES = KB * W4U_A_BYTES;
+template <bool SPLIT, int PARTS>
+__global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];           // full[8], empty[8], acc_full[2], acc_empty[2]
   __shared__ unsigned tmem_base_s;
-  __shared__ int gave_up;                // the epilogue has
+  __shared__ int dead;                   // a wait gave up
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const unsigned x_bytes = (unsigned)a.bn * 128u, stage_bytes = A_BYTES + KB * x_bytes;
+  const unsigned x_bytes = (unsigned)a.bn * 128u, stage_bytes = W4U_A_BYTES + x_bytes;
   const unsigned full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[8]), accfull0 = smem_u32(&bars[16]), accempty0 = smem_u32(&bars[18]);
   const int m_tiles = (a.M + a.bn - 1) / a.bn, n_tiles = (a.w.N + 127) / 128, total = m_tiles * n_tiles;
   const int rank = SPLIT ? (int)cluster_rank() : 0;
   const int first = SPLIT ? (int)blockIdx.x / a.splits : (int)blockIdx.x, step = SPLIT ? total : (int)gridDim.x;
   // this CTA's chunks of K
-  const int stages_of_k = (a.w.chunks + KB - 1) / KB;
-  const int c_lo = SPLIT ? (int)((long long)stages_of_k * rank / a.splits) * KB : 0, c_hi = SPLIT ? (int)((long long)stages_of_k * (rank + 1) / a.splits) * KB : stages_of_k * KB;
-  const int blocks = (c_hi - c_lo) / KB * PARTS;
+  const int c_lo = SPLIT ? (int)((long long)a.w.chunks * rank / a.splits) : 0, c_hi = SPLIT ? (int)((long long)a.w.chunks * (rank + 1) / a.splits) : a.w.chunks;
+  const int blocks = (c_hi - c_lo) * PARTS;
 
   if (threadIdx.x == 0) {
-    gave_up = 0;
+    dead = 0;
     for (int s = 0; s < a.stages; ++s) { mbar_init(full0 + 8 * s, 1 + 8); mbar_init(empty0 + 8 * s, 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(accfull0 + 8 * b, 1); mbar_init(accempty0 + 8 * b, 4); }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -241,18 +232,16 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
   if (warp == 0) {
     pdl_wait();                                              // x is the output of the kernel before this one
     Ring ring;
-    bool ok = true;
-    for (int t = first; t < total && ok; t += step) {
+    for (int t = first; t < total; t += step) {
       const int m0 = (t % m_tiles) * a.bn;
-      for (int b = 0; b < blocks && ok; ++b) {
-        ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * ring.stage, ring.parity ^ 1u, a.status, 141));
-        if (ok && elect_one()) {
-          mbar_expect_tx(full0 + 8 * ring.stage, KB * x_bytes);
-#pragma unroll
-          for (int i = 0; i < KB; ++i)                       // (behind the end of K: zeros)
-            tma_load_2d(tiles + ring.stage * stage_bytes + A_BYTES + i * x_bytes, &map_x, (c_lo * PARTS + b * KB + i) * W4_CHUNK, m0, full0 + 8 * ring.stage);
-        }
+      for (int b = 0; b < blocks; ++b) {
+        const unsigned full = full0 + 8 * ring.stage;
+        W4U_WAIT(empty0 + 8 * ring.stage, ring.parity ^ 1u, 141);
         __syncwarp();
+        if (elect_one()) {
+          mbar_expect_tx(full, x_bytes);
+          tma_load_2d(tiles + ring.stage * stage_bytes + W4U_A_BYTES, &map_x, (c_lo * PARTS + b) * W4_CHUNK, m0, full);      // (behind the end of K: zeros)
+        }
         ring.add(1, a.stages);
       }
     }
@@ -260,25 +249,19 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
     const unsigned idesc = umma_idesc(128, a.bn), a_lo = umma_desc_lo(tiles);
     unsigned use = 0;
     Ring ring;
-    bool ok = true;
-    for (int t = first; t < total && ok; t += step, ++use) {
+    for (int t = first; t < total; t += step, ++use) {
       const unsigned acc = use & 1, d = tmem_base + acc * acc_cols;
-      if (use >= 2) {
-        ok = __all_sync(0xffffffffu, mbar_wait(accempty0 + 8 * acc, ((use >> 1) - 1) & 1, a.status, 145));
+      if (use >= 2) W4U_WAIT(accempty0 + 8 * acc, ((use >> 1) - 1) & 1, 145);
+      for (int b = 0; b < blocks; ++b) {
+        const unsigned lo = a_lo + ring.stage * (stage_bytes >> 4), empty = empty0 + 8 * ring.stage;
+        W4U_WAIT(full0 + 8 * ring.stage, ring.parity, 142);
+        __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-      }
-      for (int b = 0; b < blocks && ok; ++b) {
-        ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * ring.stage, ring.parity, a.status, 142));
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const unsigned lo = a_lo + ring.stage * (stage_bytes >> 4);
-        if (ok && elect_one()) {
-#pragma unroll
-          for (int i = 0; i < KB; ++i)
-            umma_stage(d, lo + i * (W4U_A_BYTES >> 4), lo + (A_BYTES >> 4) + i * (x_bytes >> 4), idesc, (b | i) ? 1u : 0u);
-          umma_commit(empty0 + 8 * ring.stage);
+        if (elect_one()) {
+          umma_stage(d, lo, lo + (W4U_A_BYTES >> 4), idesc, b ? 1u : 0u);
+          umma_commit(empty);
           if (b == blocks - 1) umma_commit(accfull0 + 8 * acc);
         }
-        __syncwarp();
         ring.add(1, a.stages);
       }
     }
@@ -286,67 +269,57 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
     // weights: nothing in front of this kernel writes them, so they need not wait for it
     const int sl = (warp - 2) & 7, set = (warp - 2) >> 3, g = lane >> 2, c = lane & 3, slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB;
     Ring base;
-    bool ok = true;
     // where the lane's pieces lie in the tile: row 16 sl + g (and + 8: the same swizzle), pieces c and 4 + c of its eight.  Odd rows
     // are written the far piece first, so that eight lanes of a store meet every bank once.
     const bool flip = g & 1, two_scales = a.w.gshift == 5;
     const unsigned row = tiles + (unsigned)(16 * sl + g) * 128u, near = (unsigned)(c ^ g) * 16u, far = (unsigned)((c + 4) ^ g) * 16u;
     const unsigned p0 = row + (flip ? far : near), p1 = row + (flip ? near : far);
-    for (int t = first; t < total && ok; t += step) {
+    for (int t = first; t < total; t += step) {
       const int slab = (t / m_tiles) * 8 + sl;
       const bool have = slab < slabs;
       const uint4* q = a.w.q + ((size_t)(have ? slab : 0) * a.w.chunks + c_lo) * 32 + lane;
       const unsigned* sc = a.w.s + (size_t)(have ? slab : 0) * a.w.groups * 8 + g;
-      uint4 qv[AHEAD][KB];
-      unsigned sv[AHEAD][KB][2];
+      uint4 qv[AHEAD];
+      unsigned sv[AHEAD][2];
       // This set's blocks of the tile: set, set + SETS, ...; `ahead`: the next one to be fetched.  Behind the last one loads go on
       // (into the next slab or the room behind the matrix): a load that may not happen would have to be waited for at once.
       unsigned ahead = set;
       auto fetch = [&](int u) {
-#pragma unroll
-        for (int i = 0; i < KB; ++i) {
-          const unsigned ch = PARTS == 1 ? ahead * KB + i : ahead / 3;
-          qv[u][i] = __ldg(q + ch * 32u);
-          const unsigned* at = sc + ((((unsigned)c_lo + ch) * W4_CHUNK) >> a.w.gshift) * 8u;
-          sv[u][i][0] = __ldg(at);
-          sv[u][i][1] = __ldg(at + (two_scales ? 8 : 0));
-        }
+        const unsigned ch = PARTS == 1 ? ahead : ahead / 3;
+        qv[u] = __ldg(q + ch * 32u);
+        const unsigned* at = sc + ((((unsigned)c_lo + ch) * W4_CHUNK) >> a.w.gshift) * 8u;
+        sv[u][0] = __ldg(at);
+        sv[u][1] = __ldg(at + (two_scales ? 8 : 0));
         ahead += SETS;
       };
       Ring ring = base;
       ring.add(set, a.stages);
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) fetch(u);
-      for (int b0 = set; b0 < blocks && ok; b0 += SETS * AHEAD) {
+      for (int b0 = set; b0 < blocks; b0 += SETS * AHEAD) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
           if (b0 + u * SETS >= blocks) break;
-          unsigned v[KB][2][2][4];                          // [chunk][row g, g + 8][piece][..]
+          const uint4 x = qv[u];
+          const unsigned sa = have ? sv[u][0] : 0u, sb = have ? sv[u][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
+          const unsigned w[4] = {flip ? x.z : x.x, flip ? x.w : x.y, flip ? x.x : x.z, flip ? x.y : x.w};
+          unsigned v[2][2][4];                              // [row g, g + 8][piece][..]
 #pragma unroll
-          for (int i = 0; i < KB; ++i) {
-            const bool in = have && (KB == 1 || i == 0 || c_lo + (b0 + u * SETS) * KB + i < a.w.chunks);
-            const uint4 x = qv[u][i];
-            const unsigned sa = in ? sv[u][i][0] : 0u, sb = in ? sv[u][i][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
-            const unsigned w[4] = {flip ? x.z : x.x, flip ? x.w : x.y, flip ? x.x : x.z, flip ? x.y : x.w};
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
-                v[i][r][h][0] = w4_value(w[2 * h], r, s2, off); v[i][r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
-                v[i][r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[i][r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
-              }
-          }
+            for (int h = 0; h < 2; ++h) {
+              const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
+              v[r][h][0] = w4_value(w[2 * h], r, s2, off); v[r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
+              v[r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
+            }
           fetch(u);
-          ok = mbar_wait(empty0 + 8 * ring.stage, ring.parity ^ 1u, a.status, 143) && ok;
+          W4U_WAIT(empty0 + 8 * ring.stage, ring.parity ^ 1u, 143);
           const unsigned at = ring.stage * stage_bytes;
 #pragma unroll
-          for (int i = 0; i < KB; ++i)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {                   // (row g + 8: eight rows of 128 bytes further on)
-              st_shared_v4(at + p0 + i * W4U_A_BYTES + r * 1024u, v[i][r][0][0], v[i][r][0][1], v[i][r][0][2], v[i][r][0][3]);
-              st_shared_v4(at + p1 + i * W4U_A_BYTES + r * 1024u, v[i][r][1][0], v[i][r][1][1], v[i][r][1][2], v[i][r][1][3]);
-            }
+          for (int r = 0; r < 2; ++r) {                     // (row g + 8: eight rows of 128 bytes further on)
+            st_shared_v4(at + p0 + r * 1024u, v[r][0][0], v[r][0][1], v[r][0][2], v[r][0][3]);
+            st_shared_v4(at + p1 + r * 1024u, v[r][1][0], v[r][1][1], v[r][1][2], v[r][1][3]);
+          }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
           __syncwarp();
           if (lane == 0) mbar_arrive(full0 + 8 * ring.stage);
@@ -365,7 +338,7 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
       const unsigned acc = use & 1;
       const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + quarter * 32 + lane;
       const float bias = a.bias && n < a.w.N ? a.bias[n] : 0.f;
-      if (!epilogue_wait(accfull0 + 8 * acc, (use >> 1) & 1, a.status, &gave_up, quarter == 2)) break;
+      W4U_WAIT_EPILOGUE(accfull0 + 8 * acc, (use >> 1) & 1);
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       for (int c0 = 0; c0 < a.bn && m0 + c0 < a.M; c0 += 16) {
         float v[16];
@@ -384,16 +357,15 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
     const int share = ((a.bn / 16 + a.splits - 1) / a.splits) * 16;               // columns a rank finishes, a multiple of 16
     const unsigned recv = tiles;                                                  // (over the stages: they have been read when it is written)
     const bool epi_warp = warp >= 2 + 8 * SETS;
-    bool ok = true;
     if (epi_warp) {
       pdl_wait();
-      ok = epilogue_wait(accfull0, 0, a.status, &gave_up, quarter == 2);
+      W4U_WAIT_EPILOGUE(accfull0, 0);
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     }
     __syncwarp();
     cluster_sync();                                                               // every rank's MMAs have read their stages
     if (epi_warp) {
-      for (int c0 = 0; ok && c0 < a.bn && m0 + c0 < a.M; c0 += 16) {
+      for (int c0 = 0; c0 < a.bn && m0 + c0 < a.M; c0 += 16) {
         const int owner = c0 / share;
         if (owner == rank) continue;
         float v[16];
@@ -405,7 +377,7 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
     }
     __syncwarp();
     cluster_sync();
-    if (epi_warp && ok) {
+    if (epi_warp) {
       const float bias = a.bias && n < a.w.N ? a.bias[n] : 0.f;
       const float* mine = reinterpret_cast<const float*>(smem_raw + (recv - smem_u32(smem_raw))) + quarter * 32 + lane;
       for (int c0 = rank * share; c0 < a.bn && c0 < (rank + 1) * share && m0 + c0 < a.M; c0 += 16) {
@@ -423,6 +395,7 @@ __global__ void __launch_bounds__(w4u_threads(SETS), SETS == 1 ? 2 : 1) gemm_w4_
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
+  if (dead) for (int i = 0; i < 64; ++i) __nanosleep(100000);        // (some milliseconds: what is on its way into this memory has come)
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(a.tmem_cols) : "memory");
@@ -482,15 +455,22 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   }
   W4uArgs a = {*w, bias, out, status, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0};
   const int n_sm = fellm_sm_count(), n_tiles = ceil_div(N, 128);
-  // columns of a tile: all rows in one where they fit, else as few tiles as 256 allow, equally wide
-  const int wide = n_tiles * ceil_div(M, 256) >= n_sm ? 256 : 128;
-  a.bn = ceil_div(ceil_div(M, ceil_div(M, wide)), 16) * 16;
-  const int total = n_tiles * ceil_div(M, a.bn), sets = a.bn <= 128 ? 1 : 2;
-  a.splits = 1;
-  while (sets == 1 && a.splits < 8 && total * a.splits * 2 <= 2 * n_sm && chunks >= a.splits * 2 * 4) a.splits *= 2;
-  const int kb = parts == 1 && a.bn <= 64 ? 2 : 1, stage = kb * (W4U_A_BYTES + a.bn * 128);
+  // Columns of a tile and CTAs that share its K, by the time of the busiest SM: a stage (64 k) took 0.25 us up to some 112 columns, where
+  // making weights bounds it, 0.28 at 128, 0.45 at 256, where the MMAs do; a cluster's exchange some 2 us.
+  double least = 1e30;
+  int total = 1;
+  a.bn = 16; a.splits = 1;
+  for (int m_tiles = ceil_div(M, 256), i = 0; i < 8 && m_tiles <= ceil_div(M, 16); ++m_tiles, ++i) {
+    const int bn = ceil_div(ceil_div(M, m_tiles), 16) * 16, tiles = n_tiles * ceil_div(M, bn);
+    const double stage_us = bn <= 112 ? 0.25 : 0.1 + 0.00137 * bn;
+    for (int s = 1; s <= 8 && (s == 1 || (tiles * s <= n_sm && chunks >= 4 * s)); s *= 2) {
+      const double t = ceil_div(tiles * s, n_sm) * (double)ceil_div(chunks, s) * parts * stage_us + (s > 1 ? 2.0 : 0.0);
+      if (t < least) { least = t; a.bn = bn; a.splits = s; total = tiles; }
+    }
+  }
+  const int stage = W4U_A_BYTES + a.bn * 128;
   const int share = ceil_div(a.bn / 16, a.splits) * 16, recv = a.splits > 1 ? a.splits * share * 512 : 0;
-  a.stages = (sets == 1 ? 112 : 220) * 1024 / stage;
+  a.stages = 220 * 1024 / stage;
   if (a.stages > 8) a.stages = 8;
   a.tmem_cols = 32;
   while (a.tmem_cols < (a.splits > 1 ? 1 : 2) * a.bn) a.tmem_cols *= 2;
@@ -505,17 +485,12 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return 1000 + (int)r;
   const size_t smem = (size_t)a.stages * stage + 1024;
-  const int grid = a.splits > 1 ? total * a.splits : (total < (3 - sets) * n_sm ? total : (3 - sets) * n_sm);
+  const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
   auto go = [&](auto kern) -> int {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(w4u_threads(sets), 1, 1), smem, stream, a.splits, map, a);
+    return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
   };
-  if (parts == 1) {
-    if (sets == 2) return go(gemm_w4_umma_kernel<false, 1, 2, 1>);
-    if (kb == 2) return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 1, 1, 2>) : go(gemm_w4_umma_kernel<false, 1, 1, 2>);
-    return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 1, 1, 1>) : go(gemm_w4_umma_kernel<false, 1, 1, 1>);
-  }
-  if (sets == 2) return go(gemm_w4_umma_kernel<false, 3, 2, 1>);
-  return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 3, 1, 1>) : go(gemm_w4_umma_kernel<false, 3, 1, 1>);
+  if (parts == 1) return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 1>) : go(gemm_w4_umma_kernel<false, 1>);
+  return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 3>) : go(gemm_w4_umma_kernel<false, 3>);
 }
