@@ -28,7 +28,7 @@ LOG_LEVELS = {"error": logging.ERROR, "warn": logging.WARNING, "warning": loggin
 RUN_DEFAULTS = dict(  # fellm.toml [run]
     max_tokens=128, temperature=0.2, top_k=80, top_p=1.0, min_p=0.0, seed=0, repetition_penalty=1.05,
     frequency_penalty=0.0, presence_penalty=0.0, ctx_size=8192, batch_size=2048, ubatch_size=512,
-    kv_device_budget=0, kv_memory_fraction=0.25, dtype="bfloat16", page_tokens=64, max_requests=64)
+    kv_device_budget=0, kv_memory_fraction=0.25, dtype="bfloat16", weights="kept", weight_group=64, page_tokens=64, max_requests=64)
 
 
 def _parser():
@@ -58,6 +58,8 @@ def _parser():
                      help="bytes of cache pages (0 = from free memory)")
     run.add_argument("--kv-memory-fraction", type=float)
     run.add_argument("--dtype", choices=["bfloat16", "float32"])
+    run.add_argument("--weights", choices=["kept", "int4"], help="int4: matrices in four bits")
+    run.add_argument("--weight-group", type=int, choices=[32, 64, 128], help="elements of a row that share a scale (int4)")
     run.add_argument("--page-tokens", type=int)
     run.add_argument("--echo-prompt", action="store_true")
     bench = sub.add_parser("bench", help="run N random prompts together and print prompt-eval / eval tokens a second")
@@ -70,7 +72,8 @@ def _parser():
     bench.add_argument("--seed", type=int)
     for flag, kw in (("--ctx-size", dict(type=int)), ("--batch-size", dict(type=int)), ("--ubatch-size", dict(type=int)),
                      ("--kv-device-budget", dict(type=int)), ("--kv-memory-fraction", dict(type=float)),
-                     ("--dtype", dict(choices=["bfloat16", "float32"])), ("--page-tokens", dict(type=int))):
+                     ("--dtype", dict(choices=["bfloat16", "float32"])), ("--page-tokens", dict(type=int)),
+                     ("--weights", dict(choices=["kept", "int4"])), ("--weight-group", dict(type=int, choices=[32, 64, 128]))):
         bench.add_argument(flag, **kw)
     ins = sub.add_parser("inspect", help="print a model folder's configuration and tensors")
     ins.add_argument("--model", required=True)
@@ -135,7 +138,8 @@ def _open_engine(args, r):
     from .config.errors import ConfigError
     from .config.options import EngineOptions
     from .engine import Engine
-    opts = EngineOptions(dtype=r["dtype"], n_ctx=r["ctx_size"], n_batch=r["batch_size"], n_ubatch=r["ubatch_size"],
+    opts = EngineOptions(dtype=r["dtype"], weights=r["weights"], weight_group=r["weight_group"],
+                         n_ctx=r["ctx_size"], n_batch=r["batch_size"], n_ubatch=r["ubatch_size"],
                          page_tokens=r["page_tokens"], max_requests=r["max_requests"],
                          kv_memory_fraction=r["kv_memory_fraction"], kv_device_budget=r["kv_device_budget"])
     t0 = time.perf_counter()

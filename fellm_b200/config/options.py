@@ -8,6 +8,8 @@ from typing import Optional
 from .errors import ConfigError
 
 DTYPES = ("bfloat16", "float32")
+WEIGHTS = ("kept", "int4")
+WEIGHT_GROUPS = (32, 64, 128)
 
 
 @dataclass
@@ -16,6 +18,8 @@ class EngineOptions:
     n_ctx 8192 clamped to the model's maximum (0 = the model's maximum), n_batch = tokens a
     scheduler iteration may run, n_ubatch = the longest portion of one prompt in a step."""
     dtype: str = "bfloat16"
+    weights: str = "kept"           # "kept": matrices as the loader keeps them; "int4": the large ones in four bits (Model.quantize)
+    weight_group: int = 64          # elements of a row that share a scale ("int4")
     n_ctx: int = 8192
     n_batch: int = 2048
     n_ubatch: int = 512
@@ -31,6 +35,10 @@ class EngineOptions:
     def validate(self):
         if self.dtype not in DTYPES:
             raise ConfigError(f"dtype must be one of {DTYPES}, got {self.dtype!r}")
+        if self.weights not in WEIGHTS:
+            raise ConfigError(f"weights must be one of {WEIGHTS}, got {self.weights!r}")
+        if self.weight_group not in WEIGHT_GROUPS:
+            raise ConfigError(f"weight_group must be one of {WEIGHT_GROUPS}, got {self.weight_group}")
         if self.page_tokens < 1 or (self.page_tokens & (self.page_tokens - 1)):
             raise ConfigError(f"page_tokens must be a power of two, got {self.page_tokens}")
         if self.page_tokens > 256:

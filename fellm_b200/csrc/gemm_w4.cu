@@ -120,7 +120,7 @@ __host__ __device__ constexpr int rows_buffers(int nt) { return nt < 4 ? 2 : 1; 
 // XT: what x is.  NT: tiles of eight rows of x.  GS: log2 of the group.  R: neighbouring slabs a warp takes together (a "slab" below is
 // R of them, a unit 4 / R chunks of each): the same columns' operands for both.
 template <int XT, int NT, int GS, int R>
-__global__ void __maxnreg__(128) gemm_w4_rows_kernel(GwArgs a) {
+__maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
   constexpr int UNIT = 4 / R, ROWS = R * W4_SLAB, P = XParts<XT>::N, COLS = 8 * NT, XB = XT == X_F32 ? 4 : 2;      // XB: bytes of an element of x
   extern __shared__ __align__(16) unsigned char smem[];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;

@@ -535,11 +535,9 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   if (r != CUDA_SUCCESS) return 1000 + (int)r;
   const size_t smem = (size_t)a.stages * stage + 1024;
   const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
-  auto go = [&](auto kern) -> int {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-    return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
-  };
-  if (parts == 1) return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 1>) : go(gemm_w4_umma_kernel<false, 1>);
-  return a.splits > 1 ? go(gemm_w4_umma_kernel<true, 3>) : go(gemm_w4_umma_kernel<false, 3>);
+  auto kern = parts == 1 ? (a.splits > 1 ? gemm_w4_umma_kernel<true, 1> : gemm_w4_umma_kernel<false, 1>)
+                         : (a.splits > 1 ? gemm_w4_umma_kernel<true, 3> : gemm_w4_umma_kernel<false, 3>);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
 }

@@ -14,6 +14,7 @@ from typing import Iterable, List, Optional
 
 import torch
 
+from .. import ops
 from ..cache.manager import CacheManager
 from ..config.errors import ConfigError, KernelError
 from ..config.options import EngineOptions
@@ -46,11 +47,13 @@ class Engine:
         spec = arch.build_spec(config)
         self.spec = spec
         self.model = build_model(spec, options.dtype)
-        jit.compile_many(self.model.kernel_modules())
+        jit.compile_many(self.model.kernel_modules() + (ops.w4_modules() if options.weights == "int4" else []))
         if folder is not None:
             load_into(self.model, folder, self.device)
         else:
             bind_tensors(self.model, tensors, self.device)
+        if options.weights == "int4":
+            self.model.quantize(options.weight_group)
         # context: FeLLM clamps n_ctx to the model's maximum, 0 = the maximum (engine.rs:190-197)
         n_ctx = spec.max_position if options.n_ctx == 0 else min(options.n_ctx, spec.max_position)
         if options.ctx_past_model and options.n_ctx > 0:
@@ -69,7 +72,6 @@ class Engine:
         max_rows = max(options.n_batch, options.n_ubatch) + max_items
         for part in self.model.all_parts():
             part.reserve(self.device, max_items, n_ctx)
-        from .. import ops
         ops.register_weight_chain(self.model.weight_chain())
         self.stepper = Stepper(self.model, self.cache, max_rows=max_rows, max_items=max_items,
                                device=self.device, cuda_graphs=options.cuda_graphs)

@@ -220,6 +220,16 @@ class Block:
             at += n
         self.joint = (joint, bias, cols)
 
+    def quantize(self, group: int):
+        """The matrix that join_inputs() made, in four bits; the parts keep no views of what it was."""
+        if self.joint is None:
+            return
+        w, bias, cols = self.joint
+        self.joint = (ops.quantize_w4(w, group), bias, cols)
+        for key, p in (("mixer", self.mixer), ("gate", self.gate), ("ffn", self.ffn)):
+            if key in cols:
+                p.w.pop(p.input_rows)
+
     def parts(self):
         return [q for p in (self.norm1, self.mixer, self.norm1b, self.norm2, self.ffn, self.norm2b, self.gate, self.side) if p is not None
                 for q in _with_children(p)]
@@ -296,6 +306,18 @@ class Model:
                 part.attach(by_name[want])
         for block in self.blocks:
             block.join_inputs()
+
+    def quantize(self, group: int):
+        """After bind(): every matrix that is only multiplied with rows of activations (parts say which: Part.four_bit), the
+        embedding and the head, in four bits.  Experts, convolutions, norms, routers and what a kernel of a mixer reads stay."""
+        for block in self.blocks:
+            block.quantize(group)
+        tied = getattr(self.head, "tied", False)
+        for part in self.all_parts():
+            if not (part is self.head and tied):
+                part.quantize(group)
+        if tied:
+            self.head.w["weight"] = self.embedding.w["weight"]
 
     def kernel_modules(self):
         mods = []

@@ -1982,6 +1982,10 @@ W4_READ_AHEAD = 32                       # chunks behind the end of a matrix tha
 W4_FEW_ROWS = 16                         # up to so many rows: mma.sync, a warp a slab of 16 weight rows; more: tcgen05
 
 
+def w4_modules():
+    return [("w4", None), ("gemm_w4", None), ("gemm_w4_umma", None)]
+
+
 class _W4Ref(ctypes.Structure):
     """csrc/w4.h W4Ref: what a launcher is told of a matrix, in one pointer."""
     _fields_ = [("q", _c_p), ("s", _c_p), ("N", _c_int), ("K", _c_int), ("chunks", _c_int), ("groups", _c_int), ("gshift", _c_int)]
@@ -2145,7 +2149,7 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
         odt, ldo = out_dtype or dt, cols
         if odt is not dt and (odt is not torch.float32):
             raise KernelError(f"gemm_w4: rows of {dt} do not make a result of {odt}")
-        out = torch.empty((M, cols), dtype=odt, device=x.device)
+        out = x.new_empty((M, cols)) if odt is dt else torch.empty((M, cols), dtype=odt, device=x.device)
     else:
         if out.dim() != 2 or out.shape[0] != M or out.shape[1] != cols or (cols > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < cols):
             raise KernelError(f"gemm_w4: the result is {[M, cols]} with contiguous rows, not {list(out.shape)} with strides {list(out.stride())}")

@@ -201,12 +201,15 @@ class Attention(Mixer):
         self.position.to(q.device)
         if self.sink_score is not None:
             self.w["sink"] = torch.full((self.H,), self.sink_score, dtype=torch.float32, device=q.device)
+        self.kept_bf16 = self.w["qkv.weight"].dtype == torch.bfloat16
+
+    four_bit = ("qkv.weight", "out_proj.weight")
 
     def reserve(self, device, max_rows, n_ctx):
-        if self.w["qkv.weight"].dtype == torch.bfloat16 and not self.general:
+        if self.kept_bf16 and not self.general:
             floats, counters = ops.decode_scratch_need(max_rows, self.H, self.G, self.hd, n_ctx)
             ops.reserve_decode_scratch(device, 1, self.H, self.G, self.hd, 1, floats=floats, counters=counters)
-        elif self.w["qkv.weight"].dtype == torch.bfloat16 and self.written:
+        elif self.kept_bf16 and self.written:
             floats, counters = ops.decode_scratch_need(max_rows, self.H, self.G, self.vd, n_ctx)
             floats = max(floats, ops.decode_wide_scratch_need(max_rows, self.H, self.G, self.hd, self.vd, n_ctx, self.window)[0])
             ops.reserve_decode_scratch(device, 1, self.H, self.G, self.vd, 1, floats=floats, counters=counters)

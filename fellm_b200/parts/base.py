@@ -105,6 +105,16 @@ class Part:
     def prepare(self):
         """Called once after bind(): repack or fuse weights for the kernels."""
 
+    four_bit = ()          # names in self.w, after prepare(), of the matrices that forward() hands to linear() and nothing else
+
+    def quantize(self, group: int):
+        """The matrices named `four_bit` in four bits (ops.quantize_w4), groups of `group` elements of a row.  Called once, after
+        bind() and whatever puts parts' matrices together."""
+        from .. import ops
+        for name in self.four_bit:
+            if isinstance(self.w.get(name), torch.Tensor):
+                self.w[name] = ops.quantize_w4(self.w[name], group)
+
     def weight_order(self):
         """The part's matrices in the order its forward() reads them (for the engine's chain of weights:
         each product asks the L2 for the matrix of the product after it)."""

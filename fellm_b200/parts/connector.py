@@ -25,6 +25,8 @@ class ConcatProjection(Connector):
         self.decls = {"in.weight": ParamDecl((self.size, 2 * self.size)),
                       "step": ParamDecl((self.steps, self.size), role="vector", init=("normal", 0.05))}
 
+    four_bit = ("in.weight",)
+
     def forward(self, x, x0, step, act_dtype):
         xc = ops.concat_cast(x, x0, act_dtype)
         ops.residual_written(x)

@@ -18,9 +18,14 @@ class TableEmbedding(Embedding):
         self.vocab, self.size, self.scale = int(vocab), int(size), float(scale)
         self.decls = {"weight": ParamDecl((self.vocab, self.size))}
 
+    four_bit = ("weight",)
+
     def forward(self, tokens, status=None):
         out = torch.empty((tokens.numel(), self.size), dtype=torch.float32, device=tokens.device)
-        return ops.embed_rows(tokens, self.w["weight"], out, status, self.scale)
+        table = self.w["weight"]
+        if isinstance(table, ops.W4):
+            return ops.embed_rows_w4(tokens, table, out, status, self.scale)
+        return ops.embed_rows(tokens, table, out, status, self.scale)
 
     def kernel_modules(self, dtype):
         return [("elementwise", None)]
@@ -37,6 +42,7 @@ class LinearHead(Head):
         self.decls = {} if self.tied else {"weight": ParamDecl((self.vocab, self.size))}
 
     takes_lazy_norm = True
+    four_bit = ("weight",)
 
     def forward(self, xf):
         z = linear(xf, self.w["weight"], out_dtype=torch.float32)

@@ -119,6 +119,8 @@ class GatedDelta(Mixer):
         self.rows = {n: m.shape[0] for n, m in zip(names, mats)}
         w["taps"] = torch.cat([w.pop("q.conv"), w.pop("k.conv"), w.pop("v.conv")], 0).contiguous()
 
+    four_bit = ("in.weight", "o.weight")
+
     def cache_need(self):
         return [FixedState((self.taps - 1, 2 * self.G * self.dk + self.H * self.dv)),
                 FixedState((self.H, self.dk, self.dv))]

@@ -47,6 +47,8 @@ class Hgrn2(Mixer):
         w["qfv.weight"] = _pad_rows(torch.cat(mats, 0))          # q | f | v rows, one product
         w["f.bias"], w["lower"] = w["f.bias"].contiguous(), w["lower"].contiguous()
 
+    four_bit = ("qfv.weight", "o.weight")
+
     def cache_need(self):
         return FixedState((self.H, self.dk, self.dv))
 

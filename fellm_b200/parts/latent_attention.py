@@ -110,6 +110,7 @@ class LatentAttention(Mixer):
         return dtype == torch.bfloat16 and bool(ops.latent_expand_key_rows(self.H, self.dn, self.dr, self.dv, self.rk, self.window, 64, 1 << 20, 1, 1))
 
     can_store = True       # forward(store=True) writes the float32 rows `out` instead of adding into them
+    four_bit = ("down.weight", "uq.weight", "o.weight")       # (what a head's keys and values are made with stays: head_gemm reads it)
     input_rows = "down.weight"      # forward(pre=z): the float32 product of the layer's input with these rows, made elsewhere
 
     def forward(self, xn, ctx, cache, out, reads_only=False, store=False, pre=None):
@@ -170,7 +171,7 @@ class LatentAttention(Mixer):
         return out
 
     def weight_order(self):
-        return [self.w["down.weight"], self.w["uq.weight"], self.w["o.weight"]]
+        return [self.w.get("down.weight"), self.w["uq.weight"], self.w["o.weight"]]
 
     def kernel_modules(self, dtype):
         mods = linear_modules(dtype) + [("latent", None), ("attention_simt", None)]

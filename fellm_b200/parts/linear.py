@@ -1,5 +1,6 @@
 """y = x W^T (+ b): the one place that picks the matrix-product kernel.
 
+A matrix in four bits (ops.W4) goes to the kernels that read one, whatever the activations; else
 bfloat16 x bfloat16 goes to the tensor-core kernels; everything else (the 32-bit engine, and a
 matrix a file stores in 32-bit under a bfloat16 engine) to the float32-FMA kernel.  FeLLM's CUDA
 plugin has one dense product, bf16_matmul_rows (plugins/cuda_kernels/src/oxide_kernels.rs:3165),
@@ -49,6 +50,9 @@ def linear(x, w, bias=None, *, out=None, out_dtype=None, accumulate=False, swigl
     """x [T, K] (a tensor or a LazyNorm), w [N, K] -> [T, N].  accumulate=True adds into the
     float32 `out` (the residual stream) instead of storing; swiglu=True: w is the interleaved
     gate/up matrix and the result is SiLU(gate)*up; act="relu2": the result is max(., 0)^2 in x's dtype."""
+    if isinstance(w, ops.W4):
+        x = x.tensor() if isinstance(x, LazyNorm) else x
+        return ops.gemm_w4(x, w, bias, out=out, out_dtype=out_dtype, accumulate=accumulate, swiglu=swiglu, act=act)
     if isinstance(x, LazyNorm):
         h = x.handed_on()
         if (h is not None and ops.fast_gemm_takes(h.xg, w) and w.data_ptr() % 16 == 0

@@ -26,6 +26,7 @@ class PlainFeedForward(FeedForward):
             self.decls["down.bias"] = ParamDecl((self.size,), role="vector", init=("normal", 0.1))
 
     takes_lazy_norm = True
+    four_bit = ("up.weight", "down.weight")
     can_store = True          # forward(store=True) writes the float32 rows `out` instead of adding into them
 
     def forward(self, hn, ctx, out, store=False):

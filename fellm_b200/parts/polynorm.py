@@ -28,6 +28,7 @@ class PolyNormFeedForward(FeedForward):
 
     can_store = True       # forward(store=True) writes the float32 rows `out` instead of adding into them
 
+    four_bit = ("up.weight", "down.weight")
     input_rows = "up.weight"        # forward(pre=z): the float32 product of the layer's input with these rows, made elsewhere
 
     def forward(self, hn, ctx, out, store=False, pre=None):
@@ -40,7 +41,7 @@ class PolyNormFeedForward(FeedForward):
         return out
 
     def weight_order(self):
-        return [self.w["up.weight"], self.w["down.weight"]]
+        return [self.w.get("up.weight"), self.w["down.weight"]]
 
     def kernel_modules(self, dtype):
         return linear_modules(dtype) + [("elementwise", None)]

@@ -31,6 +31,7 @@ class SigmoidGates(ResidualGate):
         self.w["weight"] = torch.cat([m.to(dt) for m in mats], 0).contiguous()           # [n size, size]
         self.w["bias"] = torch.cat([self.w.pop(f"{s}.bias") for s in range(self.n)]).contiguous()
 
+    four_bit = ("weight",)
     input_rows, input_bias = "weight", "bias"       # the block may make the logits in a product it shares with its sublayers
 
     def logits(self, h):
@@ -42,7 +43,7 @@ class SigmoidGates(ResidualGate):
         return ops.gated_add(x, results, zg)
 
     def weight_order(self):
-        return [self.w["weight"]]
+        return [self.w.get("weight")]
 
     def kernel_modules(self, dtype):
         return linear_modules(dtype) + [("elementwise", None)]

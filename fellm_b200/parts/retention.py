@@ -59,6 +59,8 @@ class Retention(Mixer):
         w["decay"] = torch.tensor(self.decay, dtype=torch.float64).to(torch.float32).to(dev)
         self.position.to(dev)
 
+    four_bit = ("in.weight", "o.weight")
+
     def cache_need(self):
         return FixedState((self.H, self.dk, self.dv))
 

@@ -36,6 +36,7 @@ class ShortConv(Mixer):
                                "out_proj.bias": ParamDecl((d,), role="vector", init=("normal", 0.01))})
 
     takes_lazy_norm = True
+    four_bit = ("in_proj.weight", "out_proj.weight")
     blocked = False
 
     def prepare(self):
@@ -57,7 +58,8 @@ class ShortConv(Mixer):
         if reads_only:
             raise ConfigError("a shortconv layer cannot run on another layer's state")
         w_in, b_in = self.w["in_proj.weight"], self.w.get("in_proj.bias")
-        if self.blocked and FUSE_DECODE_CONV and ctx.all_single and ops.conv_product_takes(ctx.n_rows, 3 * self.size, self.size, self.taps):
+        if (self.blocked and FUSE_DECODE_CONV and isinstance(w_in, torch.Tensor) and ctx.all_single
+                and ops.conv_product_takes(ctx.n_rows, 3 * self.size, self.size, self.taps)):
             # a decode step: product and convolution in one launch
             h = xn.handed_on() if isinstance(xn, LazyNorm) else None
             scale = None

@@ -39,6 +39,7 @@ class SwiGLU(FeedForward):
             self.w["gate_up.weight"] = torch.cat([g, u], dim=0).contiguous()
 
     takes_lazy_norm = True
+    four_bit = ("gate_up.weight", "down.weight")
 
     can_store = True          # forward(store=True) writes its rows instead of adding them
 

@@ -52,6 +52,8 @@ class TimeMix(Mixer):
         for name in ("r.weight", "k.weight", "v.weight", "g.weight", "w1.weight"):
             w[name] = _pad_rows(w[name])        # whole groups of output columns for the products' vector stores
 
+    four_bit = ("r.weight", "k.weight", "v.weight", "g.weight", "o.weight")
+
     def cache_need(self):
         return [FixedState((self.size,)), FixedState((self.H, self.dk, self.dk))]
 
