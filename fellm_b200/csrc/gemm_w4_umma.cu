@@ -22,7 +22,6 @@
 
 #define SETS 2                         // sets of eight warps that make weights, each every other stage (three took registers from one another)
 #define W4U_THREADS (32 * (2 + 8 * SETS + 4))
-#define AHEAD 4                        // stages whose chunks a warp holds in registers ahead of the one it unpacks
 #define W4U_SPIN_LIMIT (1u << 26)
 #define W4U_A_BYTES (128 * 128)        // 128 weight rows x 64 k
 
@@ -100,7 +99,9 @@ __device__ __forceinline__ unsigned mapa(unsigned addr, unsigned rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void st_cluster(unsigned addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void st_cluster_v4(unsigned addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
@@ -113,6 +114,7 @@ struct W4uArgs {
   int M, epi, out_bf16;
   int bn;                    // rows of x a tile, a multiple of 16, <= 256
   int stages, splits, tmem_cols;
+  int recv_apart;            // what other ranks send lies behind the stages, not over them
 };
 
 // The four words of a lane (rows g and g + 8, 16 elements each) -> its pieces of the tile.  Neighbouring even and odd rows
@@ -251,22 +253,27 @@ struct Ring {
   __device__ __forceinline__ void add_many(unsigned n, unsigned stages) { stage += n; parity ^= (stage / stages) & 1u; stage %= stages; }
 };
 
-template <bool SPLIT, int PARTS>
+// KB: chunks of K a stage.  Two where a tile is narrow: one handshake and one commit cost the issuing warp as much as three MMAs of 64
+// columns (377 cycles a stage of one chunk, 40 an MMA).
+template <bool SPLIT, int PARTS, int KB>
 __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
+  constexpr int AHEAD = 4 / KB;          // stages whose chunks a warp holds in registers ahead of the one it unpacks
+  constexpr unsigned A_BYTES = KB * W4U_A_BYTES;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];           // full[8], empty[8], acc_full[2], acc_empty[2]
   __shared__ unsigned tmem_base_s;
   __shared__ int dead;                   // a wait gave up
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const unsigned x_bytes = (unsigned)a.bn * 128u, stage_bytes = W4U_A_BYTES + x_bytes;
+  const unsigned x_bytes = (unsigned)a.bn * 128u, stage_bytes = A_BYTES + KB * x_bytes;
   const unsigned full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[8]), accfull0 = smem_u32(&bars[16]), accempty0 = smem_u32(&bars[18]);
   const int m_tiles = (a.M + a.bn - 1) / a.bn, n_tiles = (a.w.N + 127) / 128, total = m_tiles * n_tiles;
   const int rank = SPLIT ? (int)cluster_rank() : 0;
   const int first = SPLIT ? (int)blockIdx.x / a.splits : (int)blockIdx.x, step = SPLIT ? total : (int)gridDim.x;
   // this CTA's chunks of K
-  const int c_lo = SPLIT ? (int)((long long)a.w.chunks * rank / a.splits) : 0, c_hi = SPLIT ? (int)((long long)a.w.chunks * (rank + 1) / a.splits) : a.w.chunks;
-  const int blocks = (c_hi - c_lo) * PARTS;
+  const int k_stages = (a.w.chunks + KB - 1) / KB;
+  const int c_lo = SPLIT ? (int)((long long)k_stages * rank / a.splits) * KB : 0, c_hi = SPLIT ? (int)((long long)k_stages * (rank + 1) / a.splits) * KB : k_stages * KB;
+  const int blocks = (c_hi - c_lo) / KB * PARTS;
 
   if (threadIdx.x == 0) {
     dead = 0;
@@ -283,6 +290,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const unsigned tmem_base = tmem_base_s, acc_cols = SPLIT ? 0u : (unsigned)a.tmem_cols / 2;
   pdl_launch_dependents();
+  if (SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");        // (waited for where another rank's memory is written)
 
   if (warp == 0) {
     pdl_wait();                                              // x is the output of the kernel before this one
@@ -294,8 +302,10 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         W4U_WAIT(empty0 + 8 * ring.stage, ring.parity ^ 1u, 141);
         __syncwarp();
         if (elect_one()) {
-          mbar_expect_tx(full, x_bytes);
-          tma_load_2d(tiles + ring.stage * stage_bytes + W4U_A_BYTES, &map_x, (c_lo * PARTS + b) * W4_CHUNK, m0, full);      // (behind the end of K: zeros)
+          mbar_expect_tx(full, KB * x_bytes);
+#pragma unroll
+          for (int i = 0; i < KB; ++i)                       // (behind the end of K: zeros)
+            tma_load_2d(tiles + ring.stage * stage_bytes + A_BYTES + i * x_bytes, &map_x, (c_lo * PARTS + b * KB + i) * W4_CHUNK, m0, full);
         }
         ring.add(1, a.stages);
       }
@@ -313,7 +323,9 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         if (elect_one()) {
-          umma_stage(d, lo, lo + (W4U_A_BYTES >> 4), idesc, b ? 1u : 0u);
+#pragma unroll
+          for (int i = 0; i < KB; ++i)
+            umma_stage(d, lo + i * (W4U_A_BYTES >> 4), lo + (A_BYTES >> 4) + i * (x_bytes >> 4), idesc, (b | i) ? 1u : 0u);
           umma_commit(empty);
           if (b == blocks - 1) umma_commit(accfull0 + 8 * acc);
         }
@@ -334,46 +346,52 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       const bool have = slab < slabs;
       const uint4* q = a.w.q + ((size_t)(have ? slab : 0) * a.w.chunks + c_lo) * 32 + lane;
       const unsigned* sc = a.w.s + (size_t)(have ? slab : 0) * a.w.groups * 8 + g;
-      uint4 qv[AHEAD];
-      unsigned sv[AHEAD][2];
+      uint4 qv[AHEAD][KB];
+      unsigned sv[AHEAD][KB][2];
       // This set's blocks of the tile: set, set + SETS, ...; `ahead`: the next one to be fetched.  Behind the last one loads go on
       // (into the next slab or the room behind the matrix): a load that may not happen would have to be waited for at once.
       unsigned ahead = set;
-      auto fetch = [&](int u) {
-        const unsigned ch = PARTS == 1 ? ahead : ahead / 3;
-        qv[u] = __ldg(q + ch * 32u);
+      auto fetch = [&](int u, int i) {
+        const unsigned ch = PARTS == 1 ? ahead * KB + i : ahead / 3;
+        qv[u][i] = __ldg(q + ch * 32u);
         const unsigned* at = sc + ((((unsigned)c_lo + ch) * W4_CHUNK) >> a.w.gshift) * 8u;
-        sv[u][0] = __ldg(at);
-        sv[u][1] = __ldg(at + (two_scales ? 8 : 0));
-        ahead += SETS;
+        sv[u][i][0] = __ldg(at);
+        sv[u][i][1] = __ldg(at + (two_scales ? 8 : 0));
+        if (i == KB - 1) ahead += SETS;
       };
       Ring ring = base;
       ring.add(set, a.stages);
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) fetch(u);
+      for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int i = 0; i < KB; ++i) fetch(u, i);
       for (int b0 = set; b0 < blocks; b0 += SETS * AHEAD) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
           if (b0 + u * SETS >= blocks) break;
-          const uint4 x = qv[u];
-          const unsigned sa = have ? sv[u][0] : 0u, sb = have ? sv[u][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
-          const unsigned w[4] = {flip ? x.z : x.x, flip ? x.w : x.y, flip ? x.x : x.z, flip ? x.y : x.w};
-          unsigned v[2][2][4];                              // [row g, g + 8][piece][..]
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
-              v[r][h][0] = w4_value(w[2 * h], r, s2, off); v[r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
-              v[r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
-            }
-          fetch(u);
-          W4U_WAIT(empty0 + 8 * ring.stage, ring.parity ^ 1u, 143);
           const unsigned at = ring.stage * stage_bytes;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {                     // (row g + 8: eight rows of 128 bytes further on)
-            st_shared_v4(at + p0 + r * 1024u, v[r][0][0], v[r][0][1], v[r][0][2], v[r][0][3]);
-            st_shared_v4(at + p1 + r * 1024u, v[r][1][0], v[r][1][1], v[r][1][2], v[r][1][3]);
+          for (int i = 0; i < KB; ++i) {
+            const bool in = have && (i == 0 || c_lo + (b0 + u * SETS) * KB + i < a.w.chunks);
+            const uint4 x = qv[u][i];
+            const unsigned sa = in ? sv[u][i][0] : 0u, sb = in ? sv[u][i][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
+            const unsigned w[4] = {flip ? x.z : x.x, flip ? x.w : x.y, flip ? x.x : x.z, flip ? x.y : x.w};
+            unsigned v[2][2][4];                            // [row g, g + 8][piece][..]
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
+                v[r][h][0] = w4_value(w[2 * h], r, s2, off); v[r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
+                v[r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
+              }
+            fetch(u, i);
+            if (i == 0) W4U_WAIT(empty0 + 8 * ring.stage, ring.parity ^ 1u, 143);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {                   // (row g + 8: eight rows of 128 bytes further on)
+              st_shared_v4(at + p0 + i * W4U_A_BYTES + r * 1024u, v[r][0][0], v[r][0][1], v[r][0][2], v[r][0][3]);
+              st_shared_v4(at + p1 + i * W4U_A_BYTES + r * 1024u, v[r][1][0], v[r][1][1], v[r][1][2], v[r][1][3]);
+            }
           }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
           __syncwarp();
@@ -402,42 +420,54 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     }
   }
   if (SPLIT) {
-    // every rank sends the other ranks' columns of its sums to them: [sending rank][column][128 rows]
-    const int quarter = warp & 3, t = first;
-    const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + quarter * 32 + lane;
+    // Every rank sends the other ranks' columns of its sums to them: [sending rank, without the owner][four columns][128 rows][4], so that a
+    // warp's store is 512 bytes in a row (16 bytes here and there took ten times as long: they travel one by one).
+    const int quarter = warp & 3, t = first, row = quarter * 32 + lane;
+    const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
     const int share = ((a.bn / 16 + a.splits - 1) / a.splits) * 16;               // columns a rank finishes, a multiple of 16
-    const unsigned recv = tiles;                                                  // (over the stages: they have been read when it is written)
+    const unsigned recv = a.recv_apart ? tiles + (unsigned)a.stages * stage_bytes : tiles;
     const bool epi_warp = warp >= 2 + 8 * SETS;
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");         // every rank has started: its memory is there
     if (epi_warp) {
       pdl_wait();
       W4U_WAIT_EPILOGUE(accfull0, 0);
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     }
     __syncwarp();
-    cluster_sync();                                                               // every rank's MMAs have read their stages
+    if (!a.recv_apart) cluster_sync();                                            // every rank's MMAs have read their stages
     if (epi_warp) {
-      for (int c0 = 0; c0 < a.bn && m0 + c0 < a.M; c0 += 16) {
-        const int owner = c0 / share;
+      for (int c = 0; c < a.bn && m0 + c < a.M; c += 16) {
+        const int owner = c / share;
         if (owner == rank) continue;
         float v[16];
-        tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c0, v);
-        const unsigned dst = mapa(recv + (unsigned)(((rank * share + c0 - owner * share) * 128 + quarter * 32 + lane) * 4), (unsigned)owner);
+        tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, v);
+        const int from = rank < owner ? rank : rank - 1;
+        const unsigned dst = mapa(recv + (unsigned)((((from * share + c - owner * share) / 4) * 128 + row) * 16), (unsigned)owner);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) st_cluster(dst + j * 512, v[j]);
+        for (int j = 0; j < 4; ++j) st_cluster_v4(dst + j * 2048, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
       }
     }
     __syncwarp();
     cluster_sync();
     if (epi_warp) {
-      const float* mine = reinterpret_cast<const float*>(smem_raw + (recv - smem_u32(smem_raw))) + quarter * 32 + lane;
+      const float4* mine = reinterpret_cast<const float4*>(smem_raw + (recv - smem_u32(smem_raw))) + row;
       finish_tile(a, [&](int c, float* v) {
         float own[16];
         tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, own);
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = 0.f;
         for (int r = 0; r < a.splits; ++r) {
+          if (r == rank) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] += r == rank ? own[j] : mine[(size_t)(r * share + c - rank * share + j) * 128];
+            for (int j = 0; j < 16; ++j) v[j] += own[j];
+          } else {
+            const float4* part = mine + (((r < rank ? r : r - 1) * share + c - rank * share) / 4) * 128;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 x = part[j * 128];
+              v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+            }
+          }
         }
       }, rank * share, min(a.bn, (rank + 1) * share), m0, n);
     }
@@ -482,6 +512,30 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// Clusters of `splits` CTAs, each an SM's all, that the device holds at once: the CTAs of one sit in one GPC, so this is less than SMs /
+// splits (a product whose clusters of 8 do not fit takes twice as long).  Asked once a device and size.
+static int clusters_at_once(int splits) {
+  static int cache[64][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!cache[dev][splits]) {
+    const size_t smem = 221 * 1024;
+    auto kern = gemm_w4_umma_kernel<true, 1, 1>;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(splits * 64, 1, 1); cfg.blockDim = dim3(W4U_THREADS, 1, 1); cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr; cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) { n = 0; cudaGetLastError(); }
+    }
+    cache[dev][splits] = n > 0 ? n : 1;
+  }
+  return cache[dev][splits];
+}
+
 // x that TMA cannot read as it is (float32, or rows that are not on 16 bytes) is copied into `scratch` first: M x chunks x 64 numbers of
 // bfloat16, three times as many for float32; scratch null: x is read itself.
 FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, const float* bias, void* out, long long ldo, int flags, int M, void* scratch,
@@ -504,26 +558,28 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   }
   W4uArgs a = {*w, bias, out, status, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0};
   const int n_sm = fellm_sm_count(), n_tiles = ceil_div(N, 128);
-  // Columns of a tile and CTAs that share its K, by the time of the busiest SM: a stage (64 k) took 0.25 us up to some 112 columns, where
-  // making weights bounds it, 0.28 at 128, 0.45 at 256, where the MMAs do; a cluster's exchange some 2 us.
+  // Columns of a tile and CTAs that share its K, by the time of the busiest SM.  A chunk took 0.21 us up to 64 columns and 0.28 at 128,
+  // where the issuing warp bounds it, 0.45 at 256, where the MMAs do; a cluster's exchange 1.2 us and what its sums take at some 22 GB/s an SM.
   double least = 1e30;
   int total = 1;
   a.bn = 16; a.splits = 1;
   for (int m_tiles = ceil_div(M, 256), i = 0; i < 8 && m_tiles <= ceil_div(M, 16); ++m_tiles, ++i) {
     const int bn = ceil_div(ceil_div(M, m_tiles), 16) * 16, tiles = n_tiles * ceil_div(M, bn);
-    const double stage_us = bn <= 112 ? 0.25 : 0.1 + 0.00137 * bn;
-    for (int s = 1; s <= 8 && (s == 1 || (tiles * s <= n_sm && chunks >= 4 * s)); s *= 2) {
-      const double t = ceil_div(tiles * s, n_sm) * (double)ceil_div(chunks, s) * parts * stage_us + (s > 1 ? 2.0 : 0.0);
+    if (m_tiles > 1 && bn < 112) break;                       // (every tile makes its weights again)
+    const double chunk_us = bn <= 64 ? 0.21 : bn <= 128 ? 0.14 + 0.0011 * bn : 0.1 + 0.00137 * bn;
+    for (int s = 1; s <= 8 && (s == 1 || (chunks >= 4 * s && tiles <= clusters_at_once(s))); s *= 2) {
+      const double t = ceil_div(tiles * s, n_sm) * (double)ceil_div(chunks, s) * parts * chunk_us + (s > 1 ? 1.2 + bn * 0.0234 * (s - 1) / s : 0.0);
       if (t < least) { least = t; a.bn = bn; a.splits = s; total = tiles; }
     }
   }
-  const int stage = W4U_A_BYTES + a.bn * 128;
-  const int share = ceil_div(a.bn / 16, a.splits) * 16, recv = a.splits > 1 ? a.splits * share * 512 : 0;
-  a.stages = 220 * 1024 / stage;
-  if (a.stages > 8) a.stages = 8;
+  const int kb = parts == 1 && a.bn <= 128 ? 2 : 1, stage = kb * (W4U_A_BYTES + a.bn * 128), room = 220 * 1024;
+  const int share = ceil_div(a.bn / 16, a.splits) * 16, recv = (a.splits - 1) * share * 512;
+  a.stages = room / stage < 8 ? room / stage : 8;
+  a.recv_apart = (room - recv) / stage >= 3;
+  if (a.recv_apart && (room - recv) / stage < a.stages) a.stages = (room - recv) / stage;
   a.tmem_cols = 32;
   while (a.tmem_cols < (a.splits > 1 ? 1 : 2) * a.bn) a.tmem_cols *= 2;
-  if (recv > a.stages * stage) return FELLM_ERR_SIZE;
+  if (!a.recv_apart && recv > a.stages * stage) return FELLM_ERR_SIZE;
   EncodeTiledFn fn = encode_fn();
   if (!fn) return FELLM_ERR_ARG;
   CUtensorMap map;
@@ -533,10 +589,11 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return 1000 + (int)r;
-  const size_t smem = (size_t)a.stages * stage + 1024;
+  const size_t smem = (size_t)a.stages * stage + (a.recv_apart ? recv : 0) + 1024;
   const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
-  auto kern = parts == 1 ? (a.splits > 1 ? gemm_w4_umma_kernel<true, 1> : gemm_w4_umma_kernel<false, 1>)
-                         : (a.splits > 1 ? gemm_w4_umma_kernel<true, 3> : gemm_w4_umma_kernel<false, 3>);
+  auto kern = parts == 3 ? (a.splits > 1 ? gemm_w4_umma_kernel<true, 3, 1> : gemm_w4_umma_kernel<false, 3, 1>)
+            : kb == 2    ? (a.splits > 1 ? gemm_w4_umma_kernel<true, 1, 2> : gemm_w4_umma_kernel<false, 1, 2>)
+                         : (a.splits > 1 ? gemm_w4_umma_kernel<true, 1, 1> : gemm_w4_umma_kernel<false, 1, 1>);
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
