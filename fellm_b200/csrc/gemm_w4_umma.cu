@@ -117,18 +117,6 @@ struct W4uArgs {
   int recv_apart;            // what other ranks send lies behind the stages, not over them
 };
 
-// The four words of a lane (rows g and g + 8, 16 elements each) -> its pieces of the tile.  Neighbouring even and odd rows
-// are written half a row apart, so that eight lanes of a store meet every bank once.
-__device__ __forceinline__ unsigned w4_value(unsigned word, int r, unsigned s2, unsigned off2) {
-  const unsigned b = w4_pair_biased(word, r);
-  __nv_bfloat162 v = __hfma2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&s2, *(const __nv_bfloat162*)&off2);
-  return *(unsigned*)&v;
-}
-__device__ __forceinline__ unsigned times_minus_24(unsigned s2) {
-  const unsigned c = W4_MINUS_24;
-  __nv_bfloat162 v = __hmul2(*(const __nv_bfloat162*)&s2, *(const __nv_bfloat162*)&c);
-  return *(unsigned*)&v;
-}
 __device__ __forceinline__ void st_shared_v4(unsigned addr, unsigned a, unsigned b, unsigned c, unsigned d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }

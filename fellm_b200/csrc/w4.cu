@@ -21,16 +21,26 @@ __device__ __forceinline__ float group_scale(float hi, float lo, bool finite) {
   if (s < 1.1754943508222875e-38f) s = 0.f;
   return hi > -lo ? -s : s;
 }
-// The level of w under scale s, 0..15 = level + 8: w / s rounded to the nearest whole number, ties to even, EXACTLY.  The
-// quotient's own rounding may carry it onto or over a half; the remainder w - q s is exact in one fused operation (q s has
-// at most nine bits, and what is left of w is below s), and it says which side w lies on.
-__device__ __forceinline__ unsigned level_of(float w, float s) {
-  if (!(s != 0.f) || s != s) return 8u;
-  float q = rintf(w / s);
-  const float left = fmaf(-q, s, w), half = 0.5f * fabsf(s);
-  if (fabsf(left) > half) q += ((left > 0.f) == (s > 0.f)) ? 1.f : -1.f;
-  q = fminf(fmaxf(q, -8.f), 7.f);
-  return (unsigned)((int)q + 8);
+// The level of w under scale s (inv: 1 / s rounded, 0 for scale 0), 0..15 = level + 8: w / s to the nearest whole number, ties to even,
+// EXACTLY.  x = w inv, corrected once by its remainder, is the quotient rounded to float32 (Markstein: a correctly rounded reciprocal
+// and one fused correction give the correctly rounded quotient).  A bfloat16 w over five bits cannot lie so near a half that this
+// rounding reaches it (both are fractions of small numbers: 2^-10 away at least, or on it).  A float32 w can: there the remainder
+// w - q s, exact in one fused operation (q s has at most nine bits, what is left of w is below s), says on which side it lies.
+template <bool NARROW>
+__device__ __forceinline__ unsigned level_of(float w, float s, float inv) {
+  float x = w * inv;
+  x = fmaf(fmaf(-x, s, w), inv, x);
+  x = fminf(fmaxf(x, -8.f), 7.f);
+  const float up = x + 12582920.f;                          // 1.5 * 2^23 + 8: the sum's last place is a whole number's
+  unsigned level = __float_as_uint(up) & 15u;
+  if (!NARROW) {
+    const float left = fmaf(-(up - 12582920.f), s, w), half = 0.5f * fabsf(s);
+    if (fabsf(left) > half) {
+      if ((left > 0.f) == (s > 0.f)) { if (level < 15u) ++level; }
+      else if (level > 0u) --level;
+    }
+  }
+  return level;
 }
 
 // What lane (g, c) keeps of two chunks: rows g, g + 8 x quarters of 32 elements x its eight.
@@ -64,10 +74,37 @@ __device__ __forceinline__ unsigned pack_word(const unsigned* a, const unsigned*
 
 struct W4Out { uint4* q; unsigned* s; int N, K, chunks, groups, gshift; };
 
-// A warp a slab x 128 elements.  Bound by the matrix's bytes: every element is read once, by loads of 16 bytes whose four
-// neighbouring lanes take 64 (128 where T is float) consecutive bytes of a row.
-template <typename T>
-__global__ void __launch_bounds__(W4_THREADS) quantize_w4_kernel(const T* w, long long ldw, int vec, W4Out o) {
+// A warp's slab x 128 elements in levels: lane (g, c) has rows g, g + 8, four quarters of 32 elements, eight of each.
+// element(r, h, i) gives them as float32, s and inv the scale and its reciprocal of every row and quarter.
+template <bool NARROW, class Element>
+__device__ __forceinline__ void put_levels(const W4Out& o, int slab, int pair, int lane, Element element, const float (*s)[4], const float (*inv)[4]) {
+#pragma unroll
+  for (int ch = 0; ch < 2; ++ch) {
+    if (2 * pair + ch >= o.chunks) break;
+    unsigned word[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int q = 2 * ch + h;
+      unsigned a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { a[i] = level_of<NARROW>(element(0, q, i), s[0][q], inv[0][q]); b[i] = level_of<NARROW>(element(1, q, i), s[1][q], inv[1][q]); }
+      word[2 * h] = pack_word(a, b); word[2 * h + 1] = pack_word(a + 4, b + 4);
+    }
+    o.q[((size_t)slab * o.chunks + 2 * pair + ch) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+  }
+  // quarter c's scales by lane c (a group's first quarter only)
+  const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    if (c != h || ((h << 5) & ((1 << o.gshift) - 1))) continue;
+    const int grp = (pair * 128 + h * 32) >> o.gshift;
+    if (grp < o.groups) o.s[((size_t)slab * o.groups + grp) * 8 + g] = __float_as_uint(s[0][h]) >> 16 | (__float_as_uint(s[1][h]) & 0xffff0000u);
+  }
+}
+
+// A warp a slab x 128 elements.  Bound by the matrix's bytes: every element is read once, by loads of 16 bytes of which four neighbouring
+// lanes take 64 consecutive bytes of a row (128 of a float32 one).
+__global__ void __launch_bounds__(W4_THREADS) quantize_w4_f32_kernel(const float* w, long long ldw, int vec, W4Out o) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int pairs = (o.chunks + 1) / 2;
   const long long unit = (long long)blockIdx.x * (W4_THREADS / 32) + (threadIdx.x >> 5);
@@ -79,7 +116,7 @@ __global__ void __launch_bounds__(W4_THREADS) quantize_w4_kernel(const T* w, lon
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int n = slab * W4_SLAB + g + 8 * r;
-    const T* row = w + (size_t)n * ldw;
+    const float* row = w + (size_t)n * ldw;
 #pragma unroll
     for (int h = 0; h < 4; ++h) load8(row, n < o.N, pair * 128 + h * 32 + c * 8, o.K, vec != 0, v[r][h]);
   }
@@ -87,10 +124,10 @@ __global__ void __launch_bounds__(W4_THREADS) quantize_w4_kernel(const T* w, lon
   for (int r = 0; r < 2; ++r)
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      float a = v[r][h][0], b = a;
-      bool ok = true;
+      float a = v[r][h][0], b = a, zero = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { a = fmaxf(a, v[r][h][i]); b = fminf(b, v[r][h][i]); ok = ok && fabsf(v[r][h][i]) <= 3.4028234663852886e38f; }
+      for (int i = 0; i < 8; ++i) { a = fmaxf(a, v[r][h][i]); b = fminf(b, v[r][h][i]); zero = fmaf(v[r][h][i], 0.f, zero); }
+      bool ok = zero == 0.f;                                // (0 times an infinity or NaN is none)
 #pragma unroll
       for (int x = 1; x < 4; x <<= 1) {
         a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
@@ -112,34 +149,79 @@ __global__ void __launch_bounds__(W4_THREADS) quantize_w4_kernel(const T* w, lon
         hi[r][h] = hi[r][h | step] = a; lo[r][h] = lo[r][h | step] = b; fin[r][h] = fin[r][h | step] = ok;
       }
     }
-  float s[2][4];
+  float s[2][4], inv[2][4];
 #pragma unroll
   for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int h = 0; h < 4; ++h) s[r][h] = group_scale(hi[r][h], lo[r][h], fin[r][h]);
-#pragma unroll
-  for (int ch = 0; ch < 2; ++ch) {
-    if (2 * pair + ch >= o.chunks) break;
-    unsigned word[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      unsigned a[8], b[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) { a[i] = level_of(v[0][2 * ch + h][i], s[0][2 * ch + h]); b[i] = level_of(v[1][2 * ch + h][i], s[1][2 * ch + h]); }
-      word[2 * h] = pack_word(a, b); word[2 * h + 1] = pack_word(a + 4, b + 4);
+    for (int h = 0; h < 4; ++h) {
+      s[r][h] = group_scale(hi[r][h], lo[r][h], fin[r][h]);
+      inv[r][h] = s[r][h] != 0.f ? 1.f / s[r][h] : 0.f;
     }
-    o.q[((size_t)slab * o.chunks + 2 * pair + ch) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
-  }
-  // quarter c's scales by lane c (a group's first quarter only)
+  put_levels<false>(o, slab, pair, lane, [&](int r, int h, int i) { return v[r][h][i]; }, s, inv);
+}
+
+// bfloat16: the elements stay as they came (two in a register), their extremes are taken two at a time.  A group's largest element and the
+// negative of its smallest travel as one pair; an element that is none makes them none, an infinity is one of them.
+__device__ __forceinline__ unsigned max2_nan(unsigned a, unsigned b) {
+  __nv_bfloat162 v = __hmax2_nan(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+  return *(unsigned*)&v;
+}
+__global__ void __launch_bounds__(W4_THREADS) quantize_w4_bf16_kernel(const bf16* w, long long ldw, int vec, W4Out o) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int pairs = (o.chunks + 1) / 2;
+  const long long unit = (long long)blockIdx.x * (W4_THREADS / 32) + (threadIdx.x >> 5);
+  const int slab = (int)(unit / pairs), pair = (int)(unit % pairs);
+  if (slab * W4_SLAB >= o.N) return;
+  uint4 raw[2][4];
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    if (c != h || ((h << 5) & ((1 << o.gshift) - 1))) continue;
-    const int grp = (pair * 128 + h * 32) >> o.gshift;
-    if (grp < o.groups) {
-      const unsigned lo16 = __float_as_uint(s[0][h]) >> 16, hi16 = __float_as_uint(s[1][h]) & 0xffff0000u;
-      o.s[((size_t)slab * o.groups + grp) * 8 + g] = lo16 | hi16;
+  for (int r = 0; r < 2; ++r) {
+    const int n = slab * W4_SLAB + g + 8 * r;
+    const unsigned short* row = (const unsigned short*)w + (size_t)n * ldw;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int k = pair * 128 + h * 32 + c * 8;
+      if (n < o.N && vec && k + 8 <= o.K) raw[r][h] = *(const uint4*)(row + k);
+      else {
+        unsigned x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned lo = n < o.N && k + 2 * i < o.K ? row[k + 2 * i] : 0, hi = n < o.N && k + 2 * i + 1 < o.K ? row[k + 2 * i + 1] : 0;
+          x[i] = lo | hi << 16;
+        }
+        raw[r][h] = make_uint4(x[0], x[1], x[2], x[3]);
+      }
     }
   }
+  unsigned m[2][4];                                          // (largest, minus the smallest)
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const unsigned x[4] = {raw[r][h].x, raw[r][h].y, raw[r][h].z, raw[r][h].w}, sign = 0x80008000u;
+      const unsigned up = max2_nan(max2_nan(x[0], x[1]), max2_nan(x[2], x[3]));
+      const unsigned down = max2_nan(max2_nan(x[0] ^ sign, x[1] ^ sign), max2_nan(x[2] ^ sign, x[3] ^ sign));
+      m[r][h] = max2_nan(__byte_perm(up, down, 0x5410), __byte_perm(up, down, 0x7632));
+    }
+  float s[2][4], inv[2][4];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    if (o.gshift >= 6) { m[r][0] = m[r][1] = max2_nan(m[r][0], m[r][1]); m[r][2] = m[r][3] = max2_nan(m[r][2], m[r][3]); }
+    if (o.gshift == 7) m[r][0] = m[r][1] = m[r][2] = m[r][3] = max2_nan(m[r][0], m[r][2]);
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      if ((h << 5) & ((1 << o.gshift) - 1)) { s[r][h] = s[r][h - 1]; inv[r][h] = inv[r][h - 1]; continue; }
+      unsigned x = m[r][h];
+      x = max2_nan(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      x = max2_nan(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      const float hi = __uint_as_float(x << 16), lo = -__uint_as_float(x & 0xffff0000u);
+      s[r][h] = group_scale(hi, lo, fabsf(hi) <= 3.4028234663852886e38f && fabsf(lo) <= 3.4028234663852886e38f);
+      inv[r][h] = s[r][h] != 0.f ? 1.f / s[r][h] : 0.f;
+    }
+  }
+  put_levels<true>(o, slab, pair, lane, [&](int r, int h, int i) {
+    const unsigned x[4] = {raw[r][h].x, raw[r][h].y, raw[r][h].z, raw[r][h].w};
+    return i & 1 ? __uint_as_float(x[i >> 1] & 0xffff0000u) : __uint_as_float(x[i >> 1] << 16);
+  }, s, inv);
 }
 
 // Levels and scales that exist already -> the layout.  bad: 1 a level outside -8..7, 2 a scale that is not finite, has more
@@ -224,16 +306,33 @@ __device__ __forceinline__ void store8(T* p, const float* v, int left, bool vec)
   for (int i = 0; i < 8; ++i) if (i < left) p[i] = from_f<T>(v[i]);
 }
 
-// A thread eight elements: the values themselves (exact in either type).
+// The matrix's values (exact in either type).  A warp a slab x chunk: 16 bytes a lane in, a lane's pieces of 8 elements of its two rows out.
 template <typename T>
 __global__ void __launch_bounds__(W4_THREADS) dequantize_w4_kernel(W4Ref m, T* out, long long ldo, int vec) {
-  const int pieces = (m.K + 7) / 8;
-  const long long i = (long long)blockIdx.x * W4_THREADS + threadIdx.x;
-  const int row = (int)(i / pieces), k = (int)(i % pieces) * 8;
-  if (row >= m.N) return;
-  float v[8];
-  row8(m, row, k, v);
-  store8(out + (size_t)row * ldo + k, v, m.K - k, vec != 0);
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const long long unit = (long long)blockIdx.x * (W4_THREADS / 32) + (threadIdx.x >> 5);
+  const int slab = (int)(unit / m.chunks), chunk = (int)(unit % m.chunks);
+  if (slab * W4_SLAB >= m.N) return;
+  const uint4 q = m.q[(size_t)unit * 32 + lane];
+  const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int k = chunk * W4_CHUNK + h * 32 + c * 8;
+    const unsigned s = m.s[((size_t)slab * m.groups + ((chunk * W4_CHUNK + h * 32) >> m.gshift)) * 8 + g];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int n = slab * W4_SLAB + g + 8 * r;
+      const unsigned s2 = __byte_perm(s, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
+      const unsigned v[4] = {w4_value(w[2 * h], r, s2, off), w4_value(w[2 * h], r + 2, s2, off), w4_value(w[2 * h + 1], r, s2, off), w4_value(w[2 * h + 1], r + 2, s2, off)};
+      if (n >= m.N) continue;
+      T* p = out + (size_t)n * ldo + k;
+      if (sizeof(T) == 2 && vec && k + 8 <= m.K) { *(uint4*)p = make_uint4(v[0], v[1], v[2], v[3]); continue; }
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(v[i] << 16); f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u); }
+      store8(p, f, m.K - k, vec != 0);
+    }
+  }
 }
 
 // A thread eight elements of a token's row, times `scale`.  A token outside the table: zeros and *status = 1.
@@ -267,8 +366,8 @@ FELLM_API int fellm_quantize_w4(const void* w, int w_bf16, long long ldw, const 
   const W4Out o = {(uint4*)m->q, (unsigned*)m->s, m->N, m->K, m->chunks, m->groups, m->gshift};
   const long long units = (long long)ceil_div(m->N, W4_SLAB) * ((m->chunks + 1) / 2), blocks = (units + W4_THREADS / 32 - 1) / (W4_THREADS / 32);
   if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
-  if (w_bf16) quantize_w4_kernel<bf16><<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const bf16*)w, ldw, ldw % 8 == 0 && ((uintptr_t)w & 15) == 0, o);
-  else quantize_w4_kernel<float><<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const float*)w, ldw, ldw % 4 == 0 && ((uintptr_t)w & 15) == 0, o);
+  if (w_bf16) quantize_w4_bf16_kernel<<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const bf16*)w, ldw, ldw % 8 == 0 && ((uintptr_t)w & 15) == 0, o);
+  else quantize_w4_f32_kernel<<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const float*)w, ldw, ldw % 4 == 0 && ((uintptr_t)w & 15) == 0, o);
   return launch_status();
 }
 FELLM_API int fellm_pack_w4(const void* levels, long long ldl, const void* scales, long long lds, int groups_in, const W4Ref* m, int* bad, cudaStream_t stream) {
@@ -283,7 +382,7 @@ FELLM_API int fellm_pack_w4(const void* levels, long long ldl, const void* scale
 FELLM_API int fellm_dequantize_w4(const W4Ref* m, void* out, int out_bf16, long long ldo, cudaStream_t stream) {
   if (!out) return FELLM_ERR_ARG;
   if (int e = w4_check(m)) return e;
-  const long long blocks = ((long long)m->N * ceil_div(m->K, 8) + W4_THREADS - 1) / W4_THREADS;
+  const long long blocks = ((long long)ceil_div(m->N, W4_SLAB) * m->chunks + W4_THREADS / 32 - 1) / (W4_THREADS / 32);
   if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
   const int vec = ldo % (out_bf16 ? 8 : 4) == 0 && ((uintptr_t)out & 15) == 0;
   if (out_bf16) dequantize_w4_kernel<bf16><<<(unsigned)blocks, W4_THREADS, 0, stream>>>(*m, (bf16*)out, ldo, vec);

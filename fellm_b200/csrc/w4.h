@@ -45,6 +45,18 @@ __device__ __forceinline__ unsigned w4_pair(unsigned word, int r) {
   __nv_bfloat162 v = __hadd2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&off);
   return *(unsigned*)&v;
 }
+// The r-th pair of a word times its scale (s2: in both halves; off2: times -24 of it): (16 + q + 8) s - 24 s in one fused operation, exact,
+// since 24 s and the result are bfloat16 numbers.
+__device__ __forceinline__ unsigned w4_value(unsigned word, int r, unsigned s2, unsigned off2) {
+  const unsigned b = w4_pair_biased(word, r);
+  __nv_bfloat162 v = __hfma2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&s2, *(const __nv_bfloat162*)&off2);
+  return *(unsigned*)&v;
+}
+__device__ __forceinline__ unsigned times_minus_24(unsigned s2) {
+  const unsigned c = W4_MINUS_24;
+  __nv_bfloat162 v = __hmul2(*(const __nv_bfloat162*)&s2, *(const __nv_bfloat162*)&c);
+  return *(unsigned*)&v;
+}
 __device__ __forceinline__ float w4_scale_lo(unsigned s) { return __uint_as_float(s << 16); }
 __device__ __forceinline__ float w4_scale_hi(unsigned s) { return __uint_as_float(s & 0xffff0000u); }
 // A float32 number as three bfloat16 ones (in the upper halves), a + b + c = v exactly: 8 bits of its mantissa each (as far
