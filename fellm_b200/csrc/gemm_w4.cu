@@ -275,7 +275,10 @@ static int launch_rows(const GwArgs& a, cudaStream_t stream) {
   const int slabs = ceil_div(ceil_div(a.w.N, W4_SLAB), R), units = ceil_div(a.w.chunks, 4 / R), n_sm = fellm_sm_count(), tiles = ceil_div(a.M, 8 * NT);
   auto kern = gemm_w4_rows_kernel<XT, NT, GS, R>;
   auto bytes = [](int warps) { return (size_t)warps * (GW_DEPTH * GW_SLOT + rows_buffers(NT) * 8 * NT * (R * W4_SLAB + 1) * 4); };
-  static int resident = 0;                              // blocks of eight warps an SM holds, asked once
+  static int asked[64];                                 // blocks of eight warps an SM holds, asked once a device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FELLM_ERR_ARG;
+  int& resident = asked[dev];
   if (!resident) {
     int n = 0;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(16));

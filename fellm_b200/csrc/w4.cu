@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(W4_THREADS) embed_rows_w4_kernel(const int* to
 
 static bool grid_ok(long long blocks) { return blocks > 0 && blocks < (1ll << 31); }
 
+// Returns when the matrix is laid out: a product reads it ahead of the kernel in front, on whatever stream.
 FELLM_API int fellm_quantize_w4(const void* w, int w_bf16, long long ldw, const W4Ref* m, cudaStream_t stream) {
   if (!w) return FELLM_ERR_ARG;
   if (int e = w4_check(m)) return e;
@@ -368,7 +369,8 @@ FELLM_API int fellm_quantize_w4(const void* w, int w_bf16, long long ldw, const 
   if (!grid_ok(blocks)) return FELLM_ERR_SIZE;
   if (w_bf16) quantize_w4_bf16_kernel<<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const bf16*)w, ldw, ldw % 8 == 0 && ((uintptr_t)w & 15) == 0, o);
   else quantize_w4_f32_kernel<<<(unsigned)blocks, W4_THREADS, 0, stream>>>((const float*)w, ldw, ldw % 4 == 0 && ((uintptr_t)w & 15) == 0, o);
-  return launch_status();
+  const int e = launch_status();
+  return e ? e : (int)cudaStreamSynchronize(stream);
 }
 FELLM_API int fellm_pack_w4(const void* levels, long long ldl, const void* scales, long long lds, int groups_in, const W4Ref* m, int* bad, cudaStream_t stream) {
   if (!levels || !scales || !bad) return FELLM_ERR_ARG;

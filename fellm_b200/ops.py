@@ -2002,7 +2002,8 @@ class W4:
         self.q, self.scales, self.shape, self.group = q, scales, (N, K), group
         self.device, self.is_cuda = q.device, q.is_cuda
         self._device = q.get_device()
-        self._ref = _W4Ref(q.data_ptr(), scales.data_ptr(), N, K, q.shape[1], scales.shape[1], group.bit_length() - 1)
+        chunks = -(-K // 64)
+        self._ref = _W4Ref(q.data_ptr(), scales.data_ptr(), N, K, chunks, -(-chunks * 64 // group), group.bit_length() - 1)
         self._at = ctypes.addressof(self._ref)
 
     def nbytes(self) -> int:
@@ -2022,18 +2023,14 @@ def _w4_dev(*tensors):
 
 
 def _w4_room(N: int, K: int, group: int, device):
-    """(levels [slabs, chunks, 128], scales [slabs, groups, 8]), each with room behind it that a kernel may read ahead into."""
+    """Levels [slabs, chunks, 128] and scales [slabs, groups, 8], each with room behind it that a kernel may read ahead into."""
     if group not in W4_GROUPS:
         raise KernelError(f"a group of {group}: four-bit matrices have groups of {', '.join(map(str, W4_GROUPS))}")
     if N < 1 or K < 1 or N > 2 ** 30 or K > 2 ** 30:
         raise KernelError(f"a matrix of {N} x {K} cannot be held in four bits")
     slabs, chunks = -(-N // 16), -(-K // 64)
-    groups = -(-chunks * 64 // group)
-    made = []
-    for shape, behind in (((slabs, chunks, 128), W4_READ_AHEAD * 128), ((slabs, groups, 8), W4_READ_AHEAD * 16)):
-        n = shape[0] * shape[1] * shape[2]
-        made.append(torch.empty(n + behind, dtype=torch.int32, device=device)[:n].view(shape))
-    return tuple(made)
+    return (torch.empty((slabs * chunks + W4_READ_AHEAD) * 128, dtype=torch.int32, device=device),
+            torch.empty(slabs * -(-chunks * 64 // group) * 8 + W4_READ_AHEAD * 16, dtype=torch.int32, device=device))
 
 
 def _w4_matrix(w, what: str):
@@ -2057,7 +2054,6 @@ def quantize_w4(w, group: int = 64) -> W4:
     out = W4(q, s, w.shape[0], w.shape[1], group)
     f = _fn("w4", "fellm_quantize_w4", [_c_p, _c_int, _c_ll, _c_p, _c_p])
     _check(f(_p(w), _is_bf16(w), w.stride(0), out._at, _stream()), "quantize_w4")
-    torch.cuda.current_stream().synchronize()
     return out
 
 
@@ -2169,16 +2165,18 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
         residual_written(out)
     if M == 0:
         return out
-    at = x.data_ptr()
+    at, to = x.data_ptr(), out.data_ptr()
+    if at == to:
+        raise KernelError("gemm_w4: the result cannot take the place of x")
     if M > W4_FEW_ROWS:
         scratch = None
         if not x_bf16 or K % 8 or ldx % 8 or ldx < K or at % 16:       # (what TMA does not read)
             scratch = torch.empty(M * -(-K // 64) * (64 if x_bf16 else 192), dtype=torch.bfloat16, device=x.device)
         f = _fn("gemm_w4_umma", "fellm_gemm_w4_umma", _GEMM_W4_ARGS[:-1] + [_c_p, _c_p, _c_p])
-        _check(f(at, ldx, w._at, _p(bias), out.data_ptr(), ldo, flags, M, _p(scratch), _p(umma_status(x.device)), _stream()), "gemm_w4_umma")
+        _check(f(at, ldx, w._at, _p(bias), to, ldo, flags, M, _p(scratch), _p(umma_status(x.device)), _stream()), "gemm_w4_umma")
         return out
     f = _fn("gemm_w4", "fellm_gemm_w4", _GEMM_W4_ARGS)
-    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), out.data_ptr(), ldo, flags, M, _stream()), "gemm_w4")
+    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), to, ldo, flags, M, _stream()), "gemm_w4")
     return out
 
 

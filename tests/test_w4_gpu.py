@@ -10,7 +10,7 @@ import w4_util
 
 DEV = "cuda"
 SIZES = [(16, 64, 32), (1, 1, 32), (17, 33, 32), (40, 200, 64), (129, 130, 128), (1003, 1357, 32), (256, 1024, 64), (272, 2056, 128), (2064, 64, 64),
-         (48, 8200, 128)]
+         (48, 8200, 128), (2100, 200, 32), (4100, 520, 128), (40000, 136, 32)]
 
 
 def _gen(*seed):
@@ -259,3 +259,77 @@ def test_the_same_bits_every_time(M):
     first = ops.gemm_w4(x, w4, out_dtype=torch.float32)
     for _ in range(5):
         assert torch.equal(ops.gemm_w4(x, w4, out_dtype=torch.float32), first)
+
+
+@pytest.mark.gpu
+def test_a_result_cannot_take_the_place_of_x():
+    from fellm_b200 import ops
+    from fellm_b200.config.errors import KernelError
+    w4 = ops.quantize_w4(torch.randn(64, 64, device=DEV), 32)
+    for M in (2, 40):
+        x = torch.randn(M, 64, device=DEV)
+        with pytest.raises(KernelError, match="place"):
+            ops.gemm_w4(x, w4, out=x)
+        with pytest.raises(KernelError, match="place"):
+            ops.gemm_w4(x, w4, out=x, accumulate=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 7, 16, 40, 200])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_captured_products_and_products_on_two_streams(M, dtype):
+    """The same matrix read by a replayed graph, by this stream and by another one at once; new rows of x for every replay."""
+    from fellm_b200 import ops
+    g = _gen(M, 11)
+    levels, scales = w4_util.random_matrix(2064, 520, 64, g, DEV)
+    w4, w = ops.pack_w4(levels, scales, 64), w4_util.plain_values(levels, scales, 64)
+    xs = [w4_util.whole_rows(M, 520, dtype, g, DEV) for _ in range(6)]
+    want = [w4_util.plain_product(x, w) for x in xs]
+    held = xs[0].clone()
+    y = torch.empty(M, 2064, device=DEV)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.gemm_w4(held, w4, out=y)                       # (loads the kernels before the capture)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        half = ops.gemm_w4(held, w4, out_dtype=torch.float32) if M > 16 else None
+        ops.gemm_w4(held, w4, out=y)
+    for i in range(1, 6):
+        held.copy_(xs[i])
+        graph.replay()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            beside = [ops.gemm_w4(xs[j], w4, out_dtype=torch.float32) for j in range(6)]
+        here = [ops.gemm_w4(xs[j], w4, out_dtype=torch.float32) for j in range(6)]
+        torch.cuda.synchronize()
+        assert torch.equal(y.double(), want[i]) and (half is None or torch.equal(half.double(), want[i]))
+        for got in (beside, here):
+            assert all(torch.equal(a.double(), b) for a, b in zip(got, want))
+    ops.check_umma_status(DEV)
+
+
+@pytest.mark.gpu
+def test_laying_out_is_refused_inside_a_capture():
+    from fellm_b200 import ops
+    from fellm_b200.config.errors import KernelError
+    w = torch.randn(64, 64, device=DEV)
+    ops.quantize_w4(w, 32)
+    lv, sc = torch.zeros(64, 64, dtype=torch.int8, device=DEV), torch.ones(64, 2, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(KernelError, match="captured"):
+            ops.quantize_w4(w, 32)
+        with pytest.raises(KernelError, match="captured"):
+            ops.pack_w4(lv, sc, 32)
+        w.add_(1)
+
+
+@pytest.mark.gpu
+def test_a_matrix_of_zeros_and_rows_of_zeros():
+    from fellm_b200 import ops
+    zero = ops.quantize_w4(torch.zeros(40, 200, device=DEV), 64)
+    assert (ops.dequantize_w4(zero) == 0).all()
+    for M in (1, 9, 40):
+        assert (ops.gemm_w4(torch.randn(M, 200, device=DEV).bfloat16(), zero) == 0).all()
+        assert (ops.gemm_w4(torch.zeros(M, 200, device=DEV), ops.quantize_w4(torch.randn(40, 200, device=DEV), 64)) == 0).all()
