@@ -13,13 +13,14 @@
 // is not unpacking is shared out over four chunks.
 //
 // float32 rows of x are cut into three bfloat16 numbers each, x = x1 + x2 + x3 exactly (8 bits of the mantissa a piece, so
-// nothing is rounded), which meet the same weights in three MMAs.
+// nothing is rounded), which meet the same weights in three MMAs.  Cut by every warp for itself, that is more work than unpacking the
+// weights (five rows, 8,192 x 8,192: 37 us): a large matrix has them cut once, by a launch in front.
 #include "w4.h"
 
 #define GW_DEPTH 4                     // units of a warp's ring: one is used, the others are on their way
 #define GW_SLOT (4 * (512 + 64))       // a unit: four chunks' levels, their groups' scales (eight at groups of 32)
 
-enum { X_BF16 = 0, X_BF16_ANY = 1, X_F32 = 2 };       // rows on 16 bytes and K a multiple of 8; any bfloat16; float32
+enum { X_BF16 = 0, X_BF16_ANY = 1, X_F32 = 2, X_CUT = 3 };       // rows on 16 bytes and K a multiple of 8; any bfloat16; float32; float32 cut by w4_rows_kernel
 
 struct GwArgs {
   W4Ref w;
@@ -33,12 +34,18 @@ __device__ __forceinline__ void mma_bf16(float* d, const unsigned* a, unsigned b
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Eight elements of a row of x from k on as operand registers [part][4].
-template <int XT> struct XParts { static constexpr int N = XT == X_F32 ? 3 : 1; };
+template <int XT> struct XParts { static constexpr int N = XT == X_F32 || XT == X_CUT ? 3 : 1; };
 // Eight elements from p on, of which `left` are the row's.  FULL: all eight.
 template <int XT, bool FULL>
 __device__ __forceinline__ void load_x8(const void* at, int left, unsigned (*b)[4]) {
   constexpr int P = XParts<XT>::N;
-  if (XT == X_BF16) {
+  if (XT == X_CUT) {
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      const uint4 v = *(const uint4*)((const unsigned char*)at + (2 - q) * W4_CHUNK * 2);
+      b[q][0] = v.x; b[q][1] = v.y; b[q][2] = v.z; b[q][3] = v.w;
+    }
+  } else if (XT == X_BF16) {
     const uint4 v = FULL || left > 0 ? *(const uint4*)at : make_uint4(0u, 0u, 0u, 0u);
     b[0][0] = v.x; b[0][1] = v.y; b[0][2] = v.z; b[0][3] = v.w;
   } else if (XT == X_BF16_ANY) {
@@ -121,7 +128,7 @@ __host__ __device__ constexpr int rows_buffers(int nt) { return nt < 4 ? 2 : 1; 
 // R of them, a unit 4 / R chunks of each): the same columns' operands for both.
 template <int XT, int NT, int GS, int R>
 __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
-  constexpr int UNIT = 4 / R, ROWS = R * W4_SLAB, P = XParts<XT>::N, COLS = 8 * NT, XB = XT == X_F32 ? 4 : 2;      // XB: bytes of an element of x
+  constexpr int UNIT = 4 / R, ROWS = R * W4_SLAB, P = XParts<XT>::N, COLS = 8 * NT, XB = XT == X_F32 ? 4 : 2, XC = W4_CHUNK * XB * (XT == X_CUT ? 3 : 1);      // bytes of an element and of a chunk of x
   extern __shared__ __align__(16) unsigned char smem[];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int all_slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB, slabs = (all_slabs + R - 1) / R, m0 = blockIdx.y * COLS, cols = min(a.M - m0, COLS);
@@ -188,7 +195,7 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          load_x8<XT, decltype(full)::value>(xu[t] + (i * W4_CHUNK + h * 32) * XB, a.w.K - (u * UNIT + i) * W4_CHUNK - h * 32 - c * 8, b[h][t]);
+          load_x8<XT, decltype(full)::value>(xu[t] + i * XC + h * 32 * XB, a.w.K - (u * UNIT + i) * W4_CHUNK - h * 32 - c * 8, b[h][t]);
 #pragma unroll
       for (int k = 0; k < R; ++k) {
         const uint4 qv = k ? lds128<i * 512 + 1024>(at + lane * 16) : lds128<i * 512>(at + lane * 16);
@@ -230,7 +237,7 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
       fetch();                                               // over that one
       const unsigned char* xu[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) xu[t] = xrow[t] + (size_t)u * (UNIT * W4_CHUNK * XB);
+      for (int t = 0; t < NT; ++t) xu[t] = xrow[t] + (size_t)u * (UNIT * XC);
       if ((u + 1) * UNIT * W4_CHUNK <= a.w.K) {
         chunk(Int<0>(), u, xu, TrueType()); chunk(Int<1>(), u, xu, TrueType());
         if (R == 1) { chunk(Int<2 / R>(), u, xu, TrueType()); chunk(Int<3 / R>(), u, xu, TrueType()); }
@@ -299,16 +306,23 @@ static int launch_rows_group(const GwArgs& a, cudaStream_t stream) {
 }
 
 // x [M, K] (x_bf16: bfloat16, else float32), out [M, N] ([M, N/2] for the gated form, whose rows are 8 gate, 8 up, ...).
-FELLM_API int fellm_gemm_w4(const void* x, long long ldx, const W4Ref* w, const float* bias, void* out, long long ldo, int flags, int M, cudaStream_t stream) {
+// scratch: null, or room for float32 rows cut in three, M x chunks x 192 numbers of bfloat16.
+FELLM_API int fellm_gemm_w4(const void* x, long long ldx, const W4Ref* w, const float* bias, void* out, long long ldo, int flags, int M, void* scratch,
+                            cudaStream_t stream) {
   if (M <= 0) return 0;
   if (!x || !out) return FELLM_ERR_ARG;
   if (int e = w4_check(w)) return e;
   if (int e = w4_check_epi(flags, w->N)) return e;
   const int x_bf16 = flags & W4_X_BF16, N = w->N, K = w->K;
-  const GwArgs a = {*w, x, bias, out, ldx, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0};
+  GwArgs a = {*w, x, bias, out, ldx, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0};
+  if (!x_bf16 && scratch) {
+    if (int e = w4_copy_rows(x, 0, ldx, scratch, M, K, w->chunks, stream)) return e;
+    a.x = scratch; a.ldx = 3ll * w->chunks * W4_CHUNK;
+    return launch_rows_group<X_CUT, 1, 1>(a, stream);
+  }
   if (!x_bf16) return launch_rows_group<X_F32, 1, 1>(a, stream);
   if (K % 8 || ldx % 8 || ((uintptr_t)x & 15)) return launch_rows_group<X_BF16_ANY, 1, 1>(a, stream);
   if (M <= 8) return launch_rows_group<X_BF16, 1, 1>(a, stream);
-  if (M <= 16) return N <= 2048 ? launch_rows_group<X_BF16, 2, 1>(a, stream) : launch_rows_group<X_BF16, 2, 2>(a, stream);
-  return launch_rows_group<X_BF16, 4, 2>(a, stream);
+  // (9 to 16 rows: pairs of slabs where every SM gets one, 9,216 x 1,024 4.2 -> 3.8 us; else each for itself, 4,096 x 1,024 3.4 -> 2.8)
+  return N <= 2 * W4_SLAB * fellm_sm_count() ? launch_rows_group<X_BF16, 2, 1>(a, stream) : launch_rows_group<X_BF16, 2, 2>(a, stream);
 }

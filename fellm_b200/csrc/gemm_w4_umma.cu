@@ -469,25 +469,6 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   }
 }
 
-// Rows that TMA cannot read as they are: bfloat16 rows on no 16-byte boundary or of a K that is no multiple of 8 (copied,
-// zeros up to whole chunks), and float32 rows, every 64 elements of which become three times 64 bfloat16 whose sum they are.
-__global__ void __launch_bounds__(256) w4_rows_kernel(const void* x, int x_bf16, long long ldx, unsigned short* out, int M, int K, int chunks) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int width = chunks * W4_CHUNK;
-  const int m = (int)(i / width), k = (int)(i % width);
-  if (m >= M) return;
-  if (x_bf16) {
-    out[i] = k < K ? ((const unsigned short*)x)[(size_t)m * ldx + k] : (unsigned short)0;
-    return;
-  }
-  unsigned a, b, c;
-  w4_split3(k < K ? ((const float*)x)[(size_t)m * ldx + k] : 0.f, a, b, c);
-  unsigned short* o = out + (size_t)m * 3 * width + (size_t)(k / W4_CHUNK) * 3 * W4_CHUNK + k % W4_CHUNK;
-  o[0] = (unsigned short)(c >> 16); o[W4_CHUNK] = (unsigned short)(b >> 16); o[2 * W4_CHUNK] = (unsigned short)(a >> 16);      // (the smallest first)
-}
-
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 static EncodeTiledFn encode_fn() {
@@ -537,11 +518,7 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   if (!copied && (!x_bf16 || K % 8 || (M > 1 && (ldx % 8 || ldx < K)) || ((uintptr_t)x & 15))) return FELLM_ERR_ARG;
   const int parts = x_bf16 ? 1 : 3;
   if (copied) {
-    if ((uintptr_t)scratch & 15) return FELLM_ERR_ARG;
-    const long long n = (long long)M * chunks * W4_CHUNK, b = (n + 255) / 256;
-    if (b >= (1ll << 31)) return FELLM_ERR_SIZE;
-    if (int e = launch_k_class(launch_class_for_rows(M, 0), w4_rows_kernel, dim3((unsigned)b, 1, 1), dim3(256, 1, 1), 0, stream, 1, x, x_bf16, ldx,
-                               (unsigned short*)scratch, M, K, chunks)) return e;
+    if (int e = w4_copy_rows(x, x_bf16, ldx, scratch, M, K, chunks, stream)) return e;
     x = scratch; ldx = (long long)parts * chunks * W4_CHUNK;
   }
   W4uArgs a = {*w, bias, out, status, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0};

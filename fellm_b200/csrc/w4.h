@@ -83,3 +83,30 @@ static inline int w4_check_epi(int flags, int N) {
   if (epi != W4_STORE && epi != W4_ACC && epi != W4_SWIGLU && epi != W4_RELU2) return FELLM_ERR_ARG;
   return epi == W4_SWIGLU && N % W4_SLAB ? FELLM_ERR_SIZE : 0;
 }
+
+// Rows of x as a product wants them where it cannot read them as they are: bfloat16 rows on no 16-byte boundary or of a K that is no
+// multiple of 8 (copied, zeros up to whole chunks), and float32 rows, every 64 elements of which become three times 64 bfloat16 whose sum
+// they are, the smallest first.
+static __global__ void __launch_bounds__(256) w4_rows_kernel(const void* x, int x_bf16, long long ldx, unsigned short* out, int M, int K, int chunks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int width = chunks * W4_CHUNK;
+  const int m = (int)(i / width), k = (int)(i % width);
+  if (m >= M) return;
+  if (x_bf16) {
+    out[i] = k < K ? ((const unsigned short*)x)[(size_t)m * ldx + k] : (unsigned short)0;
+    return;
+  }
+  unsigned a, b, c;
+  w4_split3(k < K ? ((const float*)x)[(size_t)m * ldx + k] : 0.f, a, b, c);
+  unsigned short* o = out + (size_t)m * 3 * width + (size_t)(k / W4_CHUNK) * 3 * W4_CHUNK + k % W4_CHUNK;
+  o[0] = (unsigned short)(c >> 16); o[W4_CHUNK] = (unsigned short)(b >> 16); o[2 * W4_CHUNK] = (unsigned short)(a >> 16);
+}
+static inline int w4_copy_rows(const void* x, int x_bf16, long long ldx, void* out, int M, int K, int chunks, cudaStream_t stream) {
+  if ((uintptr_t)out & 15) return FELLM_ERR_ARG;
+  const long long blocks = ((long long)M * chunks * W4_CHUNK + 255) / 256;
+  if (blocks >= (1ll << 31)) return FELLM_ERR_SIZE;
+  return launch_k_class(launch_class_for_rows(M, 0), w4_rows_kernel, dim3((unsigned)blocks, 1, 1), dim3(256, 1, 1), 0, stream, 1, x, x_bf16, ldx,
+                        (unsigned short*)out, M, K, chunks);
+}

@@ -1978,6 +1978,7 @@ def interleave_gate_up(gate, up):
 # ------------------------------------------------------------------------------ matrices in four bits
 
 W4_GROUPS = (32, 64, 128)
+W4_CUT_FIRST = 1 << 24                   # elements of a matrix from which float32 rows are cut into bfloat16 ones by a launch of their own
 W4_READ_AHEAD = 32                       # chunks behind the end of a matrix that are there to be read (not used)
 W4_FEW_ROWS = 16                         # up to so many rows: mma.sync, a warp a slab of 16 weight rows; more: tcgen05
 
@@ -2172,16 +2173,19 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
         scratch = None
         if not x_bf16 or K % 8 or ldx % 8 or ldx < K or at % 16:       # (what TMA does not read)
             scratch = torch.empty(M * -(-K // 64) * (64 if x_bf16 else 192), dtype=torch.bfloat16, device=x.device)
-        f = _fn("gemm_w4_umma", "fellm_gemm_w4_umma", _GEMM_W4_ARGS[:-1] + [_c_p, _c_p, _c_p])
+        f = _fn("gemm_w4_umma", "fellm_gemm_w4_umma", _GEMM_W4_ARGS + [_c_p])
         _check(f(at, ldx, w._at, _p(bias), to, ldo, flags, M, _p(scratch), _p(umma_status(x.device)), _stream()), "gemm_w4_umma")
         return out
+    scratch = None
+    if not x_bf16 and N * K >= W4_CUT_FIRST:
+        scratch = torch.empty(M * -(-K // 64) * 192, dtype=torch.bfloat16, device=x.device)
     f = _fn("gemm_w4", "fellm_gemm_w4", _GEMM_W4_ARGS)
-    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), to, ldo, flags, M, _stream()), "gemm_w4")
+    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), to, ldo, flags, M, _p(scratch), _stream()), "gemm_w4")
     return out
 
 
 _W4_X_BF16, _W4_OUT_BF16 = 0x100, 0x200
-_GEMM_W4_ARGS = [_c_p, _c_ll, _c_p, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_p]
+_GEMM_W4_ARGS = [_c_p, _c_ll, _c_p, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_p, _c_p]
 
 
 # ------------------------------------------------------------------------------ attention dispatch

@@ -10,7 +10,7 @@ import w4_util
 
 DEV = "cuda"
 SIZES = [(16, 64, 32), (1, 1, 32), (17, 33, 32), (40, 200, 64), (129, 130, 128), (1003, 1357, 32), (256, 1024, 64), (272, 2056, 128), (2064, 64, 64),
-         (48, 8200, 128), (2100, 200, 32), (4100, 520, 128), (40000, 136, 32)]
+         (48, 8200, 128), (2100, 200, 32), (4100, 520, 128), (40000, 136, 32), (4104, 4104, 64)]
 
 
 def _gen(*seed):
