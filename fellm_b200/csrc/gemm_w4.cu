@@ -22,11 +22,20 @@
 
 enum { X_BF16 = 0, X_BF16_ANY = 1, X_F32 = 2, X_CUT = 3 };       // rows on 16 bytes and K a multiple of 8; any bfloat16; float32; float32 cut by w4_rows_kernel
 
+// An RMSNorm handed on between two products of up to 16 rows.  The one that adds into the rows leaves, beside out += .., next_x[m, n] =
+// bfloat16(out[m, n] next_w[n]) and next_ssq[m * (N / 16) + slab] = the sum of out[m, n]^2 over the slab's 16 columns; the one behind
+// the norm reads such rows as x and multiplies its sums of row m by 1 / sqrt(sum of ssq[m * parts ..] / K + eps) before the bias.
+struct W4Norm {
+  const float* next_w; bf16* next_x; float* next_ssq;
+  const float* ssq; int parts; float eps;
+};
+
 struct GwArgs {
   W4Ref w;
   const void* x; const float* bias; void* out;
   long long ldx, ldo;
   int M, epi, out_bf16;
+  W4Norm norm;
 };
 
 __device__ __forceinline__ void mma_bf16(float* d, const unsigned* a, unsigned b0, unsigned b1) {
@@ -125,8 +134,9 @@ __device__ __forceinline__ Segment next_segment(int slab, int left, int warp, in
 __host__ __device__ constexpr int rows_buffers(int nt) { return nt < 4 ? 2 : 1; }
 
 // XT: what x is.  NT: tiles of eight rows of x.  GS: log2 of the group.  R: neighbouring slabs a warp takes together (a "slab" below is
-// R of them, a unit 4 / R chunks of each): the same columns' operands for both.
-template <int XT, int NT, int GS, int R>
+// R of them, a unit 4 / R chunks of each): the same columns' operands for both.  HANDED: a norm is handed on to it or by it (a kernel of its
+// own: carried by every product, its code cost 4% where it does not run).
+template <int XT, int NT, int GS, int R, bool HANDED>
 __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
   constexpr int UNIT = 4 / R, ROWS = R * W4_SLAB, P = XParts<XT>::N, COLS = 8 * NT, XB = XT == X_F32 ? 4 : 2, XC = W4_CHUNK * XB * (XT == X_CUT ? 3 : 1);      // bytes of an element and of a chunk of x
   extern __shared__ __align__(16) unsigned char smem[];
@@ -172,6 +182,19 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
   for (int i = 0; i < GW_DEPTH - 1; ++i) fetch();          // (weights: nothing in front of this kernel writes them)
   pdl_launch_dependents();
   pdl_wait();
+  // the rows' norm factors: row by row a warp asks for the parts now and sums them behind its first segment
+  constexpr int RS_ROWS = NT == 2 ? 2 : 1;                  // rows a warp (of eight at least; 16 rows at most)
+  __shared__ float row_factor[16];
+  float parts[RS_ROWS][4];
+  if (HANDED && a.norm.ssq) {
+#pragma unroll
+    for (int k = 0; k < RS_ROWS; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = warp + 8 * k, p = lane + 32 * i;
+        parts[k][i] = warp < 8 && m < a.M && p < a.norm.parts ? a.norm.ssq[(size_t)m * a.norm.parts + p] : 0.f;
+      }
+  }
   const unsigned char* xrow[NT];                            // (columns behind the last row repeat it: nobody reads their sums)
 #pragma unroll
   for (int t = 0; t < NT; ++t) xrow[t] = (const unsigned char*)a.x + (size_t)(m0 + min(8 * t + g, cols - 1)) * a.ldx * XB + c * 8 * XB;
@@ -260,7 +283,16 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
         if (8 * t + 2 * c < cols) { p[0] = total[k][t][0]; p[8] = total[k][t][2]; }
         if (8 * t + 2 * c + 1 < cols) { p[ROWS + 1] = total[k][t][1]; p[ROWS + 9] = total[k][t][3]; }
       }
-    if (seg.share == 1) __syncwarp();
+    const bool factors = HANDED && a.norm.ssq && next == first + seg.t;                     // (this was the first segment)
+    if (factors) {
+#pragma unroll
+      for (int k = 0; k < RS_ROWS; ++k) {
+        float sum = (parts[k][0] + parts[k][1]) + (parts[k][2] + parts[k][3]);
+        sum = warp_sum(sum);
+        if (warp < 8 && lane == 0 && warp + 8 * k < 16) row_factor[warp + 8 * k] = 1.0f / sqrtf(sum / (float)a.w.K + a.norm.eps);
+      }
+    }
+    if (seg.share == 1 && !factors) __syncwarp();
     else __syncthreads();
     const int sub = warp & (seg.share - 1);
     for (int i = 32 * sub + lane; i < (R == 2 ? cols : (cols + 1) & ~1) * ROWS; i += 32 * seg.share) {      // (whole warps: one row of x or two)
@@ -268,7 +300,23 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
       const float* p = red + ((size_t)(turn * warps + warp - sub) * COLS + t) * (ROWS + 1) + i % ROWS;
       float v = 0.f;
       for (int w = 0; w < seg.share; ++w) v += p[w * COLS * (ROWS + 1)];
+      if (HANDED && a.norm.ssq) v *= row_factor[t];
       if (a.bias && n < a.w.N) v += a.bias[n];
+      if (HANDED && a.norm.next_x) {                                   // (out += ..; N is a multiple of 16: a half warp is a row's slab)
+        const bool in = t < cols && n < a.w.N;               // (the second slab of a pair may be nobody's)
+        float sum = 0.f;
+        if (in) {
+          const size_t o = (size_t)m * a.ldo + n;
+          v += ((const float*)a.out)[o];
+          ((float*)a.out)[o] = v;
+          a.norm.next_x[(size_t)m * a.w.N + n] = __float2bfloat16_rn(v * a.norm.next_w[n]);
+          sum = v * v;
+        }
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if (in && r == 0) a.norm.next_ssq[(size_t)m * (a.w.N / W4_SLAB) + slab] = sum;
+        continue;
+      }
       if (a.epi == W4_SWIGLU) {
         const float up = __shfl_down_sync(0xffffffffu, v, 8);
         if (r < 8 && t < cols && n < a.w.N) put(a, m, slab * 8 + r, glu_act(v, up, 0.f, 1.f));
@@ -277,10 +325,10 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
   }
 }
 
-template <int XT, int NT, int GS, int R>
+template <int XT, int NT, int GS, int R, bool HANDED>
 static int launch_rows(const GwArgs& a, cudaStream_t stream) {
   const int slabs = ceil_div(ceil_div(a.w.N, W4_SLAB), R), units = ceil_div(a.w.chunks, 4 / R), n_sm = fellm_sm_count(), tiles = ceil_div(a.M, 8 * NT);
-  auto kern = gemm_w4_rows_kernel<XT, NT, GS, R>;
+  auto kern = gemm_w4_rows_kernel<XT, NT, GS, R, HANDED>;
   auto bytes = [](int warps) { return (size_t)warps * (GW_DEPTH * GW_SLOT + rows_buffers(NT) * 8 * NT * (R * W4_SLAB + 1) * 4); };
   static int asked[64];                                 // blocks of eight warps an SM holds, asked once a device
   int dev = 0;
@@ -300,29 +348,39 @@ static int launch_rows(const GwArgs& a, cudaStream_t stream) {
   if (grid.y > 65535) return FELLM_ERR_SIZE;
   return launch_k_class(1, kern, grid, dim3(warps * 32, 1, 1), bytes(warps), stream, 1, a);
 }
-template <int XT, int NT, int R>
+template <int XT, int NT, int R, bool HANDED = false>
 static int launch_rows_group(const GwArgs& a, cudaStream_t stream) {
-  return a.w.gshift == 5 ? launch_rows<XT, NT, 5, R>(a, stream) : a.w.gshift == 6 ? launch_rows<XT, NT, 6, R>(a, stream) : launch_rows<XT, NT, 7, R>(a, stream);
+  return a.w.gshift == 5   ? launch_rows<XT, NT, 5, R, HANDED>(a, stream)
+         : a.w.gshift == 6 ? launch_rows<XT, NT, 6, R, HANDED>(a, stream) : launch_rows<XT, NT, 7, R, HANDED>(a, stream);
+}
+template <bool HANDED>
+static int launch_bf16_rows(const GwArgs& a, cudaStream_t stream) {
+  if (a.M <= 8) return launch_rows_group<X_BF16, 1, 1, HANDED>(a, stream);
+  // (9 to 16 rows: pairs of slabs where every SM gets one, 9,216 x 1,024 4.2 -> 3.8 us; else each for itself, 4,096 x 1,024 3.4 -> 2.8)
+  return a.w.N <= 2 * W4_SLAB * fellm_sm_count() ? launch_rows_group<X_BF16, 2, 1, HANDED>(a, stream) : launch_rows_group<X_BF16, 2, 2, HANDED>(a, stream);
 }
 
 // x [M, K] (x_bf16: bfloat16, else float32), out [M, N] ([M, N/2] for the gated form, whose rows are 8 gate, 8 up, ...).
 // scratch: null, or room for float32 rows cut in three, M x chunks x 192 numbers of bfloat16.
 FELLM_API int fellm_gemm_w4(const void* x, long long ldx, const W4Ref* w, const float* bias, void* out, long long ldo, int flags, int M, void* scratch,
-                            cudaStream_t stream) {
+                            const W4Norm* norm, cudaStream_t stream) {
   if (M <= 0) return 0;
   if (!x || !out) return FELLM_ERR_ARG;
   if (int e = w4_check(w)) return e;
   if (int e = w4_check_epi(flags, w->N)) return e;
-  const int x_bf16 = flags & W4_X_BF16, N = w->N, K = w->K;
-  GwArgs a = {*w, x, bias, out, ldx, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0};
+  if (norm) {
+    if (M > 16 || !(flags & W4_X_BF16)) return FELLM_ERR_SIZE;
+    if (norm->next_x && (!norm->next_w || !norm->next_ssq || (flags & W4_EPI) != W4_ACC || w->N % W4_SLAB || ldo < w->N)) return FELLM_ERR_ARG;
+    if (norm->ssq && (norm->parts < 1 || norm->parts > 128)) return FELLM_ERR_ARG;
+  }
+  const int x_bf16 = flags & W4_X_BF16, K = w->K;
+  GwArgs a = {*w, x, bias, out, ldx, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0, norm ? *norm : W4Norm{}};
   if (!x_bf16 && scratch) {
     if (int e = w4_copy_rows(x, 0, ldx, scratch, M, K, w->chunks, stream)) return e;
     a.x = scratch; a.ldx = 3ll * w->chunks * W4_CHUNK;
     return launch_rows_group<X_CUT, 1, 1>(a, stream);
   }
   if (!x_bf16) return launch_rows_group<X_F32, 1, 1>(a, stream);
-  if (K % 8 || ldx % 8 || ((uintptr_t)x & 15)) return launch_rows_group<X_BF16_ANY, 1, 1>(a, stream);
-  if (M <= 8) return launch_rows_group<X_BF16, 1, 1>(a, stream);
-  // (9 to 16 rows: pairs of slabs where every SM gets one, 9,216 x 1,024 4.2 -> 3.8 us; else each for itself, 4,096 x 1,024 3.4 -> 2.8)
-  return N <= 2 * W4_SLAB * fellm_sm_count() ? launch_rows_group<X_BF16, 2, 1>(a, stream) : launch_rows_group<X_BF16, 2, 2>(a, stream);
+  if (K % 8 || ldx % 8 || ((uintptr_t)x & 15)) return norm ? FELLM_ERR_SIZE : launch_rows_group<X_BF16_ANY, 1, 1>(a, stream);
+  return norm ? launch_bf16_rows<true>(a, stream) : launch_bf16_rows<false>(a, stream);
 }

@@ -1992,6 +1992,11 @@ class _W4Ref(ctypes.Structure):
     _fields_ = [("q", _c_p), ("s", _c_p), ("N", _c_int), ("K", _c_int), ("chunks", _c_int), ("groups", _c_int), ("gshift", _c_int)]
 
 
+class _W4Norm(ctypes.Structure):
+    """csrc/gemm_w4.cu W4Norm: a norm handed on, to the next product and from the one before."""
+    _fields_ = [("next_w", _c_p), ("next_x", _c_p), ("next_ssq", _c_p), ("ssq", _c_p), ("parts", _c_int), ("eps", _c_f)]
+
+
 class W4:
     """A matrix [N, K] in four bits: w[n, k] = level[n, k] * scale[n, k // group], levels -8..7, scales of at most five
     significant bits (level * scale is a bfloat16 number exactly, so every kernel that reads the matrix multiplies with the
@@ -2113,11 +2118,14 @@ def embed_rows_w4(tokens, table: W4, out, status=None, scale: float = 1.0):
     return out
 
 
-def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, swiglu=False, act=None):
+def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, swiglu=False, act=None, row_scale=None):
     """out = x[M, K] @ w[N, K]^T (+ bias), w in four bits, x bfloat16 or float32 (row stride free), float32 sums; the result is
     bfloat16 for bfloat16 x unless out or out_dtype says float32, and float32 for float32 x.
     accumulate: out (float32 [M, N]) += ; swiglu: w's rows are interleaved in blocks of 8 gate / 8 up (interleave_gate_up)
-    and the result [M, N/2] is silu(gate) * up; act="relu2": the result is max(., 0)^2."""
+    and the result [M, N/2] is silu(gate) * up; act="relu2": the result is max(., 0)^2.
+    row_scale=(ssq, parts, eps): x is the pre-weighted input of a handed-on norm (norm_handoff), up to 16 rows; an accumulate product of
+    so few bfloat16 rows hands the norm on that expect_norm() has announced."""
+    global _handoff
     N, K = w.shape
     size = x.shape
     if len(size) != 2 or size[1] != K:
@@ -2162,13 +2170,14 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
     here = w._device
     if here < 0 or x.get_device() != here or out.get_device() != here or torch.cuda.current_device() != here or bias is not None:
         _w4_dev(x, w.q, bias, out)
-    if accumulate:
-        residual_written(out)
+    expected = residual_written(out) if accumulate else None
     if M == 0:
         return out
     at, to = x.data_ptr(), out.data_ptr()
     if at == to:
         raise KernelError("gemm_w4: the result cannot take the place of x")
+    if row_scale is not None and (M > 16 or not x_bf16 or K % 8 or (M > 1 and ldx % 8) or at % 16):
+        raise KernelError(f"a product of {M} x {N} x {K} does not take a handed-on norm")
     if M > W4_FEW_ROWS:
         scratch = None
         if not x_bf16 or K % 8 or ldx % 8 or ldx < K or at % 16:       # (what TMA does not read)
@@ -2179,8 +2188,22 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
     scratch = None
     if not x_bf16 and N * K >= W4_CUT_FIRST:
         scratch = torch.empty(M * -(-K // 64) * 192, dtype=torch.bfloat16, device=x.device)
-    f = _fn("gemm_w4", "fellm_gemm_w4", _GEMM_W4_ARGS)
-    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), to, ldo, flags, M, _p(scratch), _stream()), "gemm_w4")
+    norm = left = None
+    if expected is not None and M <= 16 and N % 16 == 0 and x_bf16 and K % 8 == 0 and (M == 1 or ldx % 8 == 0) and at % 16 == 0 and out.is_contiguous():
+        xg, ssq, _ = _handoff_bufs[out.device]
+        _handoff = None                  # the buffers are about to be rewritten
+        norm = _W4Norm(expected[1].data_ptr(), xg.data_ptr(), ssq.data_ptr())
+        left = NormHandoff()
+        left.x_ptr, left.version, left.rows, left.norm_ptr = to, out._version, M, expected[1].data_ptr()
+        left.xg, left.ssq, left.parts = xg[:M * N].view(M, N), ssq, N // 16
+    if row_scale is not None:
+        norm = norm or _W4Norm()
+        norm.ssq, norm.parts, norm.eps = row_scale[0].data_ptr(), row_scale[1], row_scale[2]
+    f = _fn("gemm_w4", "fellm_gemm_w4", _GEMM_W4_ARGS + [_c_p])
+    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), to, ldo, flags, M, _p(scratch), None if norm is None else ctypes.addressof(norm), _stream()),
+           "gemm_w4")
+    if left is not None:
+        _handoff = left
     return out
 
 

@@ -51,8 +51,11 @@ def linear(x, w, bias=None, *, out=None, out_dtype=None, accumulate=False, swigl
     float32 `out` (the residual stream) instead of storing; swiglu=True: w is the interleaved
     gate/up matrix and the result is SiLU(gate)*up; act="relu2": the result is max(., 0)^2 in x's dtype."""
     if isinstance(w, ops.W4):
-        x = x.tensor() if isinstance(x, LazyNorm) else x
-        return ops.gemm_w4(x, w, bias, out=out, out_dtype=out_dtype, accumulate=accumulate, swiglu=swiglu, act=act)
+        scale = None
+        if isinstance(x, LazyNorm):
+            h = x.handed_on() if x.shape[0] <= 16 and x.shape[1] % 8 == 0 else None
+            x, scale = (x.tensor(), None) if h is None else (h.xg, (h.ssq, h.parts, x.norm.eps))
+        return ops.gemm_w4(x, w, bias, out=out, out_dtype=out_dtype, accumulate=accumulate, swiglu=swiglu, act=act, row_scale=scale)
     if isinstance(x, LazyNorm):
         h = x.handed_on()
         if (h is not None and ops.fast_gemm_takes(h.xg, w) and w.data_ptr() % 16 == 0

@@ -333,3 +333,51 @@ def test_a_matrix_of_zeros_and_rows_of_zeros():
     for M in (1, 9, 40):
         assert (ops.gemm_w4(torch.randn(M, 200, device=DEV).bfloat16(), zero) == 0).all()
         assert (ops.gemm_w4(torch.zeros(M, 200, device=DEV), ops.quantize_w4(torch.randn(40, 200, device=DEV), 64)) == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 3, 8, 9, 16])
+@pytest.mark.parametrize("N,K", [(64, 200), (1024, 1024), (2000, 64), (48, 2048)])
+def test_a_norm_handed_on(M, N, K):
+    """What an accumulate product leaves for the RMSNorm behind it, and the product that reads that."""
+    from fellm_b200 import ops
+    g = _gen(M, N, K)
+    ops.reserve_norm_handoff(DEV, N)
+    levels, scales = w4_util.random_matrix(N, K, 64, g, DEV)
+    w4 = ops.pack_w4(levels, scales, 64)
+    x = torch.randn(M, K, generator=g, device=DEV).bfloat16()
+    stream, weight = torch.randn(M, N, generator=g, device=DEV), torch.rand(N, generator=g, device=DEV) + 0.5
+    plain = stream.clone()
+    ops.gemm_w4(x, w4, out=plain, accumulate=True)
+    ops.forget_norm_handoff()
+    ops.expect_norm(stream, weight)
+    ops.gemm_w4(x, w4, out=stream, accumulate=True)
+    assert torch.equal(stream, plain)
+    h = ops.norm_handoff(stream, weight)
+    assert h is not None and h.parts == N // 16 and h.rows == M
+    assert torch.equal(h.xg, (stream * weight).bfloat16())
+    sums = h.ssq[:M * h.parts].view(M, h.parts).double()
+    want = stream.double().view(M, h.parts, 16).pow(2).sum(-1)
+    assert ((sums - want).abs() <= 20 * 2.0 ** -24 * want).all()         # 16 squares, 15 sums of positive numbers
+    next_levels, next_scales = w4_util.random_matrix(144, N, 64, g, DEV)
+    bias = torch.randn(144, generator=g, device=DEV)
+    w = w4_util.plain_values(next_levels, next_scales, 64)
+    got = ops.gemm_w4(h.xg, ops.pack_w4(next_levels, next_scales, 64), bias, out_dtype=torch.float32, row_scale=(h.ssq, h.parts, 1e-5))
+    factor = 1 / (want.sum(-1, keepdim=True) / N + 1e-5).sqrt()
+    exact = h.xg.double() @ w.T * factor + bias.double()
+    room = 1.25 * N * 2.0 ** -23 * (h.xg.double().abs() @ w.abs().T) * factor + (20 + N / 16) * 2.0 ** -24 * (exact.abs() + bias.double().abs())
+    assert ((got.double() - exact).abs() <= room).all()
+    stream.add_(1)
+    assert ops.norm_handoff(stream, weight) is None
+    ops.forget_norm_handoff()
+
+
+@pytest.mark.gpu
+def test_a_norm_that_is_not_handed_on():
+    from fellm_b200 import ops
+    from fellm_b200.config.errors import KernelError
+    w4 = ops.quantize_w4(torch.randn(64, 64, device=DEV), 32)
+    ssq = torch.ones(64, device=DEV)
+    for x in (torch.zeros(17, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(2, 64, device=DEV), torch.zeros(130, device=DEV, dtype=torch.bfloat16)[1:129].view(2, 64)):
+        with pytest.raises(KernelError, match="handed-on"):
+            ops.gemm_w4(x, w4, row_scale=(ssq, 4, 1e-5))
