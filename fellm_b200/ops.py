@@ -41,6 +41,12 @@ except AttributeError:                                         # pragma: no cove
     _raw_stream = None
 
 
+try:
+    _current_device = torch._C._cuda_getDevice                 # (the context exists where a CUDA tensor does)
+except AttributeError:                                         # pragma: no cover
+    _current_device = torch.cuda.current_device
+
+
 def _stream() -> int:
     if _raw_stream is not None:
         return _raw_stream(torch.cuda.current_device())
@@ -2022,7 +2028,7 @@ class W4:
 def _w4_dev(*tensors):
     """Everything on the current device: its stream is the one that is launched on."""
     _dev(*tensors)
-    here = torch.cuda.current_device()
+    here = _current_device()
     for t in tensors:
         if t is not None and t.get_device() != here:
             raise KernelError(f"a tensor on {t.device}, but the current device is cuda:{here}")
@@ -2168,8 +2174,9 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != N or not bias.is_contiguous()):
         raise KernelError(f"gemm_w4: the bias is contiguous float32 [{N}]")
     here = w._device
-    if here < 0 or x.get_device() != here or out.get_device() != here or torch.cuda.current_device() != here or bias is not None:
+    if here < 0 or x.get_device() != here or out.get_device() != here or _current_device() != here or bias is not None:
         _w4_dev(x, w.q, bias, out)
+    stream = _raw_stream(here) if _raw_stream is not None else _stream()
     expected = residual_written(out) if accumulate else None
     if M == 0:
         return out
@@ -2183,7 +2190,7 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
         if not x_bf16 or K % 8 or ldx % 8 or ldx < K or at % 16:       # (what TMA does not read)
             scratch = torch.empty(M * -(-K // 64) * (64 if x_bf16 else 192), dtype=torch.bfloat16, device=x.device)
         f = _fn("gemm_w4_umma", "fellm_gemm_w4_umma", _GEMM_W4_ARGS + [_c_p])
-        _check(f(at, ldx, w._at, _p(bias), to, ldo, flags, M, _p(scratch), _p(umma_status(x.device)), _stream()), "gemm_w4_umma")
+        _check(f(at, ldx, w._at, _p(bias), to, ldo, flags, M, _p(scratch), _p(umma_status(x.device)), stream), "gemm_w4_umma")
         return out
     scratch = None
     if not x_bf16 and N * K >= W4_CUT_FIRST:
@@ -2200,8 +2207,7 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
         norm = norm or _W4Norm()
         norm.ssq, norm.parts, norm.eps = row_scale[0].data_ptr(), row_scale[1], row_scale[2]
     f = _fn("gemm_w4", "fellm_gemm_w4", _GEMM_W4_ARGS + [_c_p])
-    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), to, ldo, flags, M, _p(scratch), None if norm is None else ctypes.addressof(norm), _stream()),
-           "gemm_w4")
+    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), to, ldo, flags, M, _p(scratch), None if norm is None else ctypes.addressof(norm), stream), "gemm_w4")
     if left is not None:
         _handoff = left
     return out
