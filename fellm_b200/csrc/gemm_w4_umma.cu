@@ -111,7 +111,7 @@ struct W4uArgs {
   W4Ref w;
   const float* bias; void* out; int* status;
   long long ldo;
-  int M, epi, out_bf16;
+  int M;
   int bn;                    // rows of x a tile, a multiple of 16, <= 256
   int stages, splits, tmem_cols;
   int recv_apart;            // what other ranks send lies behind the stages, not over them
@@ -182,18 +182,6 @@ __device__ __forceinline__ void finish16(const W4uArgs& a, float* v, int m, int 
   }
   if (pairs) {
     unsigned char* p = (unsigned char*)a.out + ((size_t)(m + hi) * a.ldo + (n & ~1)) * SIZE;
-    if (EPI == W4_ACC) {
-      float2 old[8];
-      const unsigned char* from = p;
-#pragma unroll
-      for (int j = 0; j < 8; ++j, from += 2 * row) old[j] = in && 2 * j + hi < rows ? *(const float2*)from : make_float2(0.f, 0.f);
-#pragma unroll
-      for (int j = 0; j < 16; j += 2) {                      // what the neighbour will add to this lane's feature belongs to its own sum
-        const float mine = hi ? old[j / 2].y : old[j / 2].x, others = hi ? old[j / 2].x : old[j / 2].y;
-        const float got = __shfl_xor_sync(0xffffffffu, others, 1);
-        v[j] += hi ? got : mine; v[j + 1] += hi ? mine : got;
-      }
-    }
 #pragma unroll
     for (int j = 0; j < 16; j += 2, p += 2 * row) store_pair<BF16>(p, v[j], v[j + 1], hi, in && j + hi < rows);
   } else if (in) {
@@ -208,31 +196,44 @@ __device__ __forceinline__ void finish16(const W4uArgs& a, float* v, int m, int 
     for (int j = 0; j < 16; ++j, p += row) if (j < rows) store1<BF16>(p, EPI == W4_ACC ? v[j] + old[j] : v[j]);
   }
 }
-// Columns c_from .. c_to of a tile (rows of x from m0 + c_from on); take(c, v) fetches 16 of them.
-template <int EPI, bool BF16, class Take>
-__device__ __forceinline__ void finish_columns(const W4uArgs& a, Take take, int c_from, int c_to, int m0, int n) {
+// What out += .. adds to in 16 columns from m on, as store_pair will write it.
+__device__ __forceinline__ void load_old(const W4uArgs& a, float2* old, int m, int rows, int n) {
+  const int hi = threadIdx.x & 1;
+  const float* p = (const float*)a.out + (size_t)(m + hi) * a.ldo + (n & ~1);
+#pragma unroll
+  for (int j = 0; j < 8; ++j, p += 2 * a.ldo) old[j] = n < a.w.N && 2 * j + hi < rows ? *(const float2*)p : make_float2(0.f, 0.f);
+}
+// What the neighbouring lane will store of this lane's feature belongs to its own sum.
+__device__ __forceinline__ void add_old(float* v, const float2* old) {
+  const bool hi = threadIdx.x & 1;
+#pragma unroll
+  for (int j = 0; j < 16; j += 2) {
+    const float mine = hi ? old[j / 2].y : old[j / 2].x, others = hi ? old[j / 2].x : old[j / 2].y;
+    const float got = __shfl_xor_sync(0xffffffffu, others, 1);
+    v[j] += hi ? got : mine; v[j + 1] += hi ? mine : got;
+  }
+}
+// Columns c_from .. c_to of a tile (rows of x from m0 + c_from on): ready() waits for the accumulator, take(c, v) fetches 16 of its columns.
+// What is added to is asked for ahead, the first of it under the MMAs.
+template <int EPI, bool BF16, class Ready, class Take>
+__device__ __forceinline__ void finish_columns(const W4uArgs& a, Ready ready, Take take, int c_from, int c_to, int m0, int n) {
   const float bias = a.bias && n < a.w.N ? a.bias[n] : 0.f;
   const int features = EPI == W4_SWIGLU ? a.w.N / 2 : a.w.N;
-  const bool pairs = !((features | (int)a.ldo) & 1) && ((uintptr_t)a.out & (BF16 ? 3 : 7)) == 0;
-  for (int c = c_from; c < c_to && m0 + c < a.M; c += 16) {
+  const bool pairs = !((features | (int)a.ldo) & 1) && ((uintptr_t)a.out & (BF16 ? 3 : 7)) == 0, ahead = EPI == W4_ACC && pairs;
+  c_to = min(c_to, a.M - m0);
+  float2 old[EPI == W4_ACC ? 8 : 1];
+  if (ahead && c_from < c_to) load_old(a, old, m0 + c_from, a.M - m0 - c_from, n);
+  ready();
+  for (int c = c_from; c < c_to; c += 16) {
     float v[16];
     take(c, v);
+    if (ahead) {
+      add_old(v, old);
+      if (c + 16 < c_to) load_old(a, old, m0 + c + 16, a.M - m0 - c - 16, n);
+    }
     finish16<EPI, BF16>(a, v, m0 + c, a.M - m0 - c, n, bias, pairs);
   }
 }
-template <class Take>
-__device__ __forceinline__ void finish_tile(const W4uArgs& a, Take take, int c_from, int c_to, int m0, int n) {
-  if (a.epi == W4_SWIGLU) {
-    if (a.out_bf16) finish_columns<W4_SWIGLU, true>(a, take, c_from, c_to, m0, n);
-    else finish_columns<W4_SWIGLU, false>(a, take, c_from, c_to, m0, n);
-  } else if (a.epi == W4_ACC) finish_columns<W4_ACC, false>(a, take, c_from, c_to, m0, n);
-  else if (a.epi == W4_RELU2) {
-    if (a.out_bf16) finish_columns<W4_RELU2, true>(a, take, c_from, c_to, m0, n);
-    else finish_columns<W4_RELU2, false>(a, take, c_from, c_to, m0, n);
-  } else if (a.out_bf16) finish_columns<W4_STORE, true>(a, take, c_from, c_to, m0, n);
-  else finish_columns<W4_STORE, false>(a, take, c_from, c_to, m0, n);
-}
-
 // A role's place in the ring of stages, and how often it has been round (its parity).  A role that fills stages waits for the
 // parity before its own: of a new barrier that is complete.
 struct Ring {
@@ -243,7 +244,9 @@ struct Ring {
 
 // KB: chunks of K a stage.  Two where a tile is narrow: one handshake and one commit cost the issuing warp as much as three MMAs of 64
 // columns (377 cycles a stage of one chunk, 40 an MMA).
-template <bool SPLIT, int PARTS, int KB>
+// EPI, BF16: what becomes of the sums, and whether the result is bfloat16 (kernels of their own: with all of them in one, the registers that
+// one wants are spilled by the others, 2,048 rows of a gated 16,384 x 2,048 106 -> 114 us).
+template <bool SPLIT, int PARTS, int KB, int EPI, bool BF16>
 __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
   constexpr int AHEAD = 4 / KB;          // stages whose chunks a warp holds in registers ahead of the one it unpacks
   constexpr unsigned A_BYTES = KB * W4U_A_BYTES;
@@ -391,40 +394,47 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     }
   }
   __syncwarp();
-  if (!SPLIT && warp >= 2 + 8 * SETS) {
+  // The epilogue: the last four warps, a tile behind the MMAs; the CTA's last tile (a cluster's only one) by the sixteen warps that have made
+  // all weights too, a fifth of the columns each four.
+  const bool epi_warp = warp >= 2 + 8 * SETS;
+  const int quarter = warp & 3, row = quarter * 32 + lane, fifth = epi_warp ? 4 : (warp - 2) >> 2;
+  const int last = (total - 1 - first) / step;              // this CTA's last tile
+  if (!SPLIT && warp >= 2) {
     pdl_wait();
-    const int quarter = warp & 3;
-    unsigned use = 0;
-    for (int t = first; t < total; t += step, ++use) {
-      const unsigned acc = use & 1;
-      const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + quarter * 32 + lane;
-      W4U_WAIT_EPILOGUE(accfull0 + 8 * acc, (use >> 1) & 1);
-      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    for (int use = epi_warp ? 0 : last; use <= last; ++use) {
+      const int acc = use & 1, t = first + use * step, groups = a.bn / 16;
+      const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
       const unsigned from = tmem_base + ((unsigned)(quarter * 32) << 16) + acc * acc_cols;
-      finish_tile(a, [&](int c, float* v) { tmem_ld16(from + c, v); }, 0, a.bn, m0, n);
-      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(accempty0 + 8 * acc);
+      finish_columns<EPI, BF16>(a, [&]() {
+        if (epi_warp) W4U_WAIT_EPILOGUE(accfull0 + 8 * acc, (use >> 1) & 1);
+        else W4U_WAIT(accfull0 + 8 * acc, (use >> 1) & 1, 144);
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        __syncwarp();
+      }, [&](int c, float* v) { tmem_ld16(from + c, v); }, use < last ? 0 : groups * fifth / 5 * 16, use < last ? a.bn : groups * (fifth + 1) / 5 * 16, m0, n);
+      if (use < last) {
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(accempty0 + 8 * acc);
+      }
     }
   }
   if (SPLIT) {
     // Every rank sends the other ranks' columns of its sums to them: [sending rank, without the owner][four columns][128 rows][4], so that a
     // warp's store is 512 bytes in a row (16 bytes here and there took ten times as long: they travel one by one).
-    const int quarter = warp & 3, t = first, row = quarter * 32 + lane;
-    const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
+    const int t = first, m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
     const int share = ((a.bn / 16 + a.splits - 1) / a.splits) * 16;               // columns a rank finishes, a multiple of 16
     const unsigned recv = a.recv_apart ? tiles + (unsigned)a.stages * stage_bytes : tiles;
-    const bool epi_warp = warp >= 2 + 8 * SETS;
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");         // every rank has started: its memory is there
-    if (epi_warp) {
+    if (warp >= 2) {
       pdl_wait();
-      W4U_WAIT_EPILOGUE(accfull0, 0);
+      if (epi_warp) W4U_WAIT_EPILOGUE(accfull0, 0);
+      else W4U_WAIT(accfull0, 0, 144);
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     }
     __syncwarp();
     if (!a.recv_apart) cluster_sync();                                            // every rank's MMAs have read their stages
-    if (epi_warp) {
-      for (int c = 0; c < a.bn && m0 + c < a.M; c += 16) {
+    if (warp >= 2) {
+      for (int c = fifth * 16; c < a.bn && m0 + c < a.M; c += 5 * 16) {
         const int owner = c / share;
         if (owner == rank) continue;
         float v[16];
@@ -437,9 +447,10 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     }
     __syncwarp();
     cluster_sync();
-    if (epi_warp) {
+    if (warp >= 2) {
       const float4* mine = reinterpret_cast<const float4*>(smem_raw + (recv - smem_u32(smem_raw))) + row;
-      finish_tile(a, [&](int c, float* v) {
+      const int groups = share / 16, c0 = rank * share;
+      finish_columns<EPI, BF16>(a, []() {}, [&](int c, float* v) {
         float own[16];
         tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, own);
 #pragma unroll
@@ -457,7 +468,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
             }
           }
         }
-      }, rank * share, min(a.bn, (rank + 1) * share), m0, n);
+      }, c0 + groups * fifth / 5 * 16, min(a.bn, c0 + groups * (fifth + 1) / 5 * 16), m0, n);
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -489,7 +500,7 @@ static int clusters_at_once(int splits) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!cache[dev][splits]) {
     const size_t smem = 221 * 1024;
-    auto kern = gemm_w4_umma_kernel<true, 1, 1>;
+    auto kern = gemm_w4_umma_kernel<true, 1, 1, W4_STORE, true>;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess) {
       cudaLaunchConfig_t cfg = {};
@@ -503,6 +514,19 @@ static int clusters_at_once(int splits) {
     cache[dev][splits] = n > 0 ? n : 1;
   }
   return cache[dev][splits];
+}
+
+template <int EPI, bool BF16, int PARTS, int KB>
+static int launch_tiles_of(const CUtensorMap& map, const W4uArgs& a, int grid, size_t smem, cudaStream_t stream) {
+  auto kern = a.splits > 1 ? gemm_w4_umma_kernel<true, PARTS, KB, EPI, BF16> : gemm_w4_umma_kernel<false, PARTS, KB, EPI, BF16>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
+}
+template <int EPI, bool BF16>
+static int launch_tiles(const CUtensorMap& map, const W4uArgs& a, int parts, int kb, int grid, size_t smem, cudaStream_t stream) {
+  if (parts == 3) return BF16 ? FELLM_ERR_ARG : launch_tiles_of<EPI, false, 3, 1>(map, a, grid, smem, stream);      // (float32 rows make float32 results)
+  return kb == 2 ? launch_tiles_of<EPI, BF16, 1, 2>(map, a, grid, smem, stream) : launch_tiles_of<EPI, BF16, 1, 1>(map, a, grid, smem, stream);
 }
 
 // x that TMA cannot read as it is (float32, or rows that are not on 16 bytes) is copied into `scratch` first: M x chunks x 64 numbers of
@@ -521,7 +545,7 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
     if (int e = w4_copy_rows(x, x_bf16, ldx, scratch, M, K, chunks, stream)) return e;
     x = scratch; ldx = (long long)parts * chunks * W4_CHUNK;
   }
-  W4uArgs a = {*w, bias, out, status, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0};
+  W4uArgs a = {*w, bias, out, status, ldo, M};
   const int n_sm = fellm_sm_count(), n_tiles = ceil_div(N, 128);
   // Columns of a tile and CTAs that share its K, by the time of the busiest SM.  A chunk took 0.21 us up to 64 columns and 0.28 at 128,
   // where the issuing warp bounds it, 0.45 at 256, where the MMAs do; a cluster's exchange 1.2 us and what its sums take at some 22 GB/s an SM.
@@ -556,10 +580,11 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   if (r != CUDA_SUCCESS) return 1000 + (int)r;
   const size_t smem = (size_t)a.stages * stage + (a.recv_apart ? recv : 0) + 1024;
   const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
-  auto kern = parts == 3 ? (a.splits > 1 ? gemm_w4_umma_kernel<true, 3, 1> : gemm_w4_umma_kernel<false, 3, 1>)
-            : kb == 2    ? (a.splits > 1 ? gemm_w4_umma_kernel<true, 1, 2> : gemm_w4_umma_kernel<false, 1, 2>)
-                         : (a.splits > 1 ? gemm_w4_umma_kernel<true, 1, 1> : gemm_w4_umma_kernel<false, 1, 1>);
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
-  return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
+  const bool to_bf16 = (flags & W4_OUT_BF16) != 0;
+  switch (flags & W4_EPI) {
+    case W4_ACC: return to_bf16 ? FELLM_ERR_ARG : launch_tiles<W4_ACC, false>(map, a, parts, kb, grid, smem, stream);
+    case W4_SWIGLU: return to_bf16 ? launch_tiles<W4_SWIGLU, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<W4_SWIGLU, false>(map, a, parts, kb, grid, smem, stream);
+    case W4_RELU2: return to_bf16 ? launch_tiles<W4_RELU2, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<W4_RELU2, false>(map, a, parts, kb, grid, smem, stream);
+    default: return to_bf16 ? launch_tiles<W4_STORE, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<W4_STORE, false>(map, a, parts, kb, grid, smem, stream);
+  }
 }
