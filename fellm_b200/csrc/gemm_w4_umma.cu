@@ -40,6 +40,7 @@ __device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity) {
 // here), it records `code` and sets `dead`, and from then on no wait of this CTA waits: all roles run through to the common exit,
 // the same way as ever (so that no role's loop has to carry a verdict; what they store is of no use, and the status word says so).
 __device__ __forceinline__ void wait_slow(unsigned bar, unsigned parity, int* status, int code, volatile int* dead, unsigned nap) {
+  pdl_wait();                                               // (what the kernel in front takes is not counted)
   const long long t0 = clock64();
   for (unsigned i = 0; i < W4U_SPIN_LIMIT; ++i) {
     if (mbar_try(bar, parity) || *dead) return;
@@ -547,15 +548,15 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   }
   W4uArgs a = {*w, bias, out, status, ldo, M};
   const int n_sm = fellm_sm_count(), n_tiles = ceil_div(N, 128);
-  // Columns of a tile and CTAs that share its K, by the time of the busiest SM.  A chunk took 0.21 us up to 64 columns and 0.28 at 128,
-  // where the issuing warp bounds it, 0.45 at 256, where the MMAs do; a cluster's exchange 1.2 us and what its sums take at some 22 GB/s an SM.
+  // Columns of a tile and CTAs that share its K, by the time of the busiest SM.  A chunk took 0.21 us up to 64 columns and 0.29 at 128,
+  // where the issuing warp bounds it, 0.37 at 256, where the MMAs do; a cluster's exchange 1.2 us and what its sums take at some 22 GB/s an SM.
   double least = 1e30;
   int total = 1;
   a.bn = 16; a.splits = 1;
   for (int m_tiles = ceil_div(M, 256), i = 0; i < 8 && m_tiles <= ceil_div(M, 16); ++m_tiles, ++i) {
     const int bn = ceil_div(ceil_div(M, m_tiles), 16) * 16, tiles = n_tiles * ceil_div(M, bn);
     if (m_tiles > 1 && bn < 112) break;                       // (every tile makes its weights again)
-    const double chunk_us = bn <= 64 ? 0.21 : bn <= 128 ? 0.14 + 0.0011 * bn : 0.1 + 0.00137 * bn;
+    const double chunk_us = bn <= 64 ? 0.21 : bn <= 128 ? 0.13 + 0.00122 * bn : 0.2 + 0.00066 * bn;
     for (int s = 1; s <= 8 && (s == 1 || (chunks >= 4 * s && tiles <= clusters_at_once(s))); s *= 2) {
       const double t = ceil_div(tiles * s, n_sm) * (double)ceil_div(chunks, s) * parts * chunk_us + (s > 1 ? 1.2 + bn * 0.0234 * (s - 1) / s : 0.0);
       if (t < least) { least = t; a.bn = bn; a.splits = s; total = tiles; }
@@ -572,7 +573,7 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   EncodeTiledFn fn = encode_fn();
   if (!fn) return FELLM_ERR_ARG;
   CUtensorMap map;
-  cuuint64_t dims[2] = {(cuuint64_t)(copied ? parts * chunks * W4_CHUNK : K), (cuuint64_t)M};
+  cuuint64_t dims[2] = {copied ? (cuuint64_t)parts * chunks * W4_CHUNK : (cuuint64_t)K, (cuuint64_t)M};
   cuuint64_t strides[1] = {(cuuint64_t)(M == 1 && !copied ? (long long)ceil_div(K, 8) * 8 : ldx) * 2};
   cuuint32_t box[2] = {W4_CHUNK, (cuuint32_t)a.bn}, estr[2] = {1, 1};
   const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

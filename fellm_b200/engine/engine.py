@@ -54,6 +54,7 @@ class Engine:
             bind_tensors(self.model, tensors, self.device)
         if options.weights == "int4":
             self.model.quantize(options.weight_group)
+            torch.cuda.empty_cache()               # (the cache is sized by what is free)
         # context: FeLLM clamps n_ctx to the model's maximum, 0 = the maximum (engine.rs:190-197)
         n_ctx = spec.max_position if options.n_ctx == 0 else min(options.n_ctx, spec.max_position)
         if options.ctx_past_model and options.n_ctx > 0:
