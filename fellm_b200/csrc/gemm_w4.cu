@@ -22,14 +22,6 @@
 
 enum { X_BF16 = 0, X_BF16_ANY = 1, X_F32 = 2, X_CUT = 3 };       // rows on 16 bytes and K a multiple of 8; any bfloat16; float32; float32 cut by w4_rows_kernel
 
-// An RMSNorm handed on between two products of up to 16 rows.  The one that adds into the rows leaves, beside out += .., next_x[m, n] =
-// bfloat16(out[m, n] next_w[n]) and next_ssq[m * (N / 16) + slab] = the sum of out[m, n]^2 over the slab's 16 columns; the one behind
-// the norm reads such rows as x and multiplies its sums of row m by 1 / sqrt(sum of ssq[m * parts ..] / K + eps) before the bias.
-struct W4Norm {
-  const float* next_w; bf16* next_x; float* next_ssq;
-  const float* ssq; int parts; float eps;
-};
-
 struct GwArgs {
   W4Ref w;
   const void* x; const float* bias; void* out;
@@ -370,6 +362,7 @@ FELLM_API int fellm_gemm_w4(const void* x, long long ldx, const W4Ref* w, const 
   if (int e = w4_check_epi(flags, w->N)) return e;
   if (norm) {
     if (M > 16 || !(flags & W4_X_BF16)) return FELLM_ERR_SIZE;
+    if (norm->next_x && norm->ssq) return FELLM_ERR_ARG;
     if (norm->next_x && (!norm->next_w || !norm->next_ssq || (flags & W4_EPI) != W4_ACC || w->N % W4_SLAB || ldo < w->N)) return FELLM_ERR_ARG;
     if (norm->ssq && (norm->parts < 1 || norm->parts > 128)) return FELLM_ERR_ARG;
   }

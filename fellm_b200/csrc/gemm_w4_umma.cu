@@ -116,7 +116,9 @@ struct W4uArgs {
   int bn;                    // rows of x a tile, a multiple of 16, <= 256
   int stages, splits, tmem_cols;
   int recv_apart;            // what other ranks send lies behind the stages, not over them
+  W4Norm norm;
 };
+#define W4U_NORM_ROWS 128             // rows of a product that a norm is handed on to or by: one tile's
 
 __device__ __forceinline__ void st_shared_v4(unsigned addr, unsigned a, unsigned b, unsigned c, unsigned d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -214,10 +216,52 @@ __device__ __forceinline__ void add_old(float* v, const float2* old) {
     v[j] += hi ? got : mine; v[j + 1] += hi ? mine : got;
   }
 }
+// 16 finished columns of out += .. (rows of x from m on) as the norm behind them wants them: their squares' sums over the warp's 32 features
+// (each lane keeps half of its columns and gives away the other half, until a pair of lanes has one) and the weighted rows.
+__device__ __forceinline__ void hand_on16(const W4uArgs& a, const float* v, int m, int rows, int n, float weight) {
+  const int lane = threadIdx.x & 31, hi = lane & 1;
+  const bool in = n < a.w.N;
+  float s[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) s[j] = v[j] * v[j];
+#pragma unroll
+  for (int half = 8; half > 0; half >>= 1) {
+    const bool upper = lane & (2 * half);
+#pragma unroll
+    for (int j = 0; j < half; ++j) {
+      const float give = upper ? s[j] : s[j + half], keep = upper ? s[j + half] : s[j];
+      s[j] = keep + __shfl_xor_sync(0xffffffffu, give, 2 * half);
+    }
+  }
+  const float sum = s[0] + __shfl_xor_sync(0xffffffffu, s[0], 1);
+  if (in && !hi && (lane >> 1) < rows) a.norm.next_ssq[(size_t)(m + (lane >> 1)) * (a.w.N / 32) + n / 32] = sum;
+  unsigned char* p = (unsigned char*)(a.norm.next_x + (size_t)(m + hi) * a.w.N + (n & ~1));
+#pragma unroll
+  for (int j = 0; j < 16; j += 2, p += 4 * (size_t)a.w.N) store_pair<true>(p, v[j] * weight, v[j + 1] * weight, hi, in && j + hi < rows);
+}
+// A row's factor by a thread: its parts are a few lines of the second level of cache, all on their way at once.
+__device__ __forceinline__ float row_factor_of(const W4uArgs& a, int m) {
+  const float* p = a.norm.ssq + (size_t)m * a.norm.parts;
+  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+  if (a.norm.parts % 4 == 0) {
+#pragma unroll 8
+    for (int i = 0; i < a.norm.parts; i += 4) {
+      const float4 v = *(const float4*)(p + i);
+      s0 += v.x; s1 += v.y; s2 += v.z; s3 += v.w;
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < a.norm.parts; ++i) s0 += p[i];
+  }
+  return 1.0f / sqrtf(((s0 + s1) + (s2 + s3)) / (float)a.w.K + a.norm.eps);
+}
 // Columns c_from .. c_to of a tile (rows of x from m0 + c_from on): ready() waits for the accumulator, take(c, v) fetches 16 of its columns.
 // What is added to is asked for ahead, the first of it under the MMAs.
-template <int EPI, bool BF16, class Ready, class Take>
-__device__ __forceinline__ void finish_columns(const W4uArgs& a, Ready ready, Take take, int c_from, int c_to, int m0, int n) {
+// HANDED: `factors` are the rows' (a.norm.ssq), or a norm is handed on behind out += ..
+template <int EPI, bool BF16, bool HANDED, class Ready, class Take>
+__device__ __forceinline__ void finish_columns(const W4uArgs& a, const float* factors, Ready ready, Take take, int c_from, int c_to, int m0, int n) {
+  const bool handing = HANDED && EPI == W4_ACC && a.norm.next_x;
+  const float weight = handing && n < a.w.N ? a.norm.next_w[n] : 0.f;
   const float bias = a.bias && n < a.w.N ? a.bias[n] : 0.f;
   const int features = EPI == W4_SWIGLU ? a.w.N / 2 : a.w.N;
   const bool pairs = !((features | (int)a.ldo) & 1) && ((uintptr_t)a.out & (BF16 ? 3 : 7)) == 0, ahead = EPI == W4_ACC && pairs;
@@ -228,11 +272,16 @@ __device__ __forceinline__ void finish_columns(const W4uArgs& a, Ready ready, Ta
   for (int c = c_from; c < c_to; c += 16) {
     float v[16];
     take(c, v);
+    if (HANDED && a.norm.ssq) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] *= factors[m0 + c + j];
+    }
     if (ahead) {
       add_old(v, old);
       if (c + 16 < c_to) load_old(a, old, m0 + c + 16, a.M - m0 - c - 16, n);
     }
     finish16<EPI, BF16>(a, v, m0 + c, a.M - m0 - c, n, bias, pairs);
+    if (handing) hand_on16(a, v, m0 + c, a.M - m0 - c, n, weight);           // (v is what has been stored: pairs, so the old values are in it)
   }
 }
 // A role's place in the ring of stages, and how often it has been round (its parity).  A role that fills stages waits for the
@@ -247,7 +296,8 @@ struct Ring {
 // columns (377 cycles a stage of one chunk, 40 an MMA).
 // EPI, BF16: what becomes of the sums, and whether the result is bfloat16 (kernels of their own: with all of them in one, the registers that
 // one wants are spilled by the others, 2,048 rows of a gated 16,384 x 2,048 106 -> 114 us).
-template <bool SPLIT, int PARTS, int KB, int EPI, bool BF16>
+// HANDED: a norm is handed on to it or by it.
+template <bool SPLIT, int PARTS, int KB, int EPI, bool BF16, bool HANDED>
 __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
   constexpr int AHEAD = 4 / KB;          // stages whose chunks a warp holds in registers ahead of the one it unpacks
   constexpr unsigned A_BYTES = KB * W4U_A_BYTES;
@@ -255,6 +305,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];           // full[8], empty[8], acc_full[2], acc_empty[2]
   __shared__ unsigned tmem_base_s;
   __shared__ int dead;                   // a wait gave up
+  __shared__ float row_factor[HANDED ? W4U_NORM_ROWS : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const unsigned x_bytes = (unsigned)a.bn * 128u, stage_bytes = A_BYTES + KB * x_bytes;
@@ -400,13 +451,22 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   const bool epi_warp = warp >= 2 + 8 * SETS;
   const int quarter = warp & 3, row = quarter * 32 + lane, fifth = epi_warp ? 4 : (warp - 2) >> 2;
   const int last = (total - 1 - first) / step;              // this CTA's last tile
+  if (HANDED && a.norm.ssq && warp >= 2) {
+    if (epi_warp) {                                          // (while the others are at work)
+      pdl_wait();
+      const int m = threadIdx.x - 32 * (2 + 8 * SETS);
+      row_factor[m] = m < a.M ? row_factor_of(a, m) : 0.f;
+      asm volatile("bar.sync 1, 128;\n" ::: "memory");
+      asm volatile("bar.arrive 2, %0;\n" ::"n"(32 * (8 * SETS + 4)) : "memory");
+    } else asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (8 * SETS + 4)) : "memory");
+  }
   if (!SPLIT && warp >= 2) {
     pdl_wait();
     for (int use = epi_warp ? 0 : last; use <= last; ++use) {
       const int acc = use & 1, t = first + use * step, groups = a.bn / 16;
       const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
       const unsigned from = tmem_base + ((unsigned)(quarter * 32) << 16) + acc * acc_cols;
-      finish_columns<EPI, BF16>(a, [&]() {
+      finish_columns<EPI, BF16, HANDED>(a, row_factor, [&]() {
         if (epi_warp) W4U_WAIT_EPILOGUE(accfull0 + 8 * acc, (use >> 1) & 1);
         else W4U_WAIT(accfull0 + 8 * acc, (use >> 1) & 1, 144);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -451,7 +511,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     if (warp >= 2) {
       const float4* mine = reinterpret_cast<const float4*>(smem_raw + (recv - smem_u32(smem_raw))) + row;
       const int groups = share / 16, c0 = rank * share;
-      finish_columns<EPI, BF16>(a, []() {}, [&](int c, float* v) {
+      finish_columns<EPI, BF16, HANDED>(a, row_factor, []() {}, [&](int c, float* v) {
         float own[16];
         tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, own);
 #pragma unroll
@@ -501,7 +561,7 @@ static int clusters_at_once(int splits) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!cache[dev][splits]) {
     const size_t smem = 221 * 1024;
-    auto kern = gemm_w4_umma_kernel<true, 1, 1, W4_STORE, true>;
+    auto kern = gemm_w4_umma_kernel<true, 1, 1, W4_STORE, true, false>;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess) {
       cudaLaunchConfig_t cfg = {};
@@ -517,23 +577,24 @@ static int clusters_at_once(int splits) {
   return cache[dev][splits];
 }
 
-template <int EPI, bool BF16, int PARTS, int KB>
+template <int EPI, bool BF16, int PARTS, int KB, bool HANDED>
 static int launch_tiles_of(const CUtensorMap& map, const W4uArgs& a, int grid, size_t smem, cudaStream_t stream) {
-  auto kern = a.splits > 1 ? gemm_w4_umma_kernel<true, PARTS, KB, EPI, BF16> : gemm_w4_umma_kernel<false, PARTS, KB, EPI, BF16>;
+  auto kern = a.splits > 1 ? gemm_w4_umma_kernel<true, PARTS, KB, EPI, BF16, HANDED> : gemm_w4_umma_kernel<false, PARTS, KB, EPI, BF16, HANDED>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
 }
 template <int EPI, bool BF16>
 static int launch_tiles(const CUtensorMap& map, const W4uArgs& a, int parts, int kb, int grid, size_t smem, cudaStream_t stream) {
-  if (parts == 3) return BF16 ? FELLM_ERR_ARG : launch_tiles_of<EPI, false, 3, 1>(map, a, grid, smem, stream);      // (float32 rows make float32 results)
-  return kb == 2 ? launch_tiles_of<EPI, BF16, 1, 2>(map, a, grid, smem, stream) : launch_tiles_of<EPI, BF16, 1, 1>(map, a, grid, smem, stream);
+  if (parts == 3) return BF16 ? FELLM_ERR_ARG : launch_tiles_of<EPI, false, 3, 1, false>(map, a, grid, smem, stream);      // (float32 rows make float32 results)
+  if (a.norm.next_x || a.norm.ssq) return launch_tiles_of<EPI, BF16, 1, 2, true>(map, a, grid, smem, stream);      // (up to 128 rows)
+  return kb == 2 ? launch_tiles_of<EPI, BF16, 1, 2, false>(map, a, grid, smem, stream) : launch_tiles_of<EPI, BF16, 1, 1, false>(map, a, grid, smem, stream);
 }
 
 // x that TMA cannot read as it is (float32, or rows that are not on 16 bytes) is copied into `scratch` first: M x chunks x 64 numbers of
 // bfloat16, three times as many for float32; scratch null: x is read itself.
 FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, const float* bias, void* out, long long ldo, int flags, int M, void* scratch,
-                                 int* status, cudaStream_t stream) {
+                                 const W4Norm* norm, int* status, cudaStream_t stream) {
   if (M <= 0) return 0;
   if (!x || !out || !status) return FELLM_ERR_ARG;
   if (int e = w4_check(w)) return e;
@@ -542,11 +603,17 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   const bool copied = scratch != nullptr;
   if (!copied && (!x_bf16 || K % 8 || (M > 1 && (ldx % 8 || ldx < K)) || ((uintptr_t)x & 15))) return FELLM_ERR_ARG;
   const int parts = x_bf16 ? 1 : 3;
+  if (norm) {
+    if (copied || M > W4U_NORM_ROWS || (norm->next_x && norm->ssq)) return FELLM_ERR_SIZE;
+    if (norm->next_x && (!norm->next_w || !norm->next_ssq || (flags & W4_EPI) != W4_ACC || N % 32 || ldo < N || ldo % 2 || ((uintptr_t)out & 7))) return FELLM_ERR_ARG;
+    if (norm->ssq && (norm->parts < 1 || norm->parts > 128 || ((uintptr_t)norm->ssq & 15))) return FELLM_ERR_ARG;
+  }
   if (copied) {
     if (int e = w4_copy_rows(x, x_bf16, ldx, scratch, M, K, chunks, stream)) return e;
     x = scratch; ldx = (long long)parts * chunks * W4_CHUNK;
   }
   W4uArgs a = {*w, bias, out, status, ldo, M};
+  a.norm = norm ? *norm : W4Norm{};
   const int n_sm = fellm_sm_count(), n_tiles = ceil_div(N, 128);
   // Columns of a tile and CTAs that share its K, by the time of the busiest SM.  A chunk took 0.21 us up to 64 columns and 0.29 at 128,
   // where the issuing warp bounds it, 0.37 at 256, where the MMAs do; a cluster's exchange 1.2 us and what its sums take at some 22 GB/s an SM.

@@ -32,6 +32,15 @@ struct W4Ref {
   int gshift;                // log2 of the group: 5, 6 or 7
 };
 
+// An RMSNorm handed on between two products.  The one that adds into the rows leaves, beside out += .., next_x[m, n] =
+// bfloat16(out[m, n] next_w[n]) and next_ssq[m * (N / P) + n / P] = the sums of out[m, n]^2 over P columns (a slab's 16 up to 16 rows, a
+// warp's 32 beyond); the one behind the norm reads such rows as x and multiplies its sums of row m by
+// 1 / sqrt(sum of ssq[m * parts ..] / K + eps) before the bias.  A product does one of the two.
+struct W4Norm {
+  const float* next_w; bf16* next_x; float* next_ssq;
+  const float* ssq; int parts; float eps;
+};
+
 // (One three-input operation: written as an and with a constant and an or with another it becomes two.)
 __device__ __forceinline__ unsigned w4_pair_biased(unsigned word, int r) {
   unsigned v;

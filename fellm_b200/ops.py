@@ -1999,7 +1999,7 @@ class _W4Ref(ctypes.Structure):
 
 
 class _W4Norm(ctypes.Structure):
-    """csrc/gemm_w4.cu W4Norm: a norm handed on, to the next product and from the one before."""
+    """csrc/w4.h W4Norm: a norm handed on, to the next product and from the one before."""
     _fields_ = [("next_w", _c_p), ("next_x", _c_p), ("next_ssq", _c_p), ("ssq", _c_p), ("parts", _c_int), ("eps", _c_f)]
 
 
@@ -2129,8 +2129,8 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
     bfloat16 for bfloat16 x unless out or out_dtype says float32, and float32 for float32 x.
     accumulate: out (float32 [M, N]) += ; swiglu: w's rows are interleaved in blocks of 8 gate / 8 up (interleave_gate_up)
     and the result [M, N/2] is silu(gate) * up; act="relu2": the result is max(., 0)^2.
-    row_scale=(ssq, parts, eps): x is the pre-weighted input of a handed-on norm (norm_handoff), up to 16 rows; an accumulate product of
-    so few bfloat16 rows hands the norm on that expect_norm() has announced."""
+    row_scale=(ssq, parts, eps): x is the pre-weighted input of a handed-on norm (norm_handoff), up to HANDOFF_MAX_ROWS rows; an accumulate
+    product of so few bfloat16 rows hands the norm on that expect_norm() has announced."""
     global _handoff
     N, K = w.shape
     size = x.shape
@@ -2183,31 +2183,35 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
     at, to = x.data_ptr(), out.data_ptr()
     if at == to:
         raise KernelError("gemm_w4: the result cannot take the place of x")
-    if row_scale is not None and (M > 16 or not x_bf16 or K % 8 or (M > 1 and ldx % 8) or at % 16):
-        raise KernelError(f"a product of {M} x {N} x {K} does not take a handed-on norm")
+    norm = left = None
+    aligned = x_bf16 and K % 8 == 0 and (M == 1 or (ldx % 8 == 0 and ldx >= K)) and at % 16 == 0
+    if row_scale is not None:
+        if M > HANDOFF_MAX_ROWS or not aligned or row_scale[0].data_ptr() % 16:
+            raise KernelError(f"a product of {M} x {N} x {K} does not take a handed-on norm")
+        norm = _W4Norm(ssq=row_scale[0].data_ptr(), parts=row_scale[1], eps=row_scale[2])
+    elif expected is not None and aligned and N % (part := 16 if M <= W4_FEW_ROWS else 32) == 0 and out.is_contiguous() and to % 8 == 0:
+        xg, ssq, _ = _handoff_bufs[out.device]
+        if at != xg.data_ptr():              # (rows that came with a norm are not written over while they are read)
+            _handoff = None                  # the buffers are about to be rewritten
+            norm = _W4Norm(expected[1].data_ptr(), xg.data_ptr(), ssq.data_ptr())
+            left = NormHandoff()
+            left.x_ptr, left.version, left.rows, left.norm_ptr = to, out._version, M, expected[1].data_ptr()
+            left.xg, left.ssq, left.parts = xg[:M * N].view(M, N), ssq, N // part
+    handed = None if norm is None else ctypes.addressof(norm)
     if M > W4_FEW_ROWS:
         scratch = None
         if not x_bf16 or K % 8 or ldx % 8 or ldx < K or at % 16:       # (what TMA does not read)
             scratch = torch.empty(M * -(-K // 64) * (64 if x_bf16 else 192), dtype=torch.bfloat16, device=x.device)
-        f = _fn("gemm_w4_umma", "fellm_gemm_w4_umma", _GEMM_W4_ARGS + [_c_p])
-        _check(f(at, ldx, w._at, _p(bias), to, ldo, flags, M, _p(scratch), _p(umma_status(x.device)), stream), "gemm_w4_umma")
+        f = _fn("gemm_w4_umma", "fellm_gemm_w4_umma", _GEMM_W4_ARGS + [_c_p, _c_p])
+        _check(f(at, ldx, w._at, _p(bias), to, ldo, flags, M, _p(scratch), handed, _p(umma_status(x.device)), stream), "gemm_w4_umma")
+        if left is not None:
+            _handoff = left
         return out
     scratch = None
     if not x_bf16 and N * K >= W4_CUT_FIRST:
         scratch = torch.empty(M * -(-K // 64) * 192, dtype=torch.bfloat16, device=x.device)
-    norm = left = None
-    if expected is not None and M <= 16 and N % 16 == 0 and x_bf16 and K % 8 == 0 and (M == 1 or ldx % 8 == 0) and at % 16 == 0 and out.is_contiguous():
-        xg, ssq, _ = _handoff_bufs[out.device]
-        _handoff = None                  # the buffers are about to be rewritten
-        norm = _W4Norm(expected[1].data_ptr(), xg.data_ptr(), ssq.data_ptr())
-        left = NormHandoff()
-        left.x_ptr, left.version, left.rows, left.norm_ptr = to, out._version, M, expected[1].data_ptr()
-        left.xg, left.ssq, left.parts = xg[:M * N].view(M, N), ssq, N // 16
-    if row_scale is not None:
-        norm = norm or _W4Norm()
-        norm.ssq, norm.parts, norm.eps = row_scale[0].data_ptr(), row_scale[1], row_scale[2]
     f = _fn("gemm_w4", "fellm_gemm_w4", _GEMM_W4_ARGS + [_c_p])
-    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), to, ldo, flags, M, _p(scratch), None if norm is None else ctypes.addressof(norm), stream), "gemm_w4")
+    _check(f(at, ldx if M > 1 else 0, w._at, _p(bias), to, ldo, flags, M, _p(scratch), handed, stream), "gemm_w4")
     if left is not None:
         _handoff = left
     return out

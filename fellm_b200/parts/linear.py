@@ -53,7 +53,7 @@ def linear(x, w, bias=None, *, out=None, out_dtype=None, accumulate=False, swigl
     if isinstance(w, ops.W4):
         scale = None
         if isinstance(x, LazyNorm):
-            h = x.handed_on() if x.shape[0] <= 16 and x.shape[1] % 8 == 0 else None
+            h = x.handed_on() if x.shape[1] % 8 == 0 else None
             x, scale = (x.tensor(), None) if h is None else (h.xg, (h.ssq, h.parts, x.norm.eps))
         return ops.gemm_w4(x, w, bias, out=out, out_dtype=out_dtype, accumulate=accumulate, swiglu=swiglu, act=act, row_scale=scale)
     if isinstance(x, LazyNorm):

@@ -336,12 +336,12 @@ def test_a_matrix_of_zeros_and_rows_of_zeros():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M", [1, 3, 8, 9, 16])
-@pytest.mark.parametrize("N,K", [(64, 200), (1024, 1024), (2000, 64), (48, 2048)])
+@pytest.mark.parametrize("M,N,K", [(M, N, K) for M in (1, 3, 8, 9, 16) for N, K in ((64, 200), (1024, 1024), (2000, 64), (48, 2048))]
+                         + [(M, N, K) for M in (17, 32, 33, 64, 100, 128) for N, K in ((64, 200), (1024, 1024), (2016, 64), (96, 2048), (2048, 520))])
 def test_a_norm_handed_on(M, N, K):
     """What an accumulate product leaves for the RMSNorm behind it, and the product that reads that."""
     from fellm_b200 import ops
-    g = _gen(M, N, K)
+    g, part = _gen(M, N, K), 16 if M <= 16 else 32
     ops.reserve_norm_handoff(DEV, N)
     levels, scales = w4_util.random_matrix(N, K, 64, g, DEV)
     w4 = ops.pack_w4(levels, scales, 64)
@@ -354,11 +354,11 @@ def test_a_norm_handed_on(M, N, K):
     ops.gemm_w4(x, w4, out=stream, accumulate=True)
     assert torch.equal(stream, plain)
     h = ops.norm_handoff(stream, weight)
-    assert h is not None and h.parts == N // 16 and h.rows == M
+    assert h is not None and h.parts == N // part and h.rows == M
     assert torch.equal(h.xg, (stream * weight).bfloat16())
     sums = h.ssq[:M * h.parts].view(M, h.parts).double()
-    want = stream.double().view(M, h.parts, 16).pow(2).sum(-1)
-    assert ((sums - want).abs() <= 20 * 2.0 ** -24 * want).all()         # 16 squares, 15 sums of positive numbers
+    want = stream.double().view(M, h.parts, part).pow(2).sum(-1)
+    assert ((sums - want).abs() <= 20 * 2.0 ** -24 * want).all()         # squares and sums of positive numbers: 16 roundings one by one, 6 in pairs
     next_levels, next_scales = w4_util.random_matrix(144, N, 64, g, DEV)
     bias = torch.randn(144, generator=g, device=DEV)
     w = w4_util.plain_values(next_levels, next_scales, 64)
@@ -367,6 +367,15 @@ def test_a_norm_handed_on(M, N, K):
     exact = h.xg.double() @ w.T * factor + bias.double()
     room = 1.25 * N * 2.0 ** -23 * (h.xg.double().abs() @ w.abs().T) * factor + (20 + N / 16) * 2.0 ** -24 * (exact.abs() + bias.double().abs())
     assert ((got.double() - exact).abs() <= room).all()
+    gate = w4_util.random_matrix(160, N, 64, g, DEV)
+    w = w4_util.plain_values(*gate, 64)
+    got = ops.gemm_w4(h.xg, ops.pack_w4(*gate, 64), swiglu=True, out_dtype=torch.float32, row_scale=(h.ssq, h.parts, 1e-5)).double()
+    exact = (h.xg.double() @ w.T * factor).view(M, -1, 2, 8)
+    room = (1.25 * N * 2.0 ** -23 * (h.xg.double().abs() @ w.abs().T) * factor).view(M, -1, 2, 8) + (20 + N / 16) * 2.0 ** -24 * exact.abs()
+    silu = exact[:, :, 0] * torch.sigmoid(exact[:, :, 0])
+    # |d silu| <= 1.1 |d gate|; the function itself in float32: some 2^-20 of it
+    room = (1.1 * room[:, :, 0] * (exact[:, :, 1].abs() + room[:, :, 1]) + silu.abs() * room[:, :, 1] + 2.0 ** -20 * (silu * exact[:, :, 1]).abs()).reshape(M, -1)
+    assert ((got - (silu * exact[:, :, 1]).reshape(M, -1)).abs() <= room).all()
     stream.add_(1)
     assert ops.norm_handoff(stream, weight) is None
     ops.forget_norm_handoff()
@@ -377,7 +386,31 @@ def test_a_norm_that_is_not_handed_on():
     from fellm_b200 import ops
     from fellm_b200.config.errors import KernelError
     w4 = ops.quantize_w4(torch.randn(64, 64, device=DEV), 32)
-    ssq = torch.ones(64, device=DEV)
-    for x in (torch.zeros(17, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(2, 64, device=DEV), torch.zeros(130, device=DEV, dtype=torch.bfloat16)[1:129].view(2, 64)):
+    ssq = torch.ones(129 * 4, device=DEV)
+    for x in (torch.zeros(129, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(2, 64, device=DEV), torch.zeros(130, device=DEV, dtype=torch.bfloat16)[1:129].view(2, 64)):
         with pytest.raises(KernelError, match="handed-on"):
             ops.gemm_w4(x, w4, row_scale=(ssq, 4, 1e-5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [4, 40])
+def test_rows_that_came_with_a_norm_are_not_written_over(M):
+    """A product that reads a handed-on norm's rows hands none on: its rows lie where it would write."""
+    from fellm_b200 import ops
+    g = _gen(M, 7)
+    ops.reserve_norm_handoff(DEV, 256)
+    w4 = ops.pack_w4(*w4_util.random_matrix(256, 256, 64, g, DEV), 64)
+    x, weight = torch.randn(M, 256, generator=g, device=DEV).bfloat16(), torch.rand(256, generator=g, device=DEV) + 0.5
+    stream = torch.randn(M, 256, generator=g, device=DEV)
+    ops.forget_norm_handoff()
+    ops.expect_norm(stream, weight)
+    ops.gemm_w4(x, w4, out=stream, accumulate=True)
+    h = ops.norm_handoff(stream, weight)
+    rows = h.xg.clone()
+    other = torch.zeros(M, 256, device=DEV)
+    ops.expect_norm(other, weight)
+    ops.gemm_w4(h.xg, w4, out=other, accumulate=True, row_scale=(h.ssq, h.parts, 1e-5))
+    assert torch.equal(h.xg, rows) and ops.norm_handoff(other, weight) is None and ops.norm_handoff(stream, weight) is h
+    want = ops.gemm_w4(h.xg, w4, out_dtype=torch.float32, row_scale=(h.ssq, h.parts, 1e-5))
+    assert torch.equal(other, want)
+    ops.forget_norm_handoff()
