@@ -486,32 +486,33 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     const int share = ((a.bn / 16 + a.splits - 1) / a.splits) * 16;               // columns a rank finishes, a multiple of 16
     const unsigned recv = a.recv_apart ? tiles + (unsigned)a.stages * stage_bytes : tiles;
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");         // every rank has started: its memory is there
-    if (warp >= 2) {
-      pdl_wait();
-      if (epi_warp) W4U_WAIT_EPILOGUE(accfull0, 0);
-      else W4U_WAIT(accfull0, 0, 144);
-      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-    }
-    __syncwarp();
-    if (!a.recv_apart) cluster_sync();                                            // every rank's MMAs have read their stages
-    if (warp >= 2) {
-      for (int c = fifth * 16; c < a.bn && m0 + c < a.M; c += 5 * 16) {
-        const int owner = c / share;
-        if (owner == rank) continue;
-        float v[16];
-        tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, v);
-        const int from = rank < owner ? rank : rank - 1;
-        const unsigned dst = mapa(recv + (unsigned)((((from * share + c - owner * share) / 4) * 128 + row) * 16), (unsigned)owner);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) st_cluster_v4(dst + j * 2048, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-      }
-    }
-    __syncwarp();
-    cluster_sync();
-    if (warp >= 2) {
+    if (warp < 2) {
+      __syncwarp();
+      if (!a.recv_apart) cluster_sync();
+      cluster_sync();
+    } else {
       const float4* mine = reinterpret_cast<const float4*>(smem_raw + (recv - smem_u32(smem_raw))) + row;
       const int groups = share / 16, c0 = rank * share;
-      finish_columns<EPI, BF16, HANDED>(a, row_factor, []() {}, [&](int c, float* v) {
+      pdl_wait();
+      finish_columns<EPI, BF16, HANDED>(a, row_factor, [&]() {
+        if (epi_warp) W4U_WAIT_EPILOGUE(accfull0, 0);
+        else W4U_WAIT(accfull0, 0, 144);
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        __syncwarp();
+        if (!a.recv_apart) cluster_sync();                                        // every rank's MMAs have read their stages
+        for (int c = fifth * 16; c < a.bn && m0 + c < a.M; c += 5 * 16) {
+          const int owner = c / share;
+          if (owner == rank) continue;
+          float v[16];
+          tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, v);
+          const int from = rank < owner ? rank : rank - 1;
+          const unsigned dst = mapa(recv + (unsigned)((((from * share + c - owner * share) / 4) * 128 + row) * 16), (unsigned)owner);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) st_cluster_v4(dst + j * 2048, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+        __syncwarp();
+        cluster_sync();
+      }, [&](int c, float* v) {
         float own[16];
         tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, own);
 #pragma unroll
