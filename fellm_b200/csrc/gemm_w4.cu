@@ -27,6 +27,7 @@ struct GwArgs {
   const void* x; const float* bias; void* out;
   long long ldx, ldo;
   int M, epi, out_bf16;
+  int per_block, over;       // slabs a block, and how many blocks have one more
   W4Norm norm;
 };
 
@@ -134,7 +135,7 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int all_slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB, slabs = (all_slabs + R - 1) / R, m0 = blockIdx.y * COLS, cols = min(a.M - m0, COLS);
-  const int first = (int)((long long)slabs * blockIdx.x / gridDim.x), end = (int)((long long)slabs * (blockIdx.x + 1) / gridDim.x);
+  const int first = (int)blockIdx.x * a.per_block + min((int)blockIdx.x, a.over), end = first + a.per_block + ((int)blockIdx.x < a.over ? 1 : 0);
   const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * GW_DEPTH * GW_SLOT;
   float* red = reinterpret_cast<float*>(smem + (size_t)warps * GW_DEPTH * GW_SLOT);      // [buffers][warps][COLS][ROWS + 1]
   const int units = (a.w.chunks + UNIT - 1) / UNIT;
@@ -318,7 +319,7 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
 }
 
 template <int XT, int NT, int GS, int R, bool HANDED>
-static int launch_rows(const GwArgs& a, cudaStream_t stream) {
+static int launch_rows(GwArgs a, cudaStream_t stream) {
   const int slabs = ceil_div(ceil_div(a.w.N, W4_SLAB), R), units = ceil_div(a.w.chunks, 4 / R), n_sm = fellm_sm_count(), tiles = ceil_div(a.M, 8 * NT);
   auto kern = gemm_w4_rows_kernel<XT, NT, GS, R, HANDED>;
   auto bytes = [](int warps) { return (size_t)warps * (GW_DEPTH * GW_SLOT + rows_buffers(NT) * 8 * NT * (R * W4_SLAB + 1) * 4); };
@@ -338,6 +339,7 @@ static int launch_rows(const GwArgs& a, cudaStream_t stream) {
   const int warps = slabs <= n_sm && units >= 16 ? 16 : 8, per = warps == 16 ? 1 : resident;
   const dim3 grid(slabs < n_sm * per ? slabs : n_sm * per, tiles, 1);
   if (grid.y > 65535) return FELLM_ERR_SIZE;
+  a.per_block = slabs / (int)grid.x; a.over = slabs % (int)grid.x;
   return launch_k_class(1, kern, grid, dim3(warps * 32, 1, 1), bytes(warps), stream, 1, a);
 }
 template <int XT, int NT, int R, bool HANDED = false>
@@ -367,7 +369,7 @@ FELLM_API int fellm_gemm_w4(const void* x, long long ldx, const W4Ref* w, const 
     if (norm->ssq && (norm->parts < 1 || norm->parts > 128)) return FELLM_ERR_ARG;
   }
   const int x_bf16 = flags & W4_X_BF16, K = w->K;
-  GwArgs a = {*w, x, bias, out, ldx, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0, norm ? *norm : W4Norm{}};
+  GwArgs a = {*w, x, bias, out, ldx, ldo, M, flags & W4_EPI, (flags & W4_OUT_BF16) != 0, 0, 0, norm ? *norm : W4Norm{}};
   if (!x_bf16 && scratch) {
     if (int e = w4_copy_rows(x, 0, ldx, scratch, M, K, w->chunks, stream)) return e;
     a.x = scratch; a.ldx = 3ll * w->chunks * W4_CHUNK;

@@ -94,6 +94,11 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, float* v) {
                  "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
+__device__ __forceinline__ void tmem_ld4(unsigned taddr, float* v) {
+  unsigned* r = reinterpret_cast<unsigned*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+}
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r)); return r; }
 __device__ __forceinline__ unsigned mapa(unsigned addr, unsigned rank) {
   unsigned r;
@@ -114,7 +119,9 @@ struct W4uArgs {
   long long ldo;
   int M;
   int bn;                    // rows of x a tile, a multiple of 16, <= 256
-  int stages, splits, tmem_cols;
+  int m_tiles, total;        // tiles along x, and all of them
+  int stages, splits, log_splits, tmem_cols;
+  int share;                 // columns of a tile that a rank of a cluster finishes, a multiple of 4
   int recv_apart;            // what other ranks send lies behind the stages, not over them
   W4Norm norm;
 };
@@ -144,24 +151,24 @@ template <bool BF16> __device__ __forceinline__ void store1(unsigned char* p, fl
   else *(float*)p = x;
 }
 
-// 16 finished columns (rows of x from m on, `rows` of them count) of weight row n, a warp's lanes neighbouring weight rows.  The
+// COLS finished columns (rows of x from m on, `rows` of them count) of weight row n, a warp's lanes neighbouring weight rows.  The
 // result leaves in pairs of features where they lie on a pair's boundary: neighbouring lanes give each other one of two columns
 // (bfloat16, 2,048 rows, 16,384 x 2,048: 122 us a feature at a time, 104 in pairs).
-template <int EPI, bool BF16>
-__device__ __forceinline__ void finish16(const W4uArgs& a, float* v, int m, int rows, int n, float bias, bool pairs) {
+template <int EPI, bool BF16, int COLS>
+__device__ __forceinline__ void finish_some(const W4uArgs& a, float* v, int m, int rows, int n, float bias, bool pairs) {
   constexpr int SIZE = BF16 ? 2 : 4;
   const int lane = threadIdx.x & 31, hi = lane & 1;
   const bool in = n < a.w.N;
   const size_t row = (size_t)a.ldo * SIZE;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] += bias;
+  for (int j = 0; j < COLS; ++j) v[j] += bias;
   if (EPI == W4_SWIGLU) {
     // lanes 8..15 and 24..31 hold what the eight before them are multiplied with: those take the even columns, these the odd
     const bool gate = !(lane & 8);
     const int f = ((n & ~15) >> 1) + (lane & 7), odd = gate ? 0 : 1;
-    float z[8];
+    float z[COLS / 2];
 #pragma unroll
-    for (int j = 0; j < 16; j += 2) {
+    for (int j = 0; j < COLS; j += 2) {
       const float other = __shfl_xor_sync(0xffffffffu, gate ? v[j + 1] : v[j], 8), g = gate ? v[j] : other, u = gate ? other : v[j + 1];
       z[j >> 1] = BF16 ? silu_mul_fast(g, u) : glu_act(g, u, 0.f, 1.f);
     }
@@ -169,63 +176,63 @@ __device__ __forceinline__ void finish16(const W4uArgs& a, float* v, int m, int 
       const int first = odd + 2 * hi;                        // this lane's column of the first four
       unsigned char* p = (unsigned char*)a.out + ((size_t)(m + first) * a.ldo + (f & ~1)) * SIZE;
 #pragma unroll
-      for (int j = 0; j < 8; j += 2, p += 4 * row) {
+      for (int j = 0; j < COLS / 2; j += 2, p += 4 * row) {
         store_pair<BF16>(p, z[j], z[j + 1], hi, in && 2 * j + first < rows);
       }
     } else if (in) {
       unsigned char* p = (unsigned char*)a.out + ((size_t)(m + odd) * a.ldo + f) * SIZE;
 #pragma unroll
-      for (int j = 0; j < 8; ++j, p += 2 * row) if (2 * j + odd < rows) store1<BF16>(p, z[j]);
+      for (int j = 0; j < COLS / 2; ++j, p += 2 * row) if (2 * j + odd < rows) store1<BF16>(p, z[j]);
     }
     return;
   }
   if (EPI == W4_RELU2) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) { v[j] = fmaxf(v[j], 0.f); v[j] *= v[j]; }
+    for (int j = 0; j < COLS; ++j) { v[j] = fmaxf(v[j], 0.f); v[j] *= v[j]; }
   }
   if (pairs) {
     unsigned char* p = (unsigned char*)a.out + ((size_t)(m + hi) * a.ldo + (n & ~1)) * SIZE;
 #pragma unroll
-    for (int j = 0; j < 16; j += 2, p += 2 * row) store_pair<BF16>(p, v[j], v[j + 1], hi, in && j + hi < rows);
+    for (int j = 0; j < COLS; j += 2, p += 2 * row) store_pair<BF16>(p, v[j], v[j + 1], hi, in && j + hi < rows);
   } else if (in) {
     unsigned char* p = (unsigned char*)a.out + ((size_t)m * a.ldo + n) * SIZE;
-    float old[16];
+    float old[COLS];
     if (EPI == W4_ACC) {
       const unsigned char* from = p;
 #pragma unroll
-      for (int j = 0; j < 16; ++j, from += row) if (j < rows) old[j] = *(const float*)from;
+      for (int j = 0; j < COLS; ++j, from += row) if (j < rows) old[j] = *(const float*)from;
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j, p += row) if (j < rows) store1<BF16>(p, EPI == W4_ACC ? v[j] + old[j] : v[j]);
+    for (int j = 0; j < COLS; ++j, p += row) if (j < rows) store1<BF16>(p, EPI == W4_ACC ? v[j] + old[j] : v[j]);
   }
 }
-// What out += .. adds to in 16 columns from m on, as store_pair will write it.
-__device__ __forceinline__ void load_old(const W4uArgs& a, float2* old, int m, int rows, int n) {
+// What out += .. adds to in COLS columns from m on, as store_pair will write it.
+template <int COLS> __device__ __forceinline__ void load_old(const W4uArgs& a, float2* old, int m, int rows, int n) {
   const int hi = threadIdx.x & 1;
   const float* p = (const float*)a.out + (size_t)(m + hi) * a.ldo + (n & ~1);
 #pragma unroll
-  for (int j = 0; j < 8; ++j, p += 2 * a.ldo) old[j] = n < a.w.N && 2 * j + hi < rows ? *(const float2*)p : make_float2(0.f, 0.f);
+  for (int j = 0; j < COLS / 2; ++j, p += 2 * a.ldo) old[j] = n < a.w.N && 2 * j + hi < rows ? *(const float2*)p : make_float2(0.f, 0.f);
 }
 // What the neighbouring lane will store of this lane's feature belongs to its own sum.
-__device__ __forceinline__ void add_old(float* v, const float2* old) {
+template <int COLS> __device__ __forceinline__ void add_old(float* v, const float2* old) {
   const bool hi = threadIdx.x & 1;
 #pragma unroll
-  for (int j = 0; j < 16; j += 2) {
+  for (int j = 0; j < COLS; j += 2) {
     const float mine = hi ? old[j / 2].y : old[j / 2].x, others = hi ? old[j / 2].x : old[j / 2].y;
     const float got = __shfl_xor_sync(0xffffffffu, others, 1);
     v[j] += hi ? got : mine; v[j + 1] += hi ? mine : got;
   }
 }
-// 16 finished columns of out += .. (rows of x from m on) as the norm behind them wants them: their squares' sums over the warp's 32 features
-// (each lane keeps half of its columns and gives away the other half, until a pair of lanes has one) and the weighted rows.
-__device__ __forceinline__ void hand_on16(const W4uArgs& a, const float* v, int m, int rows, int n, float weight) {
-  const int lane = threadIdx.x & 31, hi = lane & 1;
+// COLS finished columns of out += .. (rows of x from m on) as the norm behind them wants them: their squares' sums over the warp's 32
+// features (a lane keeps half of its columns and gives away the other half, until it has one) and the weighted rows.
+template <int COLS> __device__ __forceinline__ void hand_on(const W4uArgs& a, const float* v, int m, int rows, int n, float weight) {
+  const int lane = threadIdx.x & 31, hi = lane & 1, column = (lane >> 1) & (COLS - 1);
   const bool in = n < a.w.N;
-  float s[16];
+  float s[COLS];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) s[j] = v[j] * v[j];
+  for (int j = 0; j < COLS; ++j) s[j] = v[j] * v[j];
 #pragma unroll
-  for (int half = 8; half > 0; half >>= 1) {
+  for (int half = COLS / 2; half > 0; half >>= 1) {
     const bool upper = lane & (2 * half);
 #pragma unroll
     for (int j = 0; j < half; ++j) {
@@ -233,11 +240,13 @@ __device__ __forceinline__ void hand_on16(const W4uArgs& a, const float* v, int 
       s[j] = keep + __shfl_xor_sync(0xffffffffu, give, 2 * half);
     }
   }
-  const float sum = s[0] + __shfl_xor_sync(0xffffffffu, s[0], 1);
-  if (in && !hi && (lane >> 1) < rows) a.norm.next_ssq[(size_t)(m + (lane >> 1)) * (a.w.N / 32) + n / 32] = sum;
+  float sum = s[0] + __shfl_xor_sync(0xffffffffu, s[0], 1);
+#pragma unroll
+  for (int bit = 2 * COLS; bit < 32; bit *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, bit);
+  if (in && lane == 2 * column && column < rows) a.norm.next_ssq[(size_t)(m + column) * (a.w.N / 32) + n / 32] = sum;
   unsigned char* p = (unsigned char*)(a.norm.next_x + (size_t)(m + hi) * a.w.N + (n & ~1));
 #pragma unroll
-  for (int j = 0; j < 16; j += 2, p += 4 * (size_t)a.w.N) store_pair<true>(p, v[j] * weight, v[j + 1] * weight, hi, in && j + hi < rows);
+  for (int j = 0; j < COLS; j += 2, p += 4 * (size_t)a.w.N) store_pair<true>(p, v[j] * weight, v[j + 1] * weight, hi, in && j + hi < rows);
 }
 // A row's factor by a thread: its parts are a few lines of the second level of cache, all on their way at once.
 __device__ __forceinline__ float row_factor_of(const W4uArgs& a, int m) {
@@ -255,10 +264,10 @@ __device__ __forceinline__ float row_factor_of(const W4uArgs& a, int m) {
   }
   return 1.0f / sqrtf(((s0 + s1) + (s2 + s3)) / (float)a.w.K + a.norm.eps);
 }
-// Columns c_from .. c_to of a tile (rows of x from m0 + c_from on): ready() waits for the accumulator, take(c, v) fetches 16 of its columns.
+// Columns c_from .. c_to of a tile (rows of x from m0 + c_from on): ready() waits for the accumulator, take(c, v) fetches COLS of its columns.
 // What is added to is asked for ahead, the first of it under the MMAs.
 // HANDED: `factors` are the rows' (a.norm.ssq), or a norm is handed on behind out += ..
-template <int EPI, bool BF16, bool HANDED, class Ready, class Take>
+template <int EPI, bool BF16, bool HANDED, int COLS, class Ready, class Take>
 __device__ __forceinline__ void finish_columns(const W4uArgs& a, const float* factors, Ready ready, Take take, int c_from, int c_to, int m0, int n) {
   const bool handing = HANDED && EPI == W4_ACC && a.norm.next_x;
   const float weight = handing && n < a.w.N ? a.norm.next_w[n] : 0.f;
@@ -266,22 +275,22 @@ __device__ __forceinline__ void finish_columns(const W4uArgs& a, const float* fa
   const int features = EPI == W4_SWIGLU ? a.w.N / 2 : a.w.N;
   const bool pairs = !((features | (int)a.ldo) & 1) && ((uintptr_t)a.out & (BF16 ? 3 : 7)) == 0, ahead = EPI == W4_ACC && pairs;
   c_to = min(c_to, a.M - m0);
-  float2 old[EPI == W4_ACC ? 8 : 1];
-  if (ahead && c_from < c_to) load_old(a, old, m0 + c_from, a.M - m0 - c_from, n);
+  float2 old[EPI == W4_ACC ? COLS / 2 : 1];
+  if (ahead && c_from < c_to) load_old<COLS>(a, old, m0 + c_from, a.M - m0 - c_from, n);
   ready();
-  for (int c = c_from; c < c_to; c += 16) {
-    float v[16];
+  for (int c = c_from; c < c_to; c += COLS) {
+    float v[COLS];
     take(c, v);
     if (HANDED && a.norm.ssq) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] *= factors[m0 + c + j];
+      for (int j = 0; j < COLS; ++j) v[j] *= factors[m0 + c + j];
     }
     if (ahead) {
-      add_old(v, old);
-      if (c + 16 < c_to) load_old(a, old, m0 + c + 16, a.M - m0 - c - 16, n);
+      add_old<COLS>(v, old);
+      if (c + COLS < c_to) load_old<COLS>(a, old, m0 + c + COLS, a.M - m0 - c - COLS, n);
     }
-    finish16<EPI, BF16>(a, v, m0 + c, a.M - m0 - c, n, bias, pairs);
-    if (handing) hand_on16(a, v, m0 + c, a.M - m0 - c, n, weight);           // (v is what has been stored: pairs, so the old values are in it)
+    finish_some<EPI, BF16, COLS>(a, v, m0 + c, a.M - m0 - c, n, bias, pairs);
+    if (handing) hand_on<COLS>(a, v, m0 + c, a.M - m0 - c, n, weight);           // (v is what has been stored: pairs, so the old values are in it)
   }
 }
 // A role's place in the ring of stages, and how often it has been round (its parity).  A role that fills stages waits for the
@@ -310,30 +319,35 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   const unsigned tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const unsigned x_bytes = (unsigned)a.bn * 128u, stage_bytes = A_BYTES + KB * x_bytes;
   const unsigned full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[8]), accfull0 = smem_u32(&bars[16]), accempty0 = smem_u32(&bars[18]);
-  const int m_tiles = (a.M + a.bn - 1) / a.bn, n_tiles = (a.w.N + 127) / 128, total = m_tiles * n_tiles;
+  const int m_tiles = a.m_tiles, total = a.total;
   const int rank = SPLIT ? (int)cluster_rank() : 0;
-  const int first = SPLIT ? (int)blockIdx.x / a.splits : (int)blockIdx.x, step = SPLIT ? total : (int)gridDim.x;
+  const int first = (int)blockIdx.x >> (SPLIT ? a.log_splits : 0), step = SPLIT ? total : (int)gridDim.x;
   // this CTA's chunks of K
   const int k_stages = (a.w.chunks + KB - 1) / KB;
-  const int c_lo = SPLIT ? (int)((long long)k_stages * rank / a.splits) * KB : 0, c_hi = SPLIT ? (int)((long long)k_stages * (rank + 1) / a.splits) * KB : k_stages * KB;
+  const int c_lo = SPLIT ? ((k_stages * rank) >> a.log_splits) * KB : 0, c_hi = SPLIT ? ((k_stages * (rank + 1)) >> a.log_splits) * KB : k_stages * KB;
   const int blocks = (c_hi - c_lo) / KB * PARTS;
 
-  if (threadIdx.x == 0) {
+  pdl_launch_dependents();
+  // Barriers and tensor memory are made while the weights' warps ask for their first chunks.
+  auto set_up = [&]() {
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    if (SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");        // (waited for where another rank's memory is written)
+  };
+  if (warp == 0 && lane == 0) {
     dead = 0;
     for (int s = 0; s < a.stages; ++s) { mbar_init(full0 + 8 * s, 1 + 8); mbar_init(empty0 + 8 * s, 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(accfull0 + 8 * b, 1); mbar_init(accempty0 + 8 * b, 4); }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
+  __syncwarp();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_base_s)), "r"(a.tmem_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
-  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-  const unsigned tmem_base = tmem_base_s, acc_cols = SPLIT ? 0u : (unsigned)a.tmem_cols / 2;
-  pdl_launch_dependents();
-  if (SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");        // (waited for where another rank's memory is written)
+  if (warp < 2 || warp >= 2 + 8 * SETS) set_up();
+  const unsigned acc_cols = SPLIT ? 0u : (unsigned)a.tmem_cols / 2;
 
   if (warp == 0) {
     pdl_wait();                                              // x is the output of the kernel before this one
@@ -354,7 +368,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       }
     }
   } else if (warp == 1) {
-    const unsigned idesc = umma_idesc(128, a.bn), a_lo = umma_desc_lo(tiles);
+    const unsigned idesc = umma_idesc(128, a.bn), a_lo = umma_desc_lo(tiles), tmem_base = tmem_base_s;
     unsigned use = 0;
     Ring ring;
     for (int t = first; t < total; t += step, ++use) {
@@ -408,6 +422,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
         for (int i = 0; i < KB; ++i) fetch(u, i);
+      if (t == first) set_up();
       for (int b0 = set; b0 < blocks; b0 += SETS * AHEAD) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
@@ -450,7 +465,8 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   // all weights too, a fifth of the columns each four.
   const bool epi_warp = warp >= 2 + 8 * SETS;
   const int quarter = warp & 3, row = quarter * 32 + lane, fifth = epi_warp ? 4 : (warp - 2) >> 2;
-  const int last = (total - 1 - first) / step;              // this CTA's last tile
+  const unsigned tmem_base = tmem_base_s;
+  const int last = SPLIT ? 0 : (total - 1 - first) / step;              // this CTA's last tile
   if (HANDED && a.norm.ssq && warp >= 2) {
     if (epi_warp) {                                          // (while the others are at work)
       pdl_wait();
@@ -466,7 +482,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       const int acc = use & 1, t = first + use * step, groups = a.bn / 16;
       const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
       const unsigned from = tmem_base + ((unsigned)(quarter * 32) << 16) + acc * acc_cols;
-      finish_columns<EPI, BF16, HANDED>(a, row_factor, [&]() {
+      finish_columns<EPI, BF16, HANDED, 16>(a, row_factor, [&]() {
         if (epi_warp) W4U_WAIT_EPILOGUE(accfull0 + 8 * acc, (use >> 1) & 1);
         else W4U_WAIT(accfull0 + 8 * acc, (use >> 1) & 1, 144);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -480,10 +496,10 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     }
   }
   if (SPLIT) {
-    // Every rank sends the other ranks' columns of its sums to them: [sending rank, without the owner][four columns][128 rows][4], so that a
+    // Every rank sends the other ranks' columns of its sums to them: [sending rank, without the owner][its groups of four columns][128 rows][4], so that a
     // warp's store is 512 bytes in a row (16 bytes here and there took ten times as long: they travel one by one).
     const int t = first, m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
-    const int share = ((a.bn / 16 + a.splits - 1) / a.splits) * 16;               // columns a rank finishes, a multiple of 16
+    const int share = a.share, groups = share / 4, c0 = rank * share;
     const unsigned recv = a.recv_apart ? tiles + (unsigned)a.stages * stage_bytes : tiles;
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");         // every rank has started: its memory is there
     if (warp < 2) {
@@ -492,45 +508,38 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       cluster_sync();
     } else {
       const float4* mine = reinterpret_cast<const float4*>(smem_raw + (recv - smem_u32(smem_raw))) + row;
-      const int groups = share / 16, c0 = rank * share;
       pdl_wait();
-      finish_columns<EPI, BF16, HANDED>(a, row_factor, [&]() {
+      finish_columns<EPI, BF16, HANDED, 4>(a, row_factor, [&]() {
         if (epi_warp) W4U_WAIT_EPILOGUE(accfull0, 0);
         else W4U_WAIT(accfull0, 0, 144);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         __syncwarp();
         if (!a.recv_apart) cluster_sync();                                        // every rank's MMAs have read their stages
         for (int c = fifth * 16; c < a.bn && m0 + c < a.M; c += 5 * 16) {
-          const int owner = c / share;
-          if (owner == rank) continue;
           float v[16];
           tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, v);
-          const int from = rank < owner ? rank : rank - 1;
-          const unsigned dst = mapa(recv + (unsigned)((((from * share + c - owner * share) / 4) * 128 + row) * 16), (unsigned)owner);
+          int owner = (c >> 2) / groups, group = (c >> 2) - owner * groups;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) st_cluster_v4(dst + j * 2048, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          for (int j = 0; j < 4; ++j) {
+            if (owner != rank && m0 + c + 4 * j < a.M)
+              st_cluster_v4(mapa(recv + (unsigned)((((rank < owner ? rank : rank - 1) * groups + group) * 128 + row) * 16), (unsigned)owner), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            if (++group == groups) { group = 0; ++owner; }
+          }
         }
         __syncwarp();
         cluster_sync();
       }, [&](int c, float* v) {
-        float own[16];
-        tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, own);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = 0.f;
-        for (int r = 0; r < a.splits; ++r) {
-          if (r == rank) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] += own[j];
-          } else {
-            const float4* part = mine + (((r < rank ? r : r - 1) * share + c - rank * share) / 4) * 128;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float4 x = part[j * 128];
-              v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
-            }
-          }
+        float own[4];
+        tmem_ld4(tmem_base + ((unsigned)(quarter * 32) << 16) + c, own);
+        const float4* part = mine + (c - c0) / 4 * 128;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < a.splits; ++r) {                 // (in the ranks' order)
+          const float4 x = r == rank ? make_float4(own[0], own[1], own[2], own[3]) : *part;
+          if (r != rank) part += groups * 128;
+          sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
         }
-      }, c0 + groups * fifth / 5 * 16, min(a.bn, c0 + groups * (fifth + 1) / 5 * 16), m0, n);
+        v[0] = sum.x; v[1] = sum.y; v[2] = sum.z; v[3] = sum.w;
+      }, c0 + groups * fifth / 5 * 4, min(a.bn, c0 + groups * (fifth + 1) / 5 * 4), m0, n);
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -620,18 +629,22 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   // where the issuing warp bounds it, 0.37 at 256, where the MMAs do; a cluster's exchange 1.2 us and what its sums take at some 22 GB/s an SM.
   double least = 1e30;
   int total = 1;
-  a.bn = 16; a.splits = 1;
+  a.bn = 16; a.splits = 1; a.log_splits = 0;
   for (int m_tiles = ceil_div(M, 256), i = 0; i < 8 && m_tiles <= ceil_div(M, 16); ++m_tiles, ++i) {
     const int bn = ceil_div(ceil_div(M, m_tiles), 16) * 16, tiles = n_tiles * ceil_div(M, bn);
     if (m_tiles > 1 && bn < 112) break;                       // (every tile makes its weights again)
     const double chunk_us = bn <= 64 ? 0.21 : bn <= 128 ? 0.13 + 0.00122 * bn : 0.2 + 0.00066 * bn;
-    for (int s = 1; s <= 8 && (s == 1 || (chunks >= 4 * s && tiles <= clusters_at_once(s))); s *= 2) {
+    for (int ls = 0; ls <= 3; ++ls) {
+      const int s = 1 << ls;
+      if (s > 1 && (chunks < 4 * s || tiles > clusters_at_once(s))) break;
       const double t = ceil_div(tiles * s, n_sm) * (double)ceil_div(chunks, s) * parts * chunk_us + (s > 1 ? 1.2 + bn * 0.0234 * (s - 1) / s : 0.0);
-      if (t < least) { least = t; a.bn = bn; a.splits = s; total = tiles; }
+      if (t < least) { least = t; a.bn = bn; a.splits = s; a.log_splits = ls; total = tiles; }
     }
   }
+  a.m_tiles = ceil_div(M, a.bn); a.total = total;
   const int kb = parts == 1 && a.bn <= 128 ? 2 : 1, stage = kb * (W4U_A_BYTES + a.bn * 128), room = 220 * 1024;
-  const int share = ceil_div(a.bn / 16, a.splits) * 16, recv = (a.splits - 1) * share * 512;
+  a.share = ceil_div(a.bn / 4, a.splits) * 4;
+  const int recv = (a.splits - 1) * a.share * 512;
   a.stages = room / stage < 8 ? room / stage : 8;
   a.recv_apart = (room - recv) / stage >= 3;
   if (a.recv_apart && (room - recv) / stage < a.stages) a.stages = (room - recv) / stage;
