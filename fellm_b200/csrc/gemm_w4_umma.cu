@@ -99,6 +99,34 @@ __device__ __forceinline__ void tmem_ld4(unsigned taddr, float* v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
+// 16 columns += 16 others (one wait for both; tmem_st_wait() behind the last of them).
+__device__ __forceinline__ void tmem_add16(unsigned to, unsigned from) {
+  unsigned r[16], f[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n"
+               "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n"
+               "tcgen05.wait::ld.sync.aligned;\n"
+               : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]), "=&r"(r[4]), "=&r"(r[5]), "=&r"(r[6]), "=&r"(r[7]), "=&r"(r[8]), "=&r"(r[9]), "=&r"(r[10]),
+                 "=&r"(r[11]), "=&r"(r[12]), "=&r"(r[13]), "=&r"(r[14]), "=&r"(r[15]), "=&r"(f[0]), "=&r"(f[1]), "=&r"(f[2]), "=&r"(f[3]), "=&r"(f[4]), "=&r"(f[5]),
+                 "=&r"(f[6]), "=&r"(f[7]), "=&r"(f[8]), "=&r"(f[9]), "=&r"(f[10]), "=&r"(f[11]), "=&r"(f[12]), "=&r"(f[13]), "=&r"(f[14]), "=&r"(f[15])
+               : "r"(to), "r"(from) : "memory");
+#pragma unroll
+  for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(f[j]));
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n"
+               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(to) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+// N columns of a tile's sums, the sums of two accumulators `lo` columns apart (0: of one).
+template <int N> __device__ __forceinline__ void tmem_sums(unsigned at, unsigned lo, float* v) {
+  if (N == 16) tmem_ld16(at, v);
+  else tmem_ld4(at, v);
+  if (!lo) return;
+  float more[N];
+  if (N == 16) tmem_ld16(at + lo, more);
+  else tmem_ld4(at + lo, more);
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] += more[j];
+}
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r)); return r; }
 __device__ __forceinline__ unsigned mapa(unsigned addr, unsigned rank) {
   unsigned r;
@@ -121,10 +149,18 @@ struct W4uArgs {
   int bn;                    // rows of x a tile, a multiple of 16, <= 256
   int m_tiles, total;        // tiles along x, and all of them
   int stages, splits, log_splits, tmem_cols;
+  int run;                   // blocks of K that are summed in one accumulator
+  int buffers, acc_cols;     // accumulators (used in turn), columns of tensor memory from one to the next
   int share;                 // columns of a tile that a rank of a cluster finishes, a multiple of 4
   int recv_apart;            // what other ranks send lies behind the stages, not over them
   W4Norm norm;
 };
+// The tensor cores cut a sum's last bits off where they add to it, always towards zero: float32 results of bfloat16 rows were off by 8e-8 of
+// themselves over 512 k, 1.8e-7 over 1,024, 4.1e-7 over 2,048, 1.0e-6 over 4,096, 2.4e-6 over 8,192, and those of float32 rows by as much again
+// for each of their small pieces' products.  So a float32 result's K is summed in runs of up to 48 chunks, which float32
+// additions put together, and the two small pieces of float32 rows have an accumulator of their own.  (bfloat16 results are rounded
+// to 2e-3 behind it.)
+#define W4U_RUN 48
 #define W4U_NORM_ROWS 128             // rows of a product that a norm is handed on to or by: one tile's
 
 __device__ __forceinline__ void st_shared_v4(unsigned addr, unsigned a, unsigned b, unsigned c, unsigned d) {
@@ -347,7 +383,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   if (warp < 2 || warp >= 2 + 8 * SETS) set_up();
-  const unsigned acc_cols = SPLIT ? 0u : (unsigned)a.tmem_cols / 2;
+  const unsigned acc_cols = a.acc_cols, lo_cols = PARTS == 3 ? acc_cols / 2 : 0u;
 
   if (warp == 0) {
     pdl_wait();                                              // x is the output of the kernel before this one
@@ -371,22 +407,27 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     const unsigned idesc = umma_idesc(128, a.bn), a_lo = umma_desc_lo(tiles), tmem_base = tmem_base_s;
     unsigned use = 0;
     Ring ring;
-    for (int t = first; t < total; t += step, ++use) {
-      const unsigned acc = use & 1, d = tmem_base + acc * acc_cols;
-      if (use >= 2) W4U_WAIT(accempty0 + 8 * acc, ((use >> 1) - 1) & 1, 145);
-      for (int b = 0; b < blocks; ++b) {
-        const unsigned lo = a_lo + ring.stage * (stage_bytes >> 4), empty = empty0 + 8 * ring.stage;
-        W4U_WAIT(full0 + 8 * ring.stage, ring.parity, 142);
-        __syncwarp();
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        if (elect_one()) {
+    for (int t = first; t < total; t += step) {
+      for (int b0 = 0; b0 < blocks; b0 += a.run, ++use) {
+        const unsigned acc = a.buffers == 2 ? use & 1 : 0u, round = a.buffers == 2 ? use >> 1 : use, d = tmem_base + acc * acc_cols;
+        if (round) W4U_WAIT(accempty0 + 8 * acc, (round - 1) & 1, 145);
+        const int run = min(blocks - b0, a.run);
+        int part = 0;
+        for (int b = 0; b < run; ++b) {
+          const unsigned lo = a_lo + ring.stage * (stage_bytes >> 4), empty = empty0 + 8 * ring.stage, to = PARTS == 3 && part < 2 ? d + lo_cols : d;
+          W4U_WAIT(full0 + 8 * ring.stage, ring.parity, 142);
+          __syncwarp();
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < KB; ++i)
-            umma_stage(d, lo + i * (W4U_A_BYTES >> 4), lo + (A_BYTES >> 4) + i * (x_bytes >> 4), idesc, (b | i) ? 1u : 0u);
-          umma_commit(empty);
-          if (b == blocks - 1) umma_commit(accfull0 + 8 * acc);
+            for (int i = 0; i < KB; ++i)
+              umma_stage(to, lo + i * (W4U_A_BYTES >> 4), lo + (A_BYTES >> 4) + i * (x_bytes >> 4), idesc, (b | i) && !(PARTS == 3 && b == 2) ? 1u : 0u);
+            umma_commit(empty);
+            if (b == run - 1) umma_commit(accfull0 + 8 * acc);
+          }
+          if (PARTS == 3) part = part == 2 ? 0 : part + 1;
+          ring.add(1, a.stages);
         }
-        ring.add(1, a.stages);
       }
     }
   } else if (warp < 2 + 8 * SETS) {
@@ -465,33 +506,58 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   // all weights too, a fifth of the columns each four.
   const bool epi_warp = warp >= 2 + 8 * SETS;
   const int quarter = warp & 3, row = quarter * 32 + lane, fifth = epi_warp ? 4 : (warp - 2) >> 2;
-  const unsigned tmem_base = tmem_base_s;
-  const int last = SPLIT ? 0 : (total - 1 - first) / step;              // this CTA's last tile
-  if (HANDED && a.norm.ssq && warp >= 2) {
-    if (epi_warp) {                                          // (while the others are at work)
-      pdl_wait();
-      const int m = threadIdx.x - 32 * (2 + 8 * SETS);
-      row_factor[m] = m < a.M ? row_factor_of(a, m) : 0.f;
-      asm volatile("bar.sync 1, 128;\n" ::: "memory");
-      asm volatile("bar.arrive 2, %0;\n" ::"n"(32 * (8 * SETS + 4)) : "memory");
-    } else asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (8 * SETS + 4)) : "memory");
-  }
-  if (!SPLIT && warp >= 2) {
+  const unsigned tmem_base = tmem_base_s, quarter_base = tmem_base + ((unsigned)(quarter * 32) << 16);
+  const int last = SPLIT ? 0 : (total - 1 - first) / step;  // this CTA's last tile
+  const int runs = BF16 || blocks <= a.run ? 1 : (blocks + a.run - 1) / a.run;              // accumulators a tile goes through
+  if (HANDED && a.norm.ssq && epi_warp) {                    // (while the others are at work; they see it behind a barrier below)
     pdl_wait();
-    for (int use = epi_warp ? 0 : last; use <= last; ++use) {
-      const int acc = use & 1, t = first + use * step, groups = a.bn / 16;
-      const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
-      const unsigned from = tmem_base + ((unsigned)(quarter * 32) << 16) + acc * acc_cols;
-      finish_columns<EPI, BF16, HANDED, 16>(a, row_factor, [&]() {
-        if (epi_warp) W4U_WAIT_EPILOGUE(accfull0 + 8 * acc, (use >> 1) & 1);
-        else W4U_WAIT(accfull0 + 8 * acc, (use >> 1) & 1, 144);
+    const int m = threadIdx.x - 32 * (2 + 8 * SETS);
+    row_factor[m] = m < a.M ? row_factor_of(a, m) : 0.f;
+  }
+  auto where = [&](int use) { return quarter_base + (a.buffers == 2 ? (unsigned)(use & 1) * acc_cols : 0u); };
+  auto release = [&](int use) {
+    if (lane == 0) mbar_arrive(accempty0 + (a.buffers == 2 ? 8 * (use & 1) : 0));
+  };
+  // A tile's sums: the epilogue's warps wait for each of its runs and add the one before to it, whose accumulator is free then.  The other
+  // warps go on when those have seen the last run (they are not there for every phase of its barrier).
+  auto tile_ready = [&](int tile, bool everyone) {
+    if (epi_warp) {
+      for (int r = 0; r < runs; ++r) {
+        const int use = tile * runs + r;
+        W4U_WAIT_EPILOGUE(accfull0 + (a.buffers == 2 ? 8 * (use & 1) : 0), (a.buffers == 2 ? use >> 1 : use) & 1);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         __syncwarp();
-      }, [&](int c, float* v) { tmem_ld16(from + c, v); }, use < last ? 0 : groups * fifth / 5 * 16, use < last ? a.bn : groups * (fifth + 1) / 5 * 16, m0, n);
-      if (use < last) {
+        if (!BF16 && r > 0) {
+          for (int c = 0; c < a.bn; c += 16) {
+            tmem_add16(where(use) + c, where(use - 1) + c);
+            if (PARTS == 3) tmem_add16(where(use) + lo_cols + c, where(use - 1) + lo_cols + c);
+          }
+          tmem_st_wait();
+          asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+          __syncwarp();
+          release(use - 1);
+        }
+      }
+      if (everyone) {
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        asm volatile("bar.arrive 2, %0;\n" ::"n"(32 * (8 * SETS + 4)) : "memory");
+      }
+    } else asm volatile("bar.sync 2, %0;\n" ::"n"(32 * (8 * SETS + 4)) : "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    __syncwarp();
+  };
+  if (!SPLIT && warp >= 2) {
+    pdl_wait();
+    for (int tile = epi_warp ? 0 : last; tile <= last; ++tile) {
+      const int t = first + tile * step, use = tile * runs + runs - 1, groups = a.bn / 16;
+      const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
+      const unsigned from = where(use);
+      finish_columns<EPI, BF16, HANDED, 16>(a, row_factor, [&]() { tile_ready(tile, tile == last); }, [&](int c, float* v) { tmem_sums<16>(from + c, lo_cols, v); },
+                                            tile < last ? 0 : groups * fifth / 5 * 16, tile < last ? a.bn : groups * (fifth + 1) / 5 * 16, m0, n);
+      if (tile < last) {
         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(accempty0 + 8 * acc);
+        release(use);
       }
     }
   }
@@ -500,6 +566,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     // warp's store is 512 bytes in a row (16 bytes here and there took ten times as long: they travel one by one).
     const int t = first, m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
     const int share = a.share, groups = share / 4, c0 = rank * share;
+    const unsigned from = where(runs - 1);
     const unsigned recv = a.recv_apart ? tiles + (unsigned)a.stages * stage_bytes : tiles;
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");         // every rank has started: its memory is there
     if (warp < 2) {
@@ -510,14 +577,11 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       const float4* mine = reinterpret_cast<const float4*>(smem_raw + (recv - smem_u32(smem_raw))) + row;
       pdl_wait();
       finish_columns<EPI, BF16, HANDED, 4>(a, row_factor, [&]() {
-        if (epi_warp) W4U_WAIT_EPILOGUE(accfull0, 0);
-        else W4U_WAIT(accfull0, 0, 144);
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        __syncwarp();
+        tile_ready(0, true);
         if (!a.recv_apart) cluster_sync();                                        // every rank's MMAs have read their stages
         for (int c = fifth * 16; c < a.bn && m0 + c < a.M; c += 5 * 16) {
           float v[16];
-          tmem_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + c, v);
+          tmem_sums<16>(from + c, lo_cols, v);
           int owner = (c >> 2) / groups, group = (c >> 2) - owner * groups;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -530,7 +594,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         cluster_sync();
       }, [&](int c, float* v) {
         float own[4];
-        tmem_ld4(tmem_base + ((unsigned)(quarter * 32) << 16) + c, own);
+        tmem_sums<4>(from + c, lo_cols, own);
         const float4* part = mine + (c - c0) / 4 * 128;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int r = 0; r < a.splits; ++r) {                 // (in the ranks' order)
@@ -625,14 +689,16 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   W4uArgs a = {*w, bias, out, status, ldo, M};
   a.norm = norm ? *norm : W4Norm{};
   const int n_sm = fellm_sm_count(), n_tiles = ceil_div(N, 128);
+  const bool to_bf16 = (flags & W4_OUT_BF16) != 0;
+  const int most = parts == 3 && chunks > W4U_RUN ? 128 : 256;          // (columns of a tile: tensor memory holds what its sums need)
   // Columns of a tile and CTAs that share its K, by the time of the busiest SM.  A chunk took 0.21 us up to 64 columns and 0.29 at 128,
   // where the issuing warp bounds it, 0.37 at 256, where the MMAs do; a cluster's exchange 1.2 us and what its sums take at some 22 GB/s an SM.
   double least = 1e30;
   int total = 1;
   a.bn = 16; a.splits = 1; a.log_splits = 0;
-  for (int m_tiles = ceil_div(M, 256), i = 0; i < 8 && m_tiles <= ceil_div(M, 16); ++m_tiles, ++i) {
+  for (int m_tiles = ceil_div(M, most), i = 0; i < 8 && m_tiles <= ceil_div(M, 16); ++m_tiles, ++i) {
     const int bn = ceil_div(ceil_div(M, m_tiles), 16) * 16, tiles = n_tiles * ceil_div(M, bn);
-    if (m_tiles > 1 && bn < 112) break;                       // (every tile makes its weights again)
+    if (i > 0 && bn < 112) break;                       // (every tile makes its weights again)
     const double chunk_us = bn <= 64 ? 0.21 : bn <= 128 ? 0.13 + 0.00122 * bn : 0.2 + 0.00066 * bn;
     for (int ls = 0; ls <= 3; ++ls) {
       const int s = 1 << ls;
@@ -648,8 +714,15 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   a.stages = room / stage < 8 ? room / stage : 8;
   a.recv_apart = (room - recv) / stage >= 3;
   if (a.recv_apart && (room - recv) / stage < a.stages) a.stages = (room - recv) / stage;
-  a.tmem_cols = 32;
-  while (a.tmem_cols < (a.splits > 1 ? 1 : 2) * a.bn) a.tmem_cols *= 2;
+  const int blocks = ceil_div(ceil_div(chunks, kb), a.splits) * parts;
+  const int runs = to_bf16 ? 1 : ceil_div(blocks, W4U_RUN / kb * parts);
+  a.run = ceil_div(blocks / parts, runs) * parts;
+  a.acc_cols = 16;
+  while (a.acc_cols < a.bn) a.acc_cols *= 2;
+  if (parts == 3) a.acc_cols *= 2;
+  a.buffers = (a.splits == 1 || runs > 1) && 2 * a.acc_cols <= 512 ? 2 : 1;
+  if (runs > 1 && a.buffers < 2) return FELLM_ERR_SIZE;
+  a.tmem_cols = a.buffers * a.acc_cols < 32 ? 32 : a.buffers * a.acc_cols;
   if (!a.recv_apart && recv > a.stages * stage) return FELLM_ERR_SIZE;
   EncodeTiledFn fn = encode_fn();
   if (!fn) return FELLM_ERR_ARG;
@@ -662,7 +735,6 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   if (r != CUDA_SUCCESS) return 1000 + (int)r;
   const size_t smem = (size_t)a.stages * stage + (a.recv_apart ? recv : 0) + 1024;
   const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
-  const bool to_bf16 = (flags & W4_OUT_BF16) != 0;
   switch (flags & W4_EPI) {
     case W4_ACC: return to_bf16 ? FELLM_ERR_ARG : launch_tiles<W4_ACC, false>(map, a, parts, kb, grid, smem, stream);
     case W4_SWIGLU: return to_bf16 ? launch_tiles<W4_SWIGLU, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<W4_SWIGLU, false>(map, a, parts, kb, grid, smem, stream);

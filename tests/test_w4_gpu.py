@@ -414,3 +414,38 @@ def test_rows_that_came_with_a_norm_are_not_written_over(M):
     want = ops.gemm_w4(h.xg, w4, out_dtype=torch.float32, row_scale=(h.ssq, h.parts, 1e-5))
     assert torch.equal(other, want)
     ops.forget_norm_handoff()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,dtype", [(17, 65536, 64, "bfloat16"), (40, 65536, 128, "bfloat16"), (128, 65536, 256, "bfloat16"), (64, 65536, 512, "bfloat16"),
+                                         (300, 40000, 32, "bfloat16"), (20, 60000, 64, "float32"), (300, 30000, 64, "float32")])
+def test_more_tiles_than_stages(M, N, K, dtype):
+    """Of a short K the warps that make weights are tiles ahead of the products when they come to finish the last one with the others."""
+    from fellm_b200 import ops
+    g = _gen(M, N, K)
+    levels, scales = w4_util.random_matrix(N, K, 64, g, DEV)
+    w4, values = ops.pack_w4(levels, scales, 64), w4_util.plain_values(levels, scales, 64)
+    x = torch.randn(M, K, generator=g, device=DEV).to(getattr(torch, dtype))
+    exact, room = x.double() @ values.T, 1.25 * K * 2.0 ** -23 * (x.double().abs() @ values.abs().T)
+    for _ in range(10):
+        assert ((ops.gemm_w4(x, w4, out_dtype=torch.float32) - exact).abs() <= room).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("M,K", [(17, 8192), (40, 16384), (200, 40000), (600, 20000), (1100, 16384), (300, 70000)])
+def test_long_sums_are_as_near_as_float32_sums(M, K, dtype):
+    """Of n numbers of one size added one by one in float32, rounding to nearest, the k-th sum is off by 2^-24 / sqrt(3) of itself in the mean, and has
+    sqrt(k / n) of the last one's size: 2^-24 sqrt(n / 6) together.  Over a whole result the kernel's sums, by the type's rules and any order,
+    are no further off."""
+    from fellm_b200 import ops
+    g = _gen(M, K)
+    levels, scales = w4_util.random_matrix(512, K, 64, g, DEV)
+    w4, values = ops.pack_w4(levels, scales, 64), w4_util.plain_values(levels, scales, 64)
+    x = torch.randn(M, K, generator=g, device=DEV).to(getattr(torch, dtype))
+    exact = x.double() @ values.T
+    for kind in ("store", "accumulate"):
+        out = torch.zeros(M, 512, device=DEV)
+        ops.gemm_w4(x, w4, out=out, accumulate=kind == "accumulate")
+        assert (out - exact).norm() <= 2.0 ** -24 * (K / 6) ** 0.5 * exact.norm()
+
