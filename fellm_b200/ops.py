@@ -2106,6 +2106,8 @@ def dequantize_w4(w: W4, out_dtype=torch.bfloat16, out=None):
     _w4_matrix(out, "dequantize_w4")
     if tuple(out.shape) != w.shape:
         raise KernelError(f"dequantize_w4: a matrix of {list(w.shape)} does not fit {list(out.shape)}")
+    if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise KernelError(f"dequantize_w4: rows that lie over one another, strides {list(out.stride())}")
     _w4_dev(w.q, out)
     f = _fn("w4", "fellm_dequantize_w4", [_c_p, _c_p, _c_int, _c_ll, _c_p])
     _check(f(w._at, _p(out), _is_bf16(out), out.stride(0), _stream()), "dequantize_w4")
@@ -2186,10 +2188,13 @@ def gemm_w4(x, w: W4, bias=None, *, out=None, out_dtype=None, accumulate=False, 
     norm = left = None
     aligned = x_bf16 and K % 8 == 0 and (M == 1 or (ldx % 8 == 0 and ldx >= K)) and at % 16 == 0
     if row_scale is not None:
-        if M > HANDOFF_MAX_ROWS or not aligned or row_scale[0].data_ptr() % 16:
+        sums, parts, _ = row_scale
+        if (M > HANDOFF_MAX_ROWS or not aligned or sums.dtype != torch.float32 or not sums.is_contiguous() or sums.numel() < M * parts
+                or not 1 <= parts <= 128 or sums.get_device() != here or sums.data_ptr() % 16):
             raise KernelError(f"a product of {M} x {N} x {K} does not take a handed-on norm")
         norm = _W4Norm(ssq=row_scale[0].data_ptr(), parts=row_scale[1], eps=row_scale[2])
-    elif expected is not None and aligned and N % (part := 16 if M <= W4_FEW_ROWS else 32) == 0 and out.is_contiguous() and to % 8 == 0:
+    elif (expected is not None and aligned and M <= HANDOFF_MAX_ROWS and expected[1].numel() == N and N % (part := 16 if M <= W4_FEW_ROWS else 32) == 0
+          and out.is_contiguous() and to % 8 == 0):
         xg, ssq, _ = _handoff_bufs[out.device]
         if at != xg.data_ptr():              # (rows that came with a norm are not written over while they are read)
             _handoff = None                  # the buffers are about to be rewritten

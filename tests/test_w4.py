@@ -82,3 +82,5 @@ def test_rows_of_a_table_that_are_refused():
         ops.embed_rows_w4(tok.long(), _fake(), torch.zeros(3, 64))
     with pytest.raises(KernelError):
         ops.dequantize_w4(_fake(), out=torch.zeros(32, 63))
+    with pytest.raises(KernelError, match="over one another"):
+        ops.dequantize_w4(_fake(), out=torch.zeros(1, 64).expand(32, 64))

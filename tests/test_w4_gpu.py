@@ -390,6 +390,31 @@ def test_a_norm_that_is_not_handed_on():
     for x in (torch.zeros(129, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(2, 64, device=DEV), torch.zeros(130, device=DEV, dtype=torch.bfloat16)[1:129].view(2, 64)):
         with pytest.raises(KernelError, match="handed-on"):
             ops.gemm_w4(x, w4, row_scale=(ssq, 4, 1e-5))
+    x = torch.zeros(40, 64, device=DEV, dtype=torch.bfloat16)
+    for sums, parts in ((ssq[:40 * 4 - 1], 4), (ssq, 0), (ssq, 129), (ssq.double(), 4), (ssq[1:], 4), (ssq.cpu(), 4), (ssq[::2], 2)):
+        for rows in (x, x[:2]):
+            if rows is x or sums.numel() > 4 * 40 or sums.dtype != torch.float32:
+                with pytest.raises(KernelError, match="handed-on"):
+                    ops.gemm_w4(rows, w4, row_scale=(sums, parts, 1e-5))
+
+
+@pytest.mark.gpu
+def test_a_norm_of_another_width_or_of_too_many_rows_is_not_handed_on():
+    """A view that begins where the announced rows do is not those rows."""
+    from fellm_b200 import ops
+    ops.reserve_norm_handoff(DEV, 128)
+    weight = torch.ones(128, device=DEV)
+    w64, w128 = (ops.quantize_w4(torch.randn(n, 64, device=DEV), 32) for n in (64, 128))
+    stream = torch.zeros(200, 128, device=DEV)
+    for rows, w, out in ((1, w64, stream[:1, :64]), (200, w128, stream), (40, w64, stream.view(-1, 64)[:40])):
+        ops.forget_norm_handoff()
+        ops.expect_norm(stream[:100], weight)
+        x = torch.randn(rows, 64, device=DEV).bfloat16()
+        want = out + ops.gemm_w4(x, w, out_dtype=torch.float32)
+        ops.expect_norm(stream[:100], weight)
+        ops.gemm_w4(x, w, out=out, accumulate=True)
+        assert torch.equal(out, want) and ops._handoff is None
+    ops.forget_norm_handoff()
 
 
 @pytest.mark.gpu
