@@ -692,7 +692,9 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   const bool to_bf16 = (flags & W4_OUT_BF16) != 0;
   const int most = parts == 3 && chunks > W4U_RUN ? 128 : 256;          // (columns of a tile: tensor memory holds what its sums need)
   // Columns of a tile and CTAs that share its K, by the time of the busiest SM.  A chunk took 0.21 us up to 64 columns and 0.29 at 128,
-  // where the issuing warp bounds it, 0.37 at 256, where the MMAs do; a cluster's exchange 1.2 us and what its sums take at some 22 GB/s an SM.
+  // where the issuing warp bounds it, 0.37 at 256, where the MMAs do; a cluster's exchange 0.9 us and what its sums take at some 22 GB/s an SM.
+  // A product that takes nearly all SMs costs its neighbours a microsecond: nothing of the next one starts under it (32 rows, gated
+  // 9,216 x 1,024, one after another: 6.6 us in clusters of two on 144 SMs, 5.0 on 72 by themselves).
   double least = 1e30;
   int total = 1;
   a.bn = 16; a.splits = 1; a.log_splits = 0;
@@ -703,7 +705,7 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
     for (int ls = 0; ls <= 3; ++ls) {
       const int s = 1 << ls;
       if (s > 1 && (chunks < 4 * s || tiles > clusters_at_once(s))) break;
-      const double t = ceil_div(tiles * s, n_sm) * (double)ceil_div(chunks, s) * parts * chunk_us + (s > 1 ? 1.2 + bn * 0.0234 * (s - 1) / s : 0.0);
+      const double t = ceil_div(tiles * s, n_sm) * (double)ceil_div(chunks, s) * parts * chunk_us + (4 * tiles * s > 3 * n_sm ? 1.0 : 0.0) + (s > 1 ? 0.9 + bn * 0.0234 * (s - 1) / s : 0.0);
       if (t < least) { least = t; a.bn = bn; a.splits = s; a.log_splits = ls; total = tiles; }
     }
   }
