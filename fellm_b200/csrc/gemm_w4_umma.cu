@@ -77,6 +77,14 @@ __device__ __forceinline__ void umma_stage(unsigned d, unsigned a_lo, unsigned b
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n"
                  ::"r"(d), "r"(a_lo + 2 * k), "r"(b_lo + 2 * k), "r"(idesc), "r"(k ? 1u : accumulate), "r"(W4U_DESC_HI) : "memory");
 }
+// The same with the weights in tensor memory (a lane a row, two k a column): 8 columns an MMA.
+__device__ __forceinline__ void umma_stage_tmem(unsigned d, unsigned a, unsigned b_lo, unsigned idesc, unsigned accumulate) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    asm volatile("{\n.reg .pred p;\n.reg .b64 db;\nsetp.ne.b32 p, %4, 0;\nmov.b64 db, {%2, %5};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n"
+                 ::"r"(d), "r"(a + 8 * k), "r"(b_lo + 2 * k), "r"(idesc), "r"(k ? 1u : accumulate), "r"(W4U_DESC_HI) : "memory");
+}
 // One lane of a converged warp, the same one every time.  (A role's loop runs in the whole warp, so that its counters and
 // descriptors are uniform; a loop inside `if (lane == 0)` took some 800 cycles a stage for its scalar arithmetic.)
 __device__ __forceinline__ bool elect_one() {
@@ -115,6 +123,13 @@ __device__ __forceinline__ void tmem_add16(unsigned to, unsigned from) {
                ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(to) : "memory");
 }
+__device__ __forceinline__ void tmem_st32(unsigned taddr, const unsigned* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+               "%27,%28,%29,%30,%31};\n"
+               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+                 "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+                 "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 // N columns of a tile's sums, the sums of two accumulators `lo` columns apart (0: of one).
 template <int N> __device__ __forceinline__ void tmem_sums(unsigned at, unsigned lo, float* v) {
@@ -150,6 +165,7 @@ struct W4uArgs {
   int m_tiles, total;        // tiles along x, and all of them
   int stages, splits, log_splits, tmem_cols;
   int run;                   // blocks of K that are summed in one accumulator
+  int raw_at, w_col;         // KB 2: where the warps' rings lie, from the stages on; the first column of tensor memory of the weights
   int buffers, acc_cols;     // accumulators (used in turn), columns of tensor memory from one to the next
   int share;                 // columns of a tile that a rank of a cluster finishes, a multiple of 4
   int recv_apart;            // what other ranks send lies behind the stages, not over them
@@ -161,11 +177,25 @@ struct W4uArgs {
 // additions put together, and the two small pieces of float32 rows have an accumulator of their own.  (bfloat16 results are rounded
 // to 2e-3 behind it.)
 #define W4U_RUN 48
+#define W4U_RAW 4                     // units of a warp's ring of levels (KB 2): two slabs' chunk, their scales
+#define W4U_RAW_SLOT 1152
 #define W4U_NORM_ROWS 128             // rows of a product that a norm is handed on to or by: one tile's
 
 __device__ __forceinline__ void st_shared_v4(unsigned addr, unsigned a, unsigned b, unsigned c, unsigned d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+
+__device__ __forceinline__ unsigned ld_shared(unsigned addr) {
+  unsigned v;
+  asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_shared_v4(unsigned addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void copy16(unsigned dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory"); }
 
 // SiLU(g) * u for a bfloat16 result: the approximate exponential and quotient are off by some 2^-20, a three-hundredth of the rounding
 // behind them, and take a fifth of the instructions (2,048 rows, 16,384 x 2,048: the epilogue took longer than the MMAs of a tile).
@@ -345,7 +375,8 @@ struct Ring {
 template <bool SPLIT, int PARTS, int KB, int EPI, bool BF16, bool HANDED>
 __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
   constexpr int AHEAD = 4 / KB;          // stages whose chunks a warp holds in registers ahead of the one it unpacks
-  constexpr unsigned A_BYTES = KB * W4U_A_BYTES;
+  constexpr bool TMEM = KB == 2;         // weights in tensor memory
+  constexpr unsigned A_BYTES = TMEM ? 0u : KB * W4U_A_BYTES;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];           // full[8], empty[8], acc_full[2], acc_empty[2]
   __shared__ unsigned tmem_base_s;
@@ -363,12 +394,13 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   const int c_lo = SPLIT ? ((k_stages * rank) >> a.log_splits) * KB : 0, c_hi = SPLIT ? ((k_stages * (rank + 1)) >> a.log_splits) * KB : k_stages * KB;
   const int blocks = (c_hi - c_lo) / KB * PARTS;
 
-  pdl_launch_dependents();
-  // Barriers and tensor memory are made while the weights' warps ask for their first chunks.
+  // Barriers and tensor memory are made while the weights' warps ask for their first chunks.  (Tensor memory before the next kernel may start:
+  // one that took it first, and waited for this one, would never see its end.)
   auto set_up = [&]() {
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    pdl_launch_dependents();
     if (SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");        // (waited for where another rank's memory is written)
   };
   if (warp == 0 && lane == 0) {
@@ -404,7 +436,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       }
     }
   } else if (warp == 1) {
-    const unsigned idesc = umma_idesc(128, a.bn), a_lo = umma_desc_lo(tiles), tmem_base = tmem_base_s;
+    const unsigned idesc = umma_idesc(128, a.bn), a_lo = umma_desc_lo(tiles), tmem_base = tmem_base_s, w_base = tmem_base + a.w_col;
     unsigned use = 0;
     Ring ring;
     for (int t = first; t < total; t += step) {
@@ -421,7 +453,8 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
           if (elect_one()) {
 #pragma unroll
             for (int i = 0; i < KB; ++i)
-              umma_stage(to, lo + i * (W4U_A_BYTES >> 4), lo + (A_BYTES >> 4) + i * (x_bytes >> 4), idesc, (b | i) && !(PARTS == 3 && b == 2) ? 1u : 0u);
+              if (TMEM) umma_stage_tmem(to, w_base + ring.stage * (KB * 32) + i * 32, lo + i * (x_bytes >> 4), idesc, (b | i) ? 1u : 0u);
+              else umma_stage(to, lo + i * (W4U_A_BYTES >> 4), lo + (A_BYTES >> 4) + i * (x_bytes >> 4), idesc, (b | i) && !(PARTS == 3 && b == 2) ? 1u : 0u);
             umma_commit(empty);
             if (b == run - 1) umma_commit(accfull0 + 8 * acc);
           }
@@ -430,7 +463,81 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         }
       }
     }
-  } else if (warp < 2 + 8 * SETS) {
+  } else if (TMEM && warp < 2 + 8 * SETS) {
+    // Weights into tensor memory: a warp has 32 rows (its quarter of the lanes) of every set's stage's one or other chunk.  A lane is a row:
+    // its 64 weights lie with those of the row 8 further on in four lanes' 16 bytes of the layout, which come through a ring of the warp's
+    // own in shared memory, in an order in which neither the copies nor the reads meet a bank twice.
+    const int quarter = warp & 3, set = (warp - 2) >> 3, sub = ((warp - 2) >> 2) & 1, g = lane & 7, slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB;
+    const unsigned raw = tiles + a.raw_at + (warp - 2) * W4U_RAW * W4U_RAW_SLOT;
+    const unsigned copy_at = (unsigned)((lane >> 2) * 4 + ((lane & 3) ^ ((lane >> 3) & 3))) * 16u;
+    const unsigned read_at = (unsigned)(lane >> 4) * 512u + (unsigned)g * 64u, turn = (unsigned)((g >> 1) & 3) * 16u, scale_at = 1024u + (unsigned)(lane >> 4) * 64u + (unsigned)g * 4u;
+    const int high = (lane >> 3) & 1;
+    const bool two_scales = a.w.gshift == 5;
+    Ring base;
+    for (int t = first; t < total; t += step) {
+      const int slab = (t / m_tiles) * 8 + quarter * 2, mine = slab + (lane >> 4);
+      // (a slab that is not there: the first one, times 0)
+      const uint4* q0 = a.w.q + ((size_t)(slab < slabs ? slab : 0) * a.w.chunks + c_lo) * 32 + lane;
+      const uint4* q1 = a.w.q + ((size_t)(slab + 1 < slabs ? slab + 1 : 0) * a.w.chunks + c_lo) * 32 + lane;
+      const int s_slab = slab + ((lane >> 2) & 1);
+      const unsigned* sc = a.w.s + (size_t)(s_slab < slabs ? s_slab : 0) * a.w.groups * 8 + (lane & 1) * 4;
+      const unsigned s_more = two_scales ? (lane >> 1) & 1 : 0;
+      int ahead = set;
+      unsigned slot = 0, read_slot = 0;
+      auto fetch = [&]() {
+        if (ahead < blocks) {
+          const unsigned to = raw + slot * W4U_RAW_SLOT, chunk = ahead * KB + sub;
+          copy16(to + copy_at, q0 + chunk * 32u);
+          copy16(to + 512u + copy_at, q1 + chunk * 32u);
+          if (lane < 8) copy16(to + 1024u + lane * 16u, sc + (((((unsigned)c_lo + chunk) * W4_CHUNK) >> a.w.gshift) + s_more) * 8u);
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        ahead += SETS;
+        slot = slot == W4U_RAW - 1 ? 0 : slot + 1;
+      };
+      Ring ring = base;
+      ring.add(set, a.stages);
+#pragma unroll 1
+      for (int u = 0; u < W4U_RAW - 1; ++u) fetch();
+      if (t == first) set_up();
+      const unsigned to = tmem_base_s + a.w_col + ((unsigned)(quarter * 32) << 16) + sub * 32;
+      for (int b = set; b < blocks; b += SETS) {
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(W4U_RAW - 2) : "memory");
+        __syncwarp();                                        // every lane's copies have come, and every lane has read the unit before
+        fetch();                                             // over that one
+        const unsigned at = raw + read_slot * W4U_RAW_SLOT;
+        read_slot = read_slot == W4U_RAW - 1 ? 0 : read_slot + 1;
+        const bool in = mine < slabs && c_lo + b * KB + sub < a.w.chunks;
+        const unsigned sa = in ? ld_shared(at + scale_at) : 0u, sb = two_scales ? (in ? ld_shared(at + scale_at + 32u) : 0u) : sa;
+        unsigned v[32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint4 x = ld_shared_v4(at + read_at + (((unsigned)c * 16u) ^ turn));
+          const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned s2 = __byte_perm(h ? sb : sa, 0, high ? 0x3232 : 0x1010), off = times_minus_24(s2);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              v[16 * h + 4 * c + 2 * j] = w4_value(w[2 * h + j], high, s2, off);
+              v[16 * h + 4 * c + 2 * j + 1] = w4_value(w[2 * h + j], high + 2, s2, off);
+            }
+          }
+        }
+        W4U_WAIT(empty0 + 8 * ring.stage, ring.parity ^ 1u, 143);
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        __syncwarp();
+        tmem_st32(to + ring.stage * (KB * 32), v);
+        tmem_st_wait();
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full0 + 8 * ring.stage);
+        ring.add(SETS, a.stages);
+      }
+      __syncwarp();
+      base.add_many(blocks, a.stages);
+    }
+  } else if (!TMEM && warp < 2 + 8 * SETS) {
     // weights: nothing in front of this kernel writes them, so they need not wait for it
     const int sl = (warp - 2) & 7, set = (warp - 2) >> 3, g = lane >> 2, c = lane & 3, slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB;
     Ring base;
@@ -710,12 +817,9 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
     }
   }
   a.m_tiles = ceil_div(M, a.bn); a.total = total;
-  const int kb = parts == 1 && a.bn <= 128 ? 2 : 1, stage = kb * (W4U_A_BYTES + a.bn * 128), room = 220 * 1024;
+  const int kb = parts == 1 && a.bn <= 128 ? 2 : 1, stage = kb * a.bn * 128 + (kb == 2 ? 0 : W4U_A_BYTES), raw = kb == 2 ? 8 * SETS * W4U_RAW * W4U_RAW_SLOT : 0;
   a.share = ceil_div(a.bn / 4, a.splits) * 4;
-  const int recv = (a.splits - 1) * a.share * 512;
-  a.stages = room / stage < 8 ? room / stage : 8;
-  a.recv_apart = (room - recv) / stage >= 3;
-  if (a.recv_apart && (room - recv) / stage < a.stages) a.stages = (room - recv) / stage;
+  const int room = 220 * 1024 - raw, recv = (a.splits - 1) * a.share * 512;
   const int blocks = ceil_div(ceil_div(chunks, kb), a.splits) * parts;
   const int runs = to_bf16 ? 1 : ceil_div(blocks, W4U_RUN / kb * parts);
   a.run = ceil_div(blocks / parts, runs) * parts;
@@ -724,8 +828,14 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   if (parts == 3) a.acc_cols *= 2;
   a.buffers = (a.splits == 1 || runs > 1) && 2 * a.acc_cols <= 512 ? 2 : 1;
   if (runs > 1 && a.buffers < 2) return FELLM_ERR_SIZE;
-  a.tmem_cols = a.buffers * a.acc_cols < 32 ? 32 : a.buffers * a.acc_cols;
+  a.tmem_cols = kb == 2 ? 512 : a.buffers * a.acc_cols < 32 ? 32 : a.buffers * a.acc_cols;
+  a.stages = room / stage < 8 ? room / stage : 8;
+  a.w_col = ceil_div(a.buffers * a.acc_cols, 64) * 64;
+  if (kb == 2 && (512 - a.w_col) / 64 < a.stages) a.stages = (512 - a.w_col) / 64;
+  a.recv_apart = (room - recv) / stage >= 3;
+  if (a.recv_apart && (room - recv) / stage < a.stages) a.stages = (room - recv) / stage;
   if (!a.recv_apart && recv > a.stages * stage) return FELLM_ERR_SIZE;
+  a.raw_at = a.stages * stage + (a.recv_apart ? recv : 0);
   EncodeTiledFn fn = encode_fn();
   if (!fn) return FELLM_ERR_ARG;
   CUtensorMap map;
@@ -735,7 +845,7 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return 1000 + (int)r;
-  const size_t smem = (size_t)a.stages * stage + (a.recv_apart ? recv : 0) + 1024;
+  const size_t smem = (size_t)a.raw_at + raw + 1024;
   const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
   switch (flags & W4_EPI) {
     case W4_ACC: return to_bf16 ? FELLM_ERR_ARG : launch_tiles<W4_ACC, false>(map, a, parts, kb, grid, smem, stream);
