@@ -477,23 +477,22 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     for (int t = first; t < total; t += step) {
       const int slab = (t / m_tiles) * 8 + quarter * 2, mine = slab + (lane >> 4);
       // (a slab that is not there: the first one, times 0)
-      const uint4* q0 = a.w.q + ((size_t)(slab < slabs ? slab : 0) * a.w.chunks + c_lo) * 32 + lane;
-      const uint4* q1 = a.w.q + ((size_t)(slab + 1 < slabs ? slab + 1 : 0) * a.w.chunks + c_lo) * 32 + lane;
-      const int s_slab = slab + ((lane >> 2) & 1);
-      const unsigned* sc = a.w.s + (size_t)(s_slab < slabs ? s_slab : 0) * a.w.groups * 8 + (lane & 1) * 4;
-      const unsigned s_more = two_scales ? (lane >> 1) & 1 : 0;
-      int ahead = set;
-      unsigned slot = 0, read_slot = 0;
+      const int s_slab = slab + ((lane >> 2) & 1), c_first = c_lo + set * KB + sub;
+      const uint4* q0 = a.w.q + ((size_t)(slab < slabs ? slab : 0) * a.w.chunks + c_first) * 32 + lane;
+      const long long q1 = ((long long)(slab + 1 < slabs ? slab + 1 : 0) - (slab < slabs ? slab : 0)) * a.w.chunks * 32;
+      const unsigned* sc = a.w.s + ((size_t)(s_slab < slabs ? s_slab : 0) * a.w.groups + (two_scales ? (lane >> 1) & 1 : 0)) * 8 + (lane & 1) * 4;
+      int left = (blocks - set + SETS - 1) / SETS;            // of this set's blocks, to be fetched
+      unsigned k = (unsigned)c_first * W4_CHUNK, write_at = raw, at = raw;
       auto fetch = [&]() {
-        if (ahead < blocks) {
-          const unsigned to = raw + slot * W4U_RAW_SLOT, chunk = ahead * KB + sub;
-          copy16(to + copy_at, q0 + chunk * 32u);
-          copy16(to + 512u + copy_at, q1 + chunk * 32u);
-          if (lane < 8) copy16(to + 1024u + lane * 16u, sc + (((((unsigned)c_lo + chunk) * W4_CHUNK) >> a.w.gshift) + s_more) * 8u);
+        if (--left >= 0) {
+          copy16(write_at + copy_at, q0);
+          copy16(write_at + 512u + copy_at, q0 + q1);
+          if (lane < 8) copy16(write_at + 1024u + lane * 16u, sc + (k >> a.w.gshift) * 8u);
+          q0 += SETS * KB * 32;
+          k += SETS * KB * W4_CHUNK;
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
-        ahead += SETS;
-        slot = slot == W4U_RAW - 1 ? 0 : slot + 1;
+        write_at = write_at == raw + (W4U_RAW - 1) * W4U_RAW_SLOT ? raw : write_at + W4U_RAW_SLOT;
       };
       Ring ring = base;
       ring.add(set, a.stages);
@@ -505,8 +504,6 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         asm volatile("cp.async.wait_group %0;\n" ::"n"(W4U_RAW - 2) : "memory");
         __syncwarp();                                        // every lane's copies have come, and every lane has read the unit before
         fetch();                                             // over that one
-        const unsigned at = raw + read_slot * W4U_RAW_SLOT;
-        read_slot = read_slot == W4U_RAW - 1 ? 0 : read_slot + 1;
         const bool in = mine < slabs && c_lo + b * KB + sub < a.w.chunks;
         const unsigned sa = in ? ld_shared(at + scale_at) : 0u, sb = two_scales ? (in ? ld_shared(at + scale_at + 32u) : 0u) : sa;
         unsigned v[32];
@@ -524,6 +521,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
             }
           }
         }
+        at = at == raw + (W4U_RAW - 1) * W4U_RAW_SLOT ? raw : at + W4U_RAW_SLOT;
         W4U_WAIT(empty0 + 8 * ring.stage, ring.parity ^ 1u, 143);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         __syncwarp();
