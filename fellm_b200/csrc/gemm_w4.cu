@@ -8,7 +8,7 @@
 // in one order.
 //
 // Bound by the matrix's bytes where enough of them are on their way and by the instructions that unpack them: an SM's four
-// schedulers have some 86 cycles each for a chunk that memory delivers.  So every warp keeps two units (4 KB) in flight through
+// schedulers have some 86 cycles each for a chunk that memory delivers.  So every warp keeps three units (6.8 KB) in flight through
 // a ring of its own in shared memory (cp.async: no registers are held, and the ring runs on over the end of a slab), and what
 // is not unpacking is shared out over four chunks.
 //

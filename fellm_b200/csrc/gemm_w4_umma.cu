@@ -1,17 +1,28 @@
 // y = x W^T of a matrix in four bits (w4.h) for more than a handful of rows, on tcgen05: D[n, t] = sum_k W[n, k] x[t, k], the
 // MMA's 128 rows are weight rows, its 16 to 256 columns are rows of x.
 //
-// The weights become bfloat16 on their way into shared memory: level * scale is a bfloat16 number exactly (w4.h), so this
-// rounds nothing, and K may be summed in one accumulator whatever the groups.  Eight warps take a slab of 16 rows each:
-// 16 bytes a lane from memory, several chunks ahead in registers, are 32 weights, four 16-byte pieces of the tile in the
-// 128-byte swizzle that the MMA reads.  (16 + level + 8) is a shift and an and-or away (the four bits at the top of bfloat16's
-// mantissa at exponent 4), and one fused multiply-add makes (that) * s - 24 s: both 24 s and the result are bfloat16 numbers.
+// The weights become bfloat16 on their way to the MMA: level * scale is a bfloat16 number exactly (w4.h), so this
+// rounds nothing, and K may be summed in one accumulator whatever the groups.  (16 + level + 8) is a shift and an and-or away (the
+// four bits at the top of bfloat16's mantissa at exponent 4), and one fused multiply-add makes (that) * s - 24 s: both 24 s and the
+// result are bfloat16 numbers.  Sixteen warps do this, eight a stage, the next stage's eight at the same time.
+//
+// Tiles of up to 128 rows of x (KB 2: two chunks of K a stage) have their weights in TENSOR memory, a lane a row: the levels come through a
+// ring of each warp's own (cp.async) and leave by tcgen05.st.  In shared memory, writing them and the MMA's reading them take 256 of the
+// some 340 cycles a chunk, whatever the width (32 rows, 8,192 x 8,192: 17.4 us, in tensor memory 15.7; 128 rows: 23.3 and 21.2).
+// Wider tiles (KB 1) need tensor memory for their sums and are bound by the MMAs: there the weights go to shared memory in the 128-byte
+// swizzle, a warp a slab of 16 rows, 16 bytes a lane from memory, several chunks ahead in registers.
 // x comes by TMA, one thread issues the MMAs, four warps store what is finished: lane = weight row, so a row of the result
 // leaves in pieces of 32 neighbouring columns.
 //
 // Persistent over tiles with two accumulators in tensor memory; where there are too few tiles for the SMs, the K range of a
 // tile is shared out over a cluster of 2, 4 or 8 CTAs, whose sums are put together through distributed shared memory, in
-// rank order, each rank finishing its share of the columns.
+// rank order, each rank finishing its share of the columns, four at a time.  A decode step's products are a few microseconds, a good part
+// of it code that runs once: a short loop over four columns beats straight code for sixteen, and every long division in front of
+// the first load shows (32 requests of a 16-layer model of width 1,024: 0.553 -> 0.495 ms a step by these).
+//
+// Measured, one after another from a graph: 64 rows, 8,192 x 8,192 16.9 us (floor 5.8: unpacking bounds it, some 280 cycles a chunk, and
+// 7 us of launch, first loads, exchange and stores); 2,048 rows, gated 16,384 x 2,048 102 us, 1,346 TFLOP/s; 4,096 rows, 8,192 x 8,192
+// 386 us, 1,422 TFLOP/s.
 //
 // Roles in a CTA: warp 0 TMA of x (one lane), warp 1 MMA issuer (one lane) and owner of tensor memory, then two sets of
 // eight warps for weights, the last four warps epilogue (tensor memory lanes 32 (warp % 4) ..).  Every wait on an mbarrier is bounded: after a
@@ -367,16 +378,16 @@ struct Ring {
   __device__ __forceinline__ void add_many(unsigned n, unsigned stages) { stage += n; parity ^= (stage / stages) & 1u; stage %= stages; }
 };
 
-// KB: chunks of K a stage.  Two where a tile is narrow: one handshake and one commit cost the issuing warp as much as three MMAs of 64
-// columns (377 cycles a stage of one chunk, 40 an MMA).
+// KB: chunks of K a stage.  Two where a tile is narrow (up to 128 columns), whose weights go to tensor memory: one handshake and one commit cost the
+// issuing warp as much as three MMAs of 64 columns.
 // EPI, BF16: what becomes of the sums, and whether the result is bfloat16 (kernels of their own: with all of them in one, the registers that
 // one wants are spilled by the others, 2,048 rows of a gated 16,384 x 2,048 106 -> 114 us).
 // HANDED: a norm is handed on to it or by it.
 template <bool SPLIT, int PARTS, int KB, int EPI, bool BF16, bool HANDED>
 __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
-  constexpr int AHEAD = 4 / KB;          // stages whose chunks a warp holds in registers ahead of the one it unpacks
+  constexpr int AHEAD = 4;               // stages (KB 1) whose chunk a warp holds in registers ahead of the one it unpacks
   constexpr bool TMEM = KB == 2;         // weights in tensor memory
-  constexpr unsigned A_BYTES = TMEM ? 0u : KB * W4U_A_BYTES;
+  constexpr unsigned A_BYTES = TMEM ? 0u : W4U_A_BYTES;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long bars[2 * 8 + 4];           // full[8], empty[8], acc_full[2], acc_empty[2]
   __shared__ unsigned tmem_base_s;
@@ -454,7 +465,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
 #pragma unroll
             for (int i = 0; i < KB; ++i)
               if (TMEM) umma_stage_tmem(to, w_base + ring.stage * (KB * 32) + i * 32, lo + i * (x_bytes >> 4), idesc, (b | i) ? 1u : 0u);
-              else umma_stage(to, lo + i * (W4U_A_BYTES >> 4), lo + (A_BYTES >> 4) + i * (x_bytes >> 4), idesc, (b | i) && !(PARTS == 3 && b == 2) ? 1u : 0u);
+              else umma_stage(to, lo, lo + (A_BYTES >> 4), idesc, b && !(PARTS == 3 && b == 2) ? 1u : 0u);
             umma_commit(empty);
             if (b == run - 1) umma_commit(accfull0 + 8 * acc);
           }
@@ -549,53 +560,47 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
       const bool have = slab < slabs;
       const uint4* q = a.w.q + ((size_t)(have ? slab : 0) * a.w.chunks + c_lo) * 32 + lane;
       const unsigned* sc = a.w.s + (size_t)(have ? slab : 0) * a.w.groups * 8 + g;
-      uint4 qv[AHEAD][KB];
-      unsigned sv[AHEAD][KB][2];
+      uint4 qv[AHEAD];
+      unsigned sv[AHEAD][2];
       // This set's blocks of the tile: set, set + SETS, ...; `ahead`: the next one to be fetched.  Behind the last one loads go on
       // (into the next slab or the room behind the matrix): a load that may not happen would have to be waited for at once.
       unsigned ahead = set;
-      auto fetch = [&](int u, int i) {
-        const unsigned ch = PARTS == 1 ? ahead * KB + i : ahead / 3;
-        qv[u][i] = __ldg(q + ch * 32u);
+      auto fetch = [&](int u) {
+        const unsigned ch = PARTS == 1 ? ahead : ahead / 3;
+        qv[u] = __ldg(q + ch * 32u);
         const unsigned* at = sc + ((((unsigned)c_lo + ch) * W4_CHUNK) >> a.w.gshift) * 8u;
-        sv[u][i][0] = __ldg(at);
-        sv[u][i][1] = __ldg(at + (two_scales ? 8 : 0));
-        if (i == KB - 1) ahead += SETS;
+        sv[u][0] = __ldg(at);
+        sv[u][1] = __ldg(at + (two_scales ? 8 : 0));
+        ahead += SETS;
       };
       Ring ring = base;
       ring.add(set, a.stages);
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-        for (int i = 0; i < KB; ++i) fetch(u, i);
+      for (int u = 0; u < AHEAD; ++u) fetch(u);
       if (t == first) set_up();
       for (int b0 = set; b0 < blocks; b0 += SETS * AHEAD) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
           if (b0 + u * SETS >= blocks) break;
           const unsigned at = ring.stage * stage_bytes;
+          const uint4 x = qv[u];
+          const unsigned sa = have ? sv[u][0] : 0u, sb = have ? sv[u][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
+          const unsigned w[4] = {flip ? x.z : x.x, flip ? x.w : x.y, flip ? x.x : x.z, flip ? x.y : x.w};
+          unsigned v[2][2][4];                              // [row g, g + 8][piece][..]
 #pragma unroll
-          for (int i = 0; i < KB; ++i) {
-            const bool in = have && (i == 0 || c_lo + (b0 + u * SETS) * KB + i < a.w.chunks);
-            const uint4 x = qv[u][i];
-            const unsigned sa = in ? sv[u][i][0] : 0u, sb = in ? sv[u][i][1] : 0u, s_first = flip ? sb : sa, s_second = flip ? sa : sb;
-            const unsigned w[4] = {flip ? x.z : x.x, flip ? x.w : x.y, flip ? x.x : x.z, flip ? x.y : x.w};
-            unsigned v[2][2][4];                            // [row g, g + 8][piece][..]
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
-                v[r][h][0] = w4_value(w[2 * h], r, s2, off); v[r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
-                v[r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
-              }
-            fetch(u, i);
-            if (i == 0) W4U_WAIT(empty0 + 8 * ring.stage, ring.parity ^ 1u, 143);
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {                   // (row g + 8: eight rows of 128 bytes further on)
-              st_shared_v4(at + p0 + i * W4U_A_BYTES + r * 1024u, v[r][0][0], v[r][0][1], v[r][0][2], v[r][0][3]);
-              st_shared_v4(at + p1 + i * W4U_A_BYTES + r * 1024u, v[r][1][0], v[r][1][1], v[r][1][2], v[r][1][3]);
+            for (int h = 0; h < 2; ++h) {
+              const unsigned s2 = __byte_perm(h ? s_second : s_first, 0, r ? 0x3232 : 0x1010), off = times_minus_24(s2);
+              v[r][h][0] = w4_value(w[2 * h], r, s2, off); v[r][h][1] = w4_value(w[2 * h], r + 2, s2, off);
+              v[r][h][2] = w4_value(w[2 * h + 1], r, s2, off); v[r][h][3] = w4_value(w[2 * h + 1], r + 2, s2, off);
             }
+          fetch(u);
+          W4U_WAIT(empty0 + 8 * ring.stage, ring.parity ^ 1u, 143);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {                     // (row g + 8: eight rows of 128 bytes further on)
+            st_shared_v4(at + p0 + r * 1024u, v[r][0][0], v[r][0][1], v[r][0][2], v[r][0][3]);
+            st_shared_v4(at + p1 + r * 1024u, v[r][1][0], v[r][1][1], v[r][1][2], v[r][1][3]);
           }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
           __syncwarp();
@@ -796,8 +801,9 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   const int n_sm = fellm_sm_count(), n_tiles = ceil_div(N, 128);
   const bool to_bf16 = (flags & W4_OUT_BF16) != 0;
   const int most = parts == 3 && chunks > W4U_RUN ? 128 : 256;          // (columns of a tile: tensor memory holds what its sums need)
-  // Columns of a tile and CTAs that share its K, by the time of the busiest SM.  A chunk took 0.21 us up to 64 columns and 0.29 at 128,
-  // where the issuing warp bounds it, 0.37 at 256, where the MMAs do; a cluster's exchange 0.9 us and what its sums take at some 22 GB/s an SM.
+  // Columns of a tile and CTAs that share its K, by the time of the busiest SM.  A chunk counts 0.21 us up to 64 columns and 0.29 at 128
+  // (weights in tensor memory take 0.15 to 0.17 in a long K, but few have one: with that, steps of 64 and 128 requests got 8 to 12% slower),
+  // 0.37 at 256, where the MMAs bound it; a cluster's exchange 0.9 us and what its sums take at some 22 GB/s an SM.
   // A product that takes nearly all SMs costs its neighbours a microsecond: nothing of the next one starts under it (32 rows, gated
   // 9,216 x 1,024, one after another: 6.6 us in clusters of two on 144 SMs, 5.0 on 72 by themselves).
   double least = 1e30;
