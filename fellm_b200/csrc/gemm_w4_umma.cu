@@ -406,7 +406,8 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   const int blocks = (c_hi - c_lo) / KB * PARTS;
 
   // Barriers and tensor memory are made while the weights' warps ask for their first chunks.  (Tensor memory before the next kernel may start:
-  // one that took it first, and waited for this one, would never see its end.)
+  // one that took it first, and waited for this one, would never see its end.  Nor is this one beside another that takes tensor memory: 704
+  // threads of 80 registers leave 9,216.)
   auto set_up = [&]() {
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
