@@ -91,6 +91,35 @@ def test_replayed_steps_are_the_launched_ones(util, name, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("requests", [24, 70, 128, 150])
+@pytest.mark.parametrize("util,name", [(tiny, "A"), (tiny, "B"), (tiny, "C"), (meresun_util, "A")], ids=["lfm2-A", "lfm2-B", "lfm2-C", "meresun-A"])
+def test_a_step_of_many_requests(util, name, requests, monkeypatch):
+    """Decode steps of up to 128 requests, whose products hand norms on where the widths are multiples of 32, and of more."""
+    opts = dict(max_requests=requests, max_tokens=requests * 64)
+    kept, four = _engines(util, name, "bfloat16", 64, **opts)
+    taken = []
+    product = ops.gemm_w4
+    monkeypatch.setattr(ops, "gemm_w4", lambda *a, **k: (taken.append(k.get("row_scale") is not None), product(*a, **k))[1])
+    rng = np.random.default_rng(requests)
+    first = rng.integers(0, four.spec.vocab_size, (requests, 3))
+    then = rng.integers(0, four.spec.vocab_size, (4, requests))
+    rows = []
+    for eng in (four, kept):
+        for r in range(requests):
+            eng.add_request(f"r{r}")
+        for lo in range(0, requests, 16):
+            eng.step([StepItem(f"r{r}", [int(t) for t in first[r]], []) for r in range(lo, min(lo + 16, requests))])
+        taken.clear()
+        rows.append(torch.cat([eng.step([StepItem(f"r{r}", [int(step[r])], [0]) for r in range(requests)]) for step in then]).double())
+        eng.check_status()
+        if eng is four and util is tiny:                     # (the other designs' blocks norm their own inputs)
+            assert any(taken) == (requests <= 128 and four.spec.hidden_size % 32 == 0)
+    got, want = (x - x.mean(-1, keepdim=True) for x in rows)
+    off = (got - want).pow(2).mean(-1).sqrt() / want.pow(2).mean().sqrt()
+    assert float(off.max()) <= _limit(util, "bfloat16"), float(off.max())
+
+
+@pytest.mark.gpu
 def test_a_portion_is_the_same_tokens_one_by_one():
     eng = tiny.make_engine("B", "float32", weights="int4")
     toks = tiny.tokens("B", 40, 3)
