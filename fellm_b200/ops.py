@@ -2006,7 +2006,7 @@ class _W4Norm(ctypes.Structure):
 
 class W4:
     """A matrix [N, K] in four bits: w[n, k] = level[n, k] * scale[n, k // group], levels -8..7, scales of at most five
-    significant bits (level * scale is a bfloat16 number exactly, so every kernel that reads the matrix multiplies with the
+    significant bits, K up to 2^20 (level * scale is a bfloat16 number exactly, so every kernel that reads the matrix multiplies with the
     same numbers).  Made by quantize_w4 or pack_w4, which return when it is laid out: any stream may read it, and a product
     may ask for it before the kernel in front has ended.  q, scales: the kernels' layout (csrc/w4.h); nothing writes them again."""
     dtype = "int4"                          # (of no torch dtype: what asks a matrix for bfloat16 leaves it alone)
@@ -2039,7 +2039,7 @@ def _w4_room(N: int, K: int, group: int, device):
     """Levels [slabs, chunks, 128] and scales [slabs, groups, 8], each with room behind it that a kernel may read ahead into."""
     if group not in W4_GROUPS:
         raise KernelError(f"a group of {group}: four-bit matrices have groups of {', '.join(map(str, W4_GROUPS))}")
-    if N < 1 or K < 1 or N > 2 ** 30 or K > 2 ** 28:
+    if N < 1 or K < 1 or N > 2 ** 30 or K > 2 ** 20:           # (a bfloat16 result's K is one sum in tensor memory: its error grows with it)
         raise KernelError(f"a matrix of {N} x {K} cannot be held in four bits")
     slabs, chunks = -(-N // 16), -(-K // 64)
     return (torch.empty((slabs * chunks + W4_READ_AHEAD) * 128, dtype=torch.int32, device=device),

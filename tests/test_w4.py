@@ -43,7 +43,7 @@ def test_groups_that_are_none(group):
 
 
 def test_matrices_that_are_none():
-    for w in (torch.zeros(64), torch.zeros(4, 4, 4), torch.zeros(0, 64), torch.zeros(64, 0), torch.zeros(64, 32).T):
+    for w in (torch.zeros(64), torch.zeros(4, 4, 4), torch.zeros(0, 64), torch.zeros(64, 0), torch.zeros(64, 32).T, torch.zeros(1, 2 ** 20 + 1)):
         with pytest.raises(KernelError):
             ops.quantize_w4(w, 32)
     with pytest.raises(KernelError, match="CUDA"):
