@@ -142,14 +142,28 @@ __device__ __forceinline__ void tmem_st32(unsigned taddr, const unsigned* r) {
                  "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
-// N columns of a tile's sums, the sums of two accumulators `lo` columns apart (0: of one).
-template <int N> __device__ __forceinline__ void tmem_sums(unsigned at, unsigned lo, float* v) {
+template <int N> __device__ __forceinline__ void tmem_ld(unsigned at, float* v) {
   if (N == 16) tmem_ld16(at, v);
   else tmem_ld4(at, v);
-  if (!lo) return;
+}
+// N columns of a tile's sums: of an accumulator and the one `before` columns from it (0: of one run), each the sums of two that lie `lo` columns
+// apart (0: of one).
+template <int N> __device__ __forceinline__ void tmem_sums(unsigned at, unsigned lo, unsigned before, float* v) {
   float more[N];
-  if (N == 16) tmem_ld16(at + lo, more);
-  else tmem_ld4(at + lo, more);
+  tmem_ld<N>(at, v);
+  if (before) {
+    tmem_ld<N>(at + before, more);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] += more[j];
+  }
+  if (!lo) return;
+  tmem_ld<N>(at + lo, more);
+  if (before) {
+    float last[N];
+    tmem_ld<N>(at + before + lo, last);
+#pragma unroll
+    for (int j = 0; j < N; ++j) more[j] += last[j];
+  }
 #pragma unroll
   for (int j = 0; j < N; ++j) v[j] += more[j];
 }
@@ -184,9 +198,11 @@ struct W4uArgs {
 };
 // The tensor cores cut a sum's last bits off where they add to it, always towards zero: float32 results of bfloat16 rows were off by 8e-8 of
 // themselves over 512 k, 1.8e-7 over 1,024, 4.1e-7 over 2,048, 1.0e-6 over 4,096, 2.4e-6 over 8,192, and those of float32 rows by as much again
-// for each of their small pieces' products.  So a float32 result's K is summed in runs of up to 48 chunks, which float32
-// additions put together, and the two small pieces of float32 rows have an accumulator of their own.  (bfloat16 results are rounded
-// to 2e-3 behind it.)
+// for each of their small pieces' products.  So K is summed in runs of up to 48 chunks, which float32
+// additions put together, and the two small pieces of float32 rows have an accumulator of their own.  bfloat16 results too, though half a
+// step of theirs is 2e-3 or more: what is cut off has a direction, goes with the largest of the sums on the way (sums over
+// 2^20 k that come back to a thirtieth of it: 3% of the result) and rounds the wrong way (1,029 x [2,056 x 8,192]: 0.14% of the results, in
+// runs 0.05%; 40.4 -> 42.3 us, 2,048 x [8,192 x 8,192] 204 -> 207).  A short K is one run and takes what it took.
 #define W4U_RUN 48
 #define W4U_RAW 4                     // units of a warp's ring of levels (KB 2): two slabs' chunk, their scales
 #define W4U_RAW_SLOT 1152
@@ -382,8 +398,9 @@ struct Ring {
 // issuing warp as much as three MMAs of 64 columns.
 // EPI, BF16: what becomes of the sums, and whether the result is bfloat16 (kernels of their own: with all of them in one, the registers that
 // one wants are spilled by the others, 2,048 rows of a gated 16,384 x 2,048 106 -> 114 us).
-// HANDED: a norm is handed on to it or by it.
-template <bool SPLIT, int PARTS, int KB, int EPI, bool BF16, bool HANDED>
+// HANDED: a norm is handed on to it or by it.  RUNS: K may be more than one run (code that runs once is cold: the bfloat16 results of a short K that
+// carry it take 3% longer, 32 rows, gated 9,216 x 1,024, 4.22 -> 4.35 us).
+template <bool SPLIT, int PARTS, int KB, int EPI, bool BF16, bool HANDED, bool RUNS>
 __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
   constexpr int AHEAD = 4;               // stages (KB 1) whose chunk a warp holds in registers ahead of the one it unpacks
   constexpr bool TMEM = KB == 2;         // weights in tensor memory
@@ -619,7 +636,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   const int quarter = warp & 3, row = quarter * 32 + lane, fifth = epi_warp ? 4 : (warp - 2) >> 2;
   const unsigned tmem_base = tmem_base_s, quarter_base = tmem_base + ((unsigned)(quarter * 32) << 16);
   const int last = SPLIT ? 0 : (total - 1 - first) / step;  // this CTA's last tile
-  const int runs = BF16 || blocks <= a.run ? 1 : (blocks + a.run - 1) / a.run;              // accumulators a tile goes through
+  const int runs = !RUNS || blocks <= a.run ? 1 : (blocks + a.run - 1) / a.run;             // accumulators a tile goes through
   if (HANDED && a.norm.ssq && epi_warp) {                    // (while the others are at work; they see it behind a barrier below)
     pdl_wait();
     const int m = threadIdx.x - 32 * (2 + 8 * SETS);
@@ -629,8 +646,10 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
   auto release = [&](int use) {
     if (lane == 0) mbar_arrive(accempty0 + (a.buffers == 2 ? 8 * (use & 1) : 0));
   };
-  // A tile's sums: the epilogue's warps wait for each of its runs and add the one before to it, whose accumulator is free then.  The other
+  // A tile's sums: the epilogue's warps wait for each of its runs and add the one before to it, whose accumulator is free then; of the CTA's last
+  // tile the last two stay apart, and whoever finishes a column adds them.  The other
   // warps go on when those have seen the last run (they are not there for every phase of its barrier).
+  auto before = [&](int tile) { return !RUNS || runs == 1 || tile < last ? 0u : where(tile * runs + runs - 2) - where(tile * runs + runs - 1); };
   auto tile_ready = [&](int tile, bool everyone) {
     if (epi_warp) {
       for (int r = 0; r < runs; ++r) {
@@ -638,7 +657,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         W4U_WAIT_EPILOGUE(accfull0 + (a.buffers == 2 ? 8 * (use & 1) : 0), (a.buffers == 2 ? use >> 1 : use) & 1);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         __syncwarp();
-        if (!BF16 && r > 0) {
+        if (RUNS && r > 0 && !(everyone && r == runs - 1)) {
           for (int c = 0; c < a.bn; c += 16) {
             tmem_add16(where(use) + c, where(use - 1) + c);
             if (PARTS == 3) tmem_add16(where(use) + lo_cols + c, where(use - 1) + lo_cols + c);
@@ -662,8 +681,8 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     for (int tile = epi_warp ? 0 : last; tile <= last; ++tile) {
       const int t = first + tile * step, use = tile * runs + runs - 1, groups = a.bn / 16;
       const int m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
-      const unsigned from = where(use);
-      finish_columns<EPI, BF16, HANDED, 16>(a, row_factor, [&]() { tile_ready(tile, tile == last); }, [&](int c, float* v) { tmem_sums<16>(from + c, lo_cols, v); },
+      const unsigned from = where(use), also = before(tile);
+      finish_columns<EPI, BF16, HANDED, 16>(a, row_factor, [&]() { tile_ready(tile, tile == last); }, [&](int c, float* v) { tmem_sums<16>(from + c, lo_cols, also, v); },
                                             tile < last ? 0 : groups * fifth / 5 * 16, tile < last ? a.bn : groups * (fifth + 1) / 5 * 16, m0, n);
       if (tile < last) {
         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -677,7 +696,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
     // warp's store is 512 bytes in a row (16 bytes here and there took ten times as long: they travel one by one).
     const int t = first, m0 = (t % m_tiles) * a.bn, n = (t / m_tiles) * 128 + row;
     const int share = a.share, groups = share / 4, c0 = rank * share;
-    const unsigned from = where(runs - 1);
+    const unsigned from = where(runs - 1), also = before(0);
     const unsigned recv = a.recv_apart ? tiles + (unsigned)a.stages * stage_bytes : tiles;
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");         // every rank has started: its memory is there
     if (warp < 2) {
@@ -692,7 +711,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         if (!a.recv_apart) cluster_sync();                                        // every rank's MMAs have read their stages
         for (int c = fifth * 16; c < a.bn && m0 + c < a.M; c += 5 * 16) {
           float v[16];
-          tmem_sums<16>(from + c, lo_cols, v);
+          tmem_sums<16>(from + c, lo_cols, also, v);
           int owner = (c >> 2) / groups, group = (c >> 2) - owner * groups;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -705,7 +724,7 @@ __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __gr
         cluster_sync();
       }, [&](int c, float* v) {
         float own[4];
-        tmem_sums<4>(from + c, lo_cols, own);
+        tmem_sums<4>(from + c, lo_cols, also, own);
         const float4* part = mine + (c - c0) / 4 * 128;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int r = 0; r < a.splits; ++r) {                 // (in the ranks' order)
@@ -746,7 +765,7 @@ static int clusters_at_once(int splits) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!cache[dev][splits]) {
     const size_t smem = 221 * 1024;
-    auto kern = gemm_w4_umma_kernel<true, 1, 1, W4_STORE, true, false>;
+    auto kern = gemm_w4_umma_kernel<true, 1, 1, W4_STORE, true, false, false>;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess) {
       cudaLaunchConfig_t cfg = {};
@@ -762,18 +781,24 @@ static int clusters_at_once(int splits) {
   return cache[dev][splits];
 }
 
-template <int EPI, bool BF16, int PARTS, int KB, bool HANDED>
+template <int EPI, bool BF16, int PARTS, int KB, bool HANDED, bool RUNS>
 static int launch_tiles_of(const CUtensorMap& map, const W4uArgs& a, int grid, size_t smem, cudaStream_t stream) {
-  auto kern = a.splits > 1 ? gemm_w4_umma_kernel<true, PARTS, KB, EPI, BF16, HANDED> : gemm_w4_umma_kernel<false, PARTS, KB, EPI, BF16, HANDED>;
+  auto kern = a.splits > 1 ? gemm_w4_umma_kernel<true, PARTS, KB, EPI, BF16, HANDED, RUNS> : gemm_w4_umma_kernel<false, PARTS, KB, EPI, BF16, HANDED, RUNS>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   return launch_k_class(1, kern, dim3(grid, 1, 1), dim3(W4U_THREADS, 1, 1), smem, stream, a.splits, map, a);
 }
-template <int EPI, bool BF16>
+template <int EPI, bool BF16, bool RUNS>
 static int launch_tiles(const CUtensorMap& map, const W4uArgs& a, int parts, int kb, int grid, size_t smem, cudaStream_t stream) {
-  if (parts == 3) return BF16 ? FELLM_ERR_ARG : launch_tiles_of<EPI, false, 3, 1, false>(map, a, grid, smem, stream);      // (float32 rows make float32 results)
-  if (a.norm.next_x || a.norm.ssq) return launch_tiles_of<EPI, BF16, 1, 2, true>(map, a, grid, smem, stream);      // (up to 128 rows)
-  return kb == 2 ? launch_tiles_of<EPI, BF16, 1, 2, false>(map, a, grid, smem, stream) : launch_tiles_of<EPI, BF16, 1, 1, false>(map, a, grid, smem, stream);
+  if (parts == 3) return BF16 ? FELLM_ERR_ARG : launch_tiles_of<EPI, false, 3, 1, false, true>(map, a, grid, smem, stream);      // (float32 rows make float32 results)
+  if (a.norm.next_x || a.norm.ssq) return launch_tiles_of<EPI, BF16, 1, 2, true, RUNS>(map, a, grid, smem, stream);      // (up to 128 rows)
+  return kb == 2 ? launch_tiles_of<EPI, BF16, 1, 2, false, RUNS>(map, a, grid, smem, stream) : launch_tiles_of<EPI, BF16, 1, 1, false, RUNS>(map, a, grid, smem, stream);
+}
+template <int EPI>
+static int launch_result(bool to_bf16, int runs, const CUtensorMap& map, const W4uArgs& a, int parts, int kb, int grid, size_t smem, cudaStream_t stream) {
+  if (!to_bf16) return launch_tiles<EPI, false, true>(map, a, parts, kb, grid, smem, stream);
+  if constexpr (EPI == W4_ACC) return FELLM_ERR_ARG;
+  else return runs > 1 ? launch_tiles<EPI, true, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<EPI, true, false>(map, a, parts, kb, grid, smem, stream);
 }
 
 // x that TMA cannot read as it is (float32, or rows that are not on 16 bytes) is copied into `scratch` first: M x chunks x 64 numbers of
@@ -826,7 +851,7 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   a.share = ceil_div(a.bn / 4, a.splits) * 4;
   const int room = 220 * 1024 - raw, recv = (a.splits - 1) * a.share * 512;
   const int blocks = ceil_div(ceil_div(chunks, kb), a.splits) * parts;
-  const int runs = to_bf16 ? 1 : ceil_div(blocks, W4U_RUN / kb * parts);
+  const int runs = ceil_div(blocks, W4U_RUN / kb * parts);
   a.run = ceil_div(blocks / parts, runs) * parts;
   a.acc_cols = 16;
   while (a.acc_cols < a.bn) a.acc_cols *= 2;
@@ -853,9 +878,9 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   const size_t smem = (size_t)a.raw_at + raw + 1024;
   const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
   switch (flags & W4_EPI) {
-    case W4_ACC: return to_bf16 ? FELLM_ERR_ARG : launch_tiles<W4_ACC, false>(map, a, parts, kb, grid, smem, stream);
-    case W4_SWIGLU: return to_bf16 ? launch_tiles<W4_SWIGLU, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<W4_SWIGLU, false>(map, a, parts, kb, grid, smem, stream);
-    case W4_RELU2: return to_bf16 ? launch_tiles<W4_RELU2, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<W4_RELU2, false>(map, a, parts, kb, grid, smem, stream);
-    default: return to_bf16 ? launch_tiles<W4_STORE, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<W4_STORE, false>(map, a, parts, kb, grid, smem, stream);
+    case W4_ACC: return launch_result<W4_ACC>(to_bf16, runs, map, a, parts, kb, grid, smem, stream);
+    case W4_SWIGLU: return launch_result<W4_SWIGLU>(to_bf16, runs, map, a, parts, kb, grid, smem, stream);
+    case W4_RELU2: return launch_result<W4_RELU2>(to_bf16, runs, map, a, parts, kb, grid, smem, stream);
+    default: return launch_result<W4_STORE>(to_bf16, runs, map, a, parts, kb, grid, smem, stream);
   }
 }
