@@ -7,6 +7,11 @@
 // is made by itself and joins the total times its scale, in float32.  The shares of a slab's warps are added in shared memory,
 // in one order.
 //
+// A group's G products of x with levels can be 8 G times as large as x, which may be no float32 number although the result, with the scales in it,
+// is one.  So the levels are unpacked as q / (8 G), exact and at no cost (the constants have other exponents): no group's sum is above the largest x,
+// and none too small to be kept (x is a multiple of 2^-133, the products of 2^-143).  The total is in the same unit and leaves it at
+// the end: what it loses by that lies below 2^-140.
+//
 // Bound by the matrix's bytes where enough of them are on their way and by the instructions that unpack them: an SM's four
 // schedulers have some 86 cycles each for a chunk that memory delivers.  So every warp keeps three units (6.8 KB) in flight through
 // a ring of its own in shared memory (cp.async: no registers are held, and the ring runs on over the end of a slab), and what
@@ -222,7 +227,7 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
           for (int j = 0; j < 2; ++j) {
             unsigned w[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[r] = w4_pair(word[2 * h + j], r);
+            for (int r = 0; r < 4; ++r) w[r] = w4_pair<GS + 3>(word[2 * h + j], r);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -293,6 +298,7 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
       const float* p = red + ((size_t)(turn * warps + warp - sub) * COLS + t) * (ROWS + 1) + i % ROWS;
       float v = 0.f;
       for (int w = 0; w < seg.share; ++w) v += p[w * COLS * (ROWS + 1)];
+      v *= (float)(1 << (GS + 3));
       if (HANDED && a.norm.ssq) v *= row_factor[t];
       if (a.bias && n < a.w.N) v += a.bias[n];
       if (HANDED && a.norm.next_x) {                                   // (out += ..; N is a multiple of 16: a half warp is a row's slab)

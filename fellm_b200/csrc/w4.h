@@ -41,23 +41,24 @@ struct W4Norm {
   const float* ssq; int parts; float eps;
 };
 
-// (One three-input operation: written as an and with a constant and an or with another it becomes two.)
-__device__ __forceinline__ unsigned w4_pair_biased(unsigned word, int r) {
+// The r-th pair of a word as 2^-DOWN (16 + q + 8).  (One three-input operation: written as an and with a constant and an or with another it
+// becomes two.)
+template <int DOWN> __device__ __forceinline__ unsigned w4_pair_biased(unsigned word, int r) {
   unsigned v;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(v) : "r"(__funnelshift_r(word, word, 4 * r)), "r"(0x00780078u), "r"(0x41804180u));
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(v) : "r"(__funnelshift_r(word, word, 4 * r)), "r"(0x00780078u), "r"(0x41804180u - DOWN * 0x00800080u));
   return v;
 }
-// minus 24: the levels themselves, exactly.
+// minus 24 of it: 2^-DOWN times the levels themselves, exactly.
 #define W4_MINUS_24 0xc1c0c1c0u
-__device__ __forceinline__ unsigned w4_pair(unsigned word, int r) {
-  const unsigned b = w4_pair_biased(word, r), off = W4_MINUS_24;
+template <int DOWN> __device__ __forceinline__ unsigned w4_pair(unsigned word, int r) {
+  const unsigned b = w4_pair_biased<DOWN>(word, r), off = W4_MINUS_24 - DOWN * 0x00800080u;
   __nv_bfloat162 v = __hadd2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&off);
   return *(unsigned*)&v;
 }
 // The r-th pair of a word times its scale (s2: in both halves; off2: times -24 of it): (16 + q + 8) s - 24 s in one fused operation, exact,
 // since 24 s and the result are bfloat16 numbers.
 __device__ __forceinline__ unsigned w4_value(unsigned word, int r, unsigned s2, unsigned off2) {
-  const unsigned b = w4_pair_biased(word, r);
+  const unsigned b = w4_pair_biased<0>(word, r);
   __nv_bfloat162 v = __hfma2(*(const __nv_bfloat162*)&b, *(const __nv_bfloat162*)&s2, *(const __nv_bfloat162*)&off2);
   return *(unsigned*)&v;
 }
