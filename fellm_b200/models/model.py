@@ -308,8 +308,9 @@ class Model:
             block.join_inputs()
 
     def quantize(self, group: int):
-        """After bind(): every matrix that is only multiplied with rows of activations (parts say which: Part.four_bit), the
-        embedding and the head, in four bits.  Experts, convolutions, norms, routers and what a kernel of a mixer reads stay."""
+        """After bind(): the matrices that are only multiplied with rows of activations (parts say which: Part.four_bit), the
+        embedding and the head, in four bits.  Experts, convolutions, norms and what a kernel of a mixer reads stay, and the few rows that make
+        logits of routers, decays, write strengths and gates a head or the factors of a low-rank decay or gate."""
         for block in self.blocks:
             block.quantize(group)
         tied = getattr(self.head, "tied", False)

@@ -105,7 +105,8 @@ class Part:
     def prepare(self):
         """Called once after bind(): repack or fuse weights for the kernels."""
 
-    four_bit = ()          # names in self.w, after prepare(), of the matrices that forward() hands to linear() and nothing else
+    four_bit = ()          # names in self.w, after prepare(), of the matrices (or rows of one) that quantize() brings into four bits: what is
+    #                        only handed to linear(), without the logits of decays, write strengths, routers and gates a head, which are few rows
 
     def quantize(self, group: int):
         """The matrices named `four_bit` in four bits (ops.quantize_w4), groups of `group` elements of a row.  Called once, after

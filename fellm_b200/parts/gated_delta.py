@@ -88,7 +88,8 @@ class GatedDelta(Mixer):
 
     def prepare(self):
         """Every projection that reads the mixer's input is one product: [q; k; v; (g); b; a or a1; (g1)], stored in
-        float32 (the logits of beta and of the decay must not be rounded, and one launch is cheaper than two)."""
+        float32 (the logits of beta and of the decay must not be rounded, and one launch is cheaper than two).  In four bits they
+        are two (quantize())."""
         w = self.w
         G, H, dk, dv = self.G, self.H, self.dk, self.dv
         self.n_conv = 2 * G * dk + H * dv
@@ -117,9 +118,29 @@ class GatedDelta(Mixer):
         w["in.weight"], offs = stack_rows(mats)
         self.off = dict(zip(names, offs))
         self.rows = {n: m.shape[0] for n, m in zip(names, mats)}
+        w["qkvg.weight"] = w["in.weight"][:self.off["b"]]        # (a view: the rows that quantize() puts in four bits)
+        self.logits_off = self.off                               # columns of b, a or a1 and g1 in what _inputs() returns last
         w["taps"] = torch.cat([w.pop("q.conv"), w.pop("k.conv"), w.pop("v.conv")], 0).contiguous()
 
-    four_bit = ("in.weight", "o.weight")
+    four_bit = ("qkvg.weight", "o.weight")
+
+    def quantize(self, group: int):
+        """q, k, v and a whole gate in four bits.  The logits of beta and of the decay and the low-rank factors stay, in a product of their own: they are
+        few rows, and an error of a decay grows over the whole context."""
+        w, n = self.w, self.off["b"]
+        whole = w.pop("in.weight")
+        w["qkvg.weight"], w["logits.weight"] = _pad_rows(whole[:n]), _pad_rows(whole[n:]).clone()      # (of memory of its own)
+        self.logits_off = {name: at - n for name, at in self.off.items() if at >= n}
+        super().quantize(group)
+
+    def _inputs(self, xn):
+        """The input's projections, float32: [T, q | k | v | (g) ..] and [T, .. b | a or a1 | (g1)], which are one product unless quantize() has
+        taken them apart."""
+        w = self.w
+        if "in.weight" in w:
+            p = linear(xn, w["in.weight"], out_dtype=torch.float32)
+            return p, p
+        return linear(xn, w["qkvg.weight"], out_dtype=torch.float32), linear(xn, w["logits.weight"], out_dtype=torch.float32)
 
     def cache_need(self):
         return [FixedState((self.taps - 1, 2 * self.G * self.dk + self.H * self.dv)),
@@ -129,29 +150,30 @@ class GatedDelta(Mixer):
         if reads_only:
             raise ConfigError("a gated_delta layer cannot run on another layer's state")
         conv_state, mat_state = cache
-        w, off = self.w, self.off
+        w, off, small_off = self.w, self.off, self.logits_off
         H, G, dk, dv = self.H, self.G, self.dk, self.dv
-        p = linear(xn, w["in.weight"], out_dtype=torch.float32)            # [T, q | k | v | (g) | b | a or a1 | (g1)] float32
+        p, small = self._inputs(xn)
         qkv = ops.causal_conv_act(p[:, :self.n_conv], w["taps"], conv_state.states, ctx.item_start,
                                   conv_state.item_slot, ctx.n_items, ctx.max_item_rows, act="silu")
         gch = None
         if self.decay == "channel":
-            gch = ops.lowrank_expand(p[:, off["a"]:off["a"] + self.rows["a"]], w["a2.weight"], w["dt_bias"],
+            gch = ops.lowrank_expand(small[:, small_off["a"]:small_off["a"] + self.rows["a"]], w["a2.weight"], w["dt_bias"],
                                      f_out="decay_softplus", rate=w["A_log"], per=dk)
-        o = ops.delta_scan(qkv, off["k"], off["v"], p, off["b"], off["a"], w["A_log"],
+        o = ops.delta_scan(qkv, off["k"], off["v"], small, small_off["b"], small_off["a"], w["A_log"],
                            None if gch is not None else w["dt_bias"], gch, mat_state.states, ctx.item_start,
                            mat_state.item_slot, ctx.n_items, H, G, dk, dv, max_item_rows=ctx.max_item_rows,
                            chunk_rows=ops.recurrent_chunk_rows(xn.dtype, xn.shape[0], ctx.n_items, ctx.max_item_rows, dk))
         if self.gate == "silu":
             gate, act = p[:, off["g"]:off["g"] + H * dv], "silu"
         else:
-            gate, act = ops.lowrank_expand(p[:, off["g"]:off["g"] + self.rows["g"]], w["g2.weight"]), "sigmoid"
+            gate, act = ops.lowrank_expand(small[:, small_off["g"]:small_off["g"] + self.rows["g"]], w["g2.weight"]), "sigmoid"
         y = ops.head_norm_gate(o, w["norm.weight"], False, gate, act, self.eps, H, dv, xn.dtype)
         linear(y, w["o.weight"], out=out, accumulate=True)
         return out
 
     def weight_order(self):
-        return [self.w["in.weight"], self.w["o.weight"]]
+        w = self.w
+        return ([w["in.weight"]] if "in.weight" in w else [w["qkvg.weight"], w["logits.weight"]]) + [w["o.weight"]]
 
     def kernel_modules(self, dtype):
         return linear_modules(dtype) + [("recurrent", None)] + ([("recurrent_chunk", None)] if dtype == "bfloat16" else [])
