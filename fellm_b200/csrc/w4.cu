@@ -10,14 +10,14 @@ __device__ __forceinline__ float round5(float a) {
   return __uint_as_float(u & 0xfff80000u);
 }
 
-// A group's scale from its largest and smallest element: an eighth of the largest magnitude, in five significant bits,
-// negative where that magnitude is a positive element's (so that the extreme is level -8, not the missing +8).  Below the
+// A group's scale from its largest and smallest element: an eighth of the largest magnitude, in five significant bits (taken before the
+// division, which is exact: behind it a number below the normal ones would have fewer), negative where that magnitude is a positive element's
+// (so that the extreme is level -8, not the missing +8).  Below the
 // normal numbers: 0, the group is zeros.  Not above 31 * 2^118: 24 s has to stay
 // finite, with which the weights are made bfloat16 numbers.  NaN where an element is not finite.
 __device__ __forceinline__ float group_scale(float hi, float lo, bool finite) {
   if (!finite) return __uint_as_float(0x7fc00000u);
-  const float a = fmaxf(hi, -lo) * 0.125f;
-  float s = fminf(round5(a), __uint_as_float(0x7cf80000u));
+  float s = fminf(round5(fmaxf(hi, -lo)) * 0.125f, __uint_as_float(0x7cf80000u));
   if (s < 1.1754943508222875e-38f) s = 0.f;
   return hi > -lo ? -s : s;
 }
