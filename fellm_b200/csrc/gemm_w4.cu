@@ -318,7 +318,7 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
       }
       if (a.epi == W4_SWIGLU) {
         const float up = __shfl_down_sync(0xffffffffu, v, 8);
-        if (r < 8 && t < cols && n < a.w.N) put(a, m, slab * 8 + r, glu_act(v, up, 0.f, 1.f));
+        if (r < 8 && t < cols && n < a.w.N) put(a, m, slab * 8 + r, w4_silu_mul(v, up));
       } else if (t < cols && n < a.w.N) put(a, m, n, v);
     }
   }

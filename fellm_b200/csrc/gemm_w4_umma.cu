@@ -224,10 +224,6 @@ __device__ __forceinline__ uint4 ld_shared_v4(unsigned addr) {
 }
 __device__ __forceinline__ void copy16(unsigned dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory"); }
 
-// SiLU(g) * u for a bfloat16 result: the approximate exponential and quotient are off by some 2^-20, a three-hundredth of the rounding
-// behind them, and take a fifth of the instructions (2,048 rows, 16,384 x 2,048: the epilogue took longer than the MMAs of a tile).
-__device__ __forceinline__ float silu_mul_fast(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
-
 // Neighbouring lanes, features n and n + 1, hold columns x and y each: the even one stores both features of x, the odd one of y.
 template <bool BF16> __device__ __forceinline__ void store_pair(unsigned char* p, float x, float y, int hi, bool in) {
   if (BF16) {
@@ -263,7 +259,7 @@ __device__ __forceinline__ void finish_some(const W4uArgs& a, float* v, int m, i
 #pragma unroll
     for (int j = 0; j < COLS; j += 2) {
       const float other = __shfl_xor_sync(0xffffffffu, gate ? v[j + 1] : v[j], 8), g = gate ? v[j] : other, u = gate ? other : v[j + 1];
-      z[j >> 1] = BF16 ? silu_mul_fast(g, u) : glu_act(g, u, 0.f, 1.f);
+      z[j >> 1] = BF16 ? w4_silu_mul_fast(g, u) : w4_silu_mul(g, u);
     }
     if (pairs) {
       const int first = odd + 2 * hi;                        // this lane's column of the first four

@@ -94,6 +94,25 @@ static inline int w4_check_epi(int flags, int N) {
   return epi == W4_SWIGLU && N % W4_SLAB ? FELLM_ERR_SIZE : 0;
 }
 
+// SiLU(g) * u with t = exp(-|g|), which is finite and whose denominator is between 1 and 2 for every g: g / (1 + exp(-g)) is 0 from g = -88.7 on, where
+// exp(-g) is no float32 number, the function down to -103 is not.
+__device__ __forceinline__ float w4_silu_mul(float g, float u) {
+  const float t = expf(-fabsf(g));
+  return (g < 0.f ? g * t : g) / (1.0f + t) * u;
+}
+// The same for a bfloat16 result, by the approximate exponential and reciprocal: 2^-24 (1 + exp(-g)), with the exponential as a square, is finite and has
+// a reciprocal down to g = -104, where the function goes below all numbers.  Both are good to 2^-22 and the exponential's argument adds 2^-24 of itself: 2^-20
+// for small gates, 2^-18 at -16, 2^-16 at -88 beside half a step of 2^-9 or more (a gate counts down to 2^-126).  Two operations more than
+// g / (1 + exp(-g)) by the same means, which is 0 from g = -87.3 on; a fifth of w4_silu_mul's (2,048 rows, 16,384 x 2,048: with that the epilogue takes longer
+// than the MMAs of a tile).
+__device__ __forceinline__ float w4_silu_mul_fast(float g, float u) {
+  const float unit = 5.9604644775390625e-8f;                // 2^-24
+  float h, r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(h) : "f"(g * -0.72134752044448170f));
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(fmaf(h * unit, h, unit)));
+  return g * unit * r * u;
+}
+
 // Rows of x as a product wants them where it cannot read them as they are: bfloat16 rows on no 16-byte boundary or of a K that is no
 // multiple of 8 (copied, zeros up to whole chunks), and float32 rows, every 64 elements of which become three times 64 bfloat16 whose sum
 // they are, the smallest first.
