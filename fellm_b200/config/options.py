@@ -18,8 +18,6 @@ class EngineOptions:
     n_ctx 8192 clamped to the model's maximum (0 = the model's maximum), n_batch = tokens a
     scheduler iteration may run, n_ubatch = the longest portion of one prompt in a step."""
     dtype: str = "bfloat16"
-    weights: str = "kept"           # "kept": matrices as the loader keeps them; "int4": the large ones in four bits (Model.quantize)
-    weight_group: int = 64          # elements of a row that share a scale ("int4")
     n_ctx: int = 8192
     n_batch: int = 2048
     n_ubatch: int = 512
@@ -31,6 +29,8 @@ class EngineOptions:
     kv_device_budget: int = 0           # bytes of cache pages when max_tokens is None; 0 = from free memory (FeLLM's --kv-device-budget)
     cuda_graphs: bool = True
     device: str = "cuda:0"
+    weights: str = "kept"           # "kept": matrices as the loader keeps them; "int4": the large ones in four bits (Model.quantize)
+    weight_group: int = 64          # elements of a row that share a scale ("int4")
 
     def validate(self):
         if self.dtype not in DTYPES:
