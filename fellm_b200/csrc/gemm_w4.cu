@@ -24,6 +24,7 @@
 
 #define GW_DEPTH 4                     // units of a warp's ring: one is used, the others are on their way
 #define GW_SLOT (4 * (512 + 64))       // a unit: four chunks' levels, their groups' scales (eight at groups of 32)
+#define GW_BUFFERS 2                   // for the warps' shares, in turn, so that one barrier a segment is enough
 
 enum { X_BF16 = 0, X_BF16_ANY = 1, X_F32 = 2, X_CUT = 3 };       // rows on 16 bytes and K a multiple of 8; any bfloat16; float32; float32 cut by w4_rows_kernel
 
@@ -128,9 +129,6 @@ __device__ __forceinline__ Segment next_segment(int slab, int left, int warp, in
   return s;
 }
 
-// Buffers for the warps' shares: two in turn, so that one barrier is enough, or one and a barrier more (two blocks an SM have to fit).
-__host__ __device__ constexpr int rows_buffers(int nt) { return nt < 4 ? 2 : 1; }
-
 // XT: what x is.  NT: tiles of eight rows of x.  GS: log2 of the group.  R: neighbouring slabs a warp takes together (a "slab" below is
 // R of them, a unit 4 / R chunks of each): the same columns' operands for both.  HANDED: a norm is handed on to it or by it (a kernel of its
 // own: carried by every product, its code cost 4% where it does not run).
@@ -142,7 +140,7 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
   const int all_slabs = (a.w.N + W4_SLAB - 1) / W4_SLAB, slabs = (all_slabs + R - 1) / R, m0 = blockIdx.y * COLS, cols = min(a.M - m0, COLS);
   const int first = (int)blockIdx.x * a.per_block + min((int)blockIdx.x, a.over), end = first + a.per_block + ((int)blockIdx.x < a.over ? 1 : 0);
   const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * GW_DEPTH * GW_SLOT;
-  float* red = reinterpret_cast<float*>(smem + (size_t)warps * GW_DEPTH * GW_SLOT);      // [buffers][warps][COLS][ROWS + 1]
+  float* red = reinterpret_cast<float*>(smem + (size_t)warps * GW_DEPTH * GW_SLOT);      // [GW_BUFFERS][warps][COLS][ROWS + 1]
   const int units = (a.w.chunks + UNIT - 1) / UNIT;
   constexpr int SCALES = (UNIT * W4_CHUNK) >> GS;           // groups a unit
   // what is fetched next: of which segment, how many units are left of it (a unit that ends behind the slab's last chunk takes what lies
@@ -198,7 +196,7 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
   for (int t = 0; t < NT; ++t) xrow[t] = (const unsigned char*)a.x + (size_t)(m0 + min(8 * t + g, cols - 1)) * a.ldx * XB + c * 8 * XB;
   unsigned at = ring;
   int turn = 0;
-  for (int next = first; next < end; turn ^= rows_buffers(NT) - 1) {
+  for (int next = first; next < end; turn ^= 1) {
     const Segment seg = next_segment(next, end - next, warp, warps, units);
     next += seg.t;
     float total[R][NT][4], part[R][NT][4];
@@ -271,7 +269,6 @@ __maxnreg__(128) __global__ void gemm_w4_rows_kernel(GwArgs a) {
       at = at == ring + (GW_DEPTH - 1) * GW_SLOT ? ring : at + GW_SLOT;
     }
     // the warps' shares together
-    if (rows_buffers(NT) == 1) __syncthreads();
     float* mine = red + ((size_t)(turn * warps + warp) * COLS) * (ROWS + 1);
 #pragma unroll
     for (int k = 0; k < R; ++k)
@@ -328,7 +325,7 @@ template <int XT, int NT, int GS, int R, bool HANDED>
 static int launch_rows(GwArgs a, cudaStream_t stream) {
   const int slabs = ceil_div(ceil_div(a.w.N, W4_SLAB), R), units = ceil_div(a.w.chunks, 4 / R), n_sm = fellm_sm_count(), tiles = ceil_div(a.M, 8 * NT);
   auto kern = gemm_w4_rows_kernel<XT, NT, GS, R, HANDED>;
-  auto bytes = [](int warps) { return (size_t)warps * (GW_DEPTH * GW_SLOT + rows_buffers(NT) * 8 * NT * (R * W4_SLAB + 1) * 4); };
+  auto bytes = [](int warps) { return (size_t)warps * (GW_DEPTH * GW_SLOT + GW_BUFFERS * 8 * NT * (R * W4_SLAB + 1) * 4); };
   static int asked[64];                                 // blocks of eight warps an SM holds, asked once a device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FELLM_ERR_ARG;

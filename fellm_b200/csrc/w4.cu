@@ -44,27 +44,19 @@ __device__ __forceinline__ unsigned level_of(float w, float s, float inv) {
 }
 
 // What lane (g, c) keeps of two chunks: rows g, g + 8 x quarters of 32 elements x its eight.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, bool row_ok, int k, int K, bool vec, float* v) {
+__device__ __forceinline__ void load8(const float* row, bool row_ok, int k, int K, bool vec, float* v) {
   if (!row_ok) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.f;
     return;
   }
   if (vec && k + 8 <= K) {
-    if (sizeof(T) == 2) {
-      const uint4 x = *(const uint4*)((const bf16*)row + k);
-      const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-    } else {
-      const float4 x = *(const float4*)((const float*)row + k), y = *(const float4*)((const float*)row + k + 4);
-      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-    }
+    const float4 x = *(const float4*)(row + k), y = *(const float4*)(row + k + 4);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f(row[k + i]) : 0.f;
+  for (int i = 0; i < 8; ++i) v[i] = k + i < K ? row[k + i] : 0.f;
 }
 // Two rows' eight levels (0..15 each) of a half chunk -> the two words of w4.h.
 __device__ __forceinline__ unsigned pack_word(const unsigned* a, const unsigned* b) {
@@ -288,18 +280,12 @@ __device__ __forceinline__ void row8(const W4Ref& m, int row, int k, float* v) {
     v[4 * i + 3] = s * (float)((int)(u >> 24 & 15u) - 8);
   }
 }
+// (whole pieces of bfloat16 do not come here: dequantize_w4_kernel has them as they are)
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* v, int left, bool vec) {
-  if (vec && left >= 8) {
-    if (sizeof(T) == 2) {
-      unsigned w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); w[i] = *(unsigned*)&b; }
-      *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
-      *(float4*)((float*)p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    }
+  if (sizeof(T) == 4 && vec && left >= 8) {
+    *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+    *(float4*)((float*)p + 4) = make_float4(v[4], v[5], v[6], v[7]);
     return;
   }
 #pragma unroll

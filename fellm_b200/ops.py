@@ -2013,17 +2013,11 @@ class W4:
 
     def __init__(self, q, scales, N: int, K: int, group: int):
         self.q, self.scales, self.shape, self.group = q, scales, (N, K), group
-        self.device, self.is_cuda = q.device, q.is_cuda
+        self.device = q.device
         self._device = q.get_device()
         chunks = -(-K // 64)
         self._ref = _W4Ref(q.data_ptr(), scales.data_ptr(), N, K, chunks, -(-chunks * 64 // group), group.bit_length() - 1)
         self._at = ctypes.addressof(self._ref)
-
-    def nbytes(self) -> int:
-        return 4 * (self.q.numel() + self.scales.numel())
-
-    def data_ptr(self) -> int:
-        return self.q.data_ptr()
 
 
 def _w4_dev(*tensors):
