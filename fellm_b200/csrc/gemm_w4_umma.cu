@@ -394,8 +394,8 @@ struct Ring {
 // issuing warp as much as three MMAs of 64 columns.
 // EPI, BF16: what becomes of the sums, and whether the result is bfloat16 (kernels of their own: with all of them in one, the registers that
 // one wants are spilled by the others, 2,048 rows of a gated 16,384 x 2,048 106 -> 114 us).
-// HANDED: a norm is handed on to it or by it.  RUNS: K may be more than one run (code that runs once is cold: the bfloat16 results of a short K that
-// carry it take 3% longer, 32 rows, gated 9,216 x 1,024, 4.22 -> 4.35 us).
+// HANDED: a norm is handed on to it or by it.  RUNS: K is more than one run (code that runs once is cold: a product of a short K that
+// carries it takes 3% longer, 32 rows, gated 9,216 x 1,024, 4.22 -> 4.35 us).
 template <bool SPLIT, int PARTS, int KB, int EPI, bool BF16, bool HANDED, bool RUNS>
 __global__ void __launch_bounds__(W4U_THREADS, 1) gemm_w4_umma_kernel(const __grid_constant__ CUtensorMap map_x, W4uArgs a) {
   constexpr int AHEAD = 4;               // stages (KB 1) whose chunk a warp holds in registers ahead of the one it unpacks
@@ -786,15 +786,13 @@ static int launch_tiles_of(const CUtensorMap& map, const W4uArgs& a, int grid, s
 }
 template <int EPI, bool BF16, bool RUNS>
 static int launch_tiles(const CUtensorMap& map, const W4uArgs& a, int parts, int kb, int grid, size_t smem, cudaStream_t stream) {
-  if (parts == 3) return BF16 ? FELLM_ERR_ARG : launch_tiles_of<EPI, false, 3, 1, false, true>(map, a, grid, smem, stream);      // (float32 rows make float32 results)
+  if (parts == 3) return BF16 ? FELLM_ERR_ARG : launch_tiles_of<EPI, false, 3, 1, false, RUNS>(map, a, grid, smem, stream);      // (float32 rows make float32 results)
   if (a.norm.next_x || a.norm.ssq) return launch_tiles_of<EPI, BF16, 1, 2, true, RUNS>(map, a, grid, smem, stream);      // (up to 128 rows)
   return kb == 2 ? launch_tiles_of<EPI, BF16, 1, 2, false, RUNS>(map, a, grid, smem, stream) : launch_tiles_of<EPI, BF16, 1, 1, false, RUNS>(map, a, grid, smem, stream);
 }
-template <int EPI>
-static int launch_result(bool to_bf16, int runs, const CUtensorMap& map, const W4uArgs& a, int parts, int kb, int grid, size_t smem, cudaStream_t stream) {
-  if (!to_bf16) return launch_tiles<EPI, false, true>(map, a, parts, kb, grid, smem, stream);
-  if constexpr (EPI == W4_ACC) return FELLM_ERR_ARG;
-  else return runs > 1 ? launch_tiles<EPI, true, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<EPI, true, false>(map, a, parts, kb, grid, smem, stream);
+template <int EPI, bool BF16>
+static int launch_runs(int runs, const CUtensorMap& map, const W4uArgs& a, int parts, int kb, int grid, size_t smem, cudaStream_t stream) {
+  return runs > 1 ? launch_tiles<EPI, BF16, true>(map, a, parts, kb, grid, smem, stream) : launch_tiles<EPI, BF16, false>(map, a, parts, kb, grid, smem, stream);
 }
 
 // x that TMA cannot read as it is (float32, or rows that are not on 16 bytes) is copied into `scratch` first: M x chunks x 64 numbers of
@@ -874,9 +872,9 @@ FELLM_API int fellm_gemm_w4_umma(const void* x, long long ldx, const W4Ref* w, c
   const size_t smem = (size_t)a.raw_at + raw + 1024;
   const int grid = a.splits > 1 ? total * a.splits : (total < n_sm ? total : n_sm);
   switch (flags & W4_EPI) {
-    case W4_ACC: return launch_result<W4_ACC>(to_bf16, runs, map, a, parts, kb, grid, smem, stream);
-    case W4_SWIGLU: return launch_result<W4_SWIGLU>(to_bf16, runs, map, a, parts, kb, grid, smem, stream);
-    case W4_RELU2: return launch_result<W4_RELU2>(to_bf16, runs, map, a, parts, kb, grid, smem, stream);
-    default: return launch_result<W4_STORE>(to_bf16, runs, map, a, parts, kb, grid, smem, stream);
+    case W4_ACC: return to_bf16 ? FELLM_ERR_ARG : launch_runs<W4_ACC, false>(runs, map, a, parts, kb, grid, smem, stream);
+    case W4_SWIGLU: return to_bf16 ? launch_runs<W4_SWIGLU, true>(runs, map, a, parts, kb, grid, smem, stream) : launch_runs<W4_SWIGLU, false>(runs, map, a, parts, kb, grid, smem, stream);
+    case W4_RELU2: return to_bf16 ? launch_runs<W4_RELU2, true>(runs, map, a, parts, kb, grid, smem, stream) : launch_runs<W4_RELU2, false>(runs, map, a, parts, kb, grid, smem, stream);
+    default: return to_bf16 ? launch_runs<W4_STORE, true>(runs, map, a, parts, kb, grid, smem, stream) : launch_runs<W4_STORE, false>(runs, map, a, parts, kb, grid, smem, stream);
   }
 }
