@@ -2,13 +2,13 @@
 // MMA's 128 rows are weight rows, its 16 to 256 columns are rows of x.
 //
 // The weights become bfloat16 on their way to the MMA: level * scale is a bfloat16 number exactly (w4.h), so this
-// rounds nothing, and K may be summed in one accumulator whatever the groups.  (16 + level + 8) is a shift and an and-or away (the
+// rounds nothing, and K may be summed whatever the groups.  (16 + level + 8) is a shift and an and-or away (the
 // four bits at the top of bfloat16's mantissa at exponent 4), and one fused multiply-add makes (that) * s - 24 s: both 24 s and the
 // result are bfloat16 numbers.  Sixteen warps do this, eight a stage, the next stage's eight at the same time.
 //
 // Tiles of up to 128 rows of x (KB 2: two chunks of K a stage) have their weights in TENSOR memory, a lane a row: the levels come through a
 // ring of each warp's own (cp.async) and leave by tcgen05.st.  In shared memory, writing them and the MMA's reading them take 256 of the
-// some 340 cycles a chunk, whatever the width (32 rows, 8,192 x 8,192: 17.4 us, in tensor memory 15.7; 128 rows: 23.3 and 21.2).
+// some 340 cycles a chunk, whatever the width (32 rows, 8,192 x 8,192: 17.4 us, in tensor memory 15.8; 128 rows: 23.3 and 21.6).
 // Wider tiles (KB 1) need tensor memory for their sums and are bound by the MMAs: there the weights go to shared memory in the 128-byte
 // swizzle, a warp a slab of 16 rows, 16 bytes a lane from memory, several chunks ahead in registers.
 // x comes by TMA, one thread issues the MMAs, four warps store what is finished: lane = weight row, so a row of the result
@@ -20,9 +20,9 @@
 // of it code that runs once: a short loop over four columns beats straight code for sixteen, and every long division in front of
 // the first load shows (32 requests of a 16-layer model of width 1,024: 0.553 -> 0.495 ms a step by these).
 //
-// Measured, one after another from a graph: 64 rows, 8,192 x 8,192 16.9 us (floor 5.8: unpacking bounds it, some 280 cycles a chunk, and
-// 7 us of launch, first loads, exchange and stores); 2,048 rows, gated 16,384 x 2,048 102 us, 1,346 TFLOP/s; 4,096 rows, 8,192 x 8,192
-// 386 us, 1,422 TFLOP/s.
+// Measured, a few one after another from a graph: 64 rows, 8,192 x 8,192 17.4 us (floor 5.8: unpacking bounds it, some 280 cycles a chunk, and
+// 7 us of launch, first loads, exchange and stores); 2,048 rows, gated 16,384 x 2,048 104 us, 1,320 TFLOP/s; 4,096 rows, 8,192 x 8,192
+// 408 us, 1,350 TFLOP/s.  Repeated for a second the GPU runs at its power's clock: the gated product 121 us, 1,135 TFLOP/s at 1,410 MHz.
 //
 // Roles in a CTA: warp 0 TMA of x (one lane), warp 1 MMA issuer (one lane) and owner of tensor memory, then two sets of
 // eight warps for weights, the last four warps epilogue (tensor memory lanes 32 (warp % 4) ..).  Every wait on an mbarrier is bounded: after a

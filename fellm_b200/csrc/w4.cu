@@ -94,8 +94,9 @@ __device__ __forceinline__ void put_levels(const W4Out& o, int slab, int pair, i
   }
 }
 
-// A warp a slab x 128 elements.  Bound by the matrix's bytes: every element is read once, by loads of 16 bytes of which four neighbouring
-// lanes take 64 consecutive bytes of a row (128 of a float32 one).
+// A warp a slab x 128 elements.  Every element is read once, by loads of 16 bytes of which four neighbouring lanes take 64 consecutive bytes of a row
+// (128 of a float32 one).  Bound by instructions (issue slots 74% of a bfloat16 launch, 60% of a float32 one, whose 121 registers a thread leave sixteen warps
+// an SM): 65,536 x 2,048 takes 82 us from bfloat16, 52 at memory's rate, and 173 from float32, 93 at memory's rate.
 __global__ void __launch_bounds__(W4_THREADS) quantize_w4_f32_kernel(const float* w, long long ldw, int vec, W4Out o) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int pairs = (o.chunks + 1) / 2;

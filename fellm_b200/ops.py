@@ -1984,7 +1984,10 @@ def interleave_gate_up(gate, up):
 # ------------------------------------------------------------------------------ matrices in four bits
 
 W4_GROUPS = (32, 64, 128)
-W4_CUT_FIRST = 1 << 24                   # elements of a matrix from which float32 rows are cut into bfloat16 ones by a launch of their own
+W4_CUT_FIRST = 1 << 24                   # elements of a matrix from which float32 rows are cut into bfloat16 ones by a launch of their own, not by every warp
+#                                          (us, by every warp and first: 1 row, 4,096 x 2,048 5.4 and 6.2, 4,096 x 4,096 9.4 and 8.4, 8,192 x 8,192 33 and 19;
+#                                          8 rows 7.5 and 7.7, 13.0 and 10.6, 46 and 25.  Few slabs of a long K and 16 rows gain from fewer on: 1 row,
+#                                          256 x 16,384 16.9 and 11.2, 16 rows, 4,096 x 2,048 14.1 and 12.0)
 W4_READ_AHEAD = 32                       # chunks behind the end of a matrix that are there to be read (not used)
 W4_FEW_ROWS = 16                         # up to so many rows: mma.sync, a warp a slab of 16 weight rows; more: tcgen05
 #                                          (9 rows, 2,048 x 8,192: 5.3 us and 6.7; 16 rows, 65,536 x 2,048: 27.5 and 26.0, 1,024 x 1,024: 2.6 and 3.0)

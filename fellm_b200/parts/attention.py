@@ -203,7 +203,7 @@ class Attention(Mixer):
             self.w["sink"] = torch.full((self.H,), self.sink_score, dtype=torch.float32, device=q.device)
         self.kept_bf16 = self.w["qkv.weight"].dtype == torch.bfloat16
 
-    four_bit = ("qkv.weight", "out_proj.weight")
+    four_bit = ("qkv.weight", "out_proj.weight")          # (the gate a head stays: H rows of logits that each turn a whole head up or down)
 
     def reserve(self, device, max_rows, n_ctx):
         if self.kept_bf16 and not self.general:
