@@ -71,3 +71,51 @@ def test_gates_whose_sums_rise_and_fall(M):
     # |silu'| <= 1.1; half a step of bfloat16 and 2^-16 for the function
     room = 1.1 * eg * (up.abs() + eu) + gate.abs() * eu + (2.0 ** -8 + 2.0 ** -16) * 1.001 * want.abs()
     assert ((got - want).abs() <= room).all(), float(((got - want).abs() / room).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(8, 1024, 16384), (17, 1024, 8192), (64, 2048, 16384), (128, 96, 40000)])
+def test_a_norm_handed_on_behind_a_long_sum(M, N, K):
+    """What is handed on are the rows as they are written, whatever the sums are put together from."""
+    from fellm_b200 import ops
+    g = torch.Generator(device=DEV).manual_seed(M + N + K)
+    ops.reserve_norm_handoff(DEV, N)
+    w4 = ops.pack_w4(*w4_util.random_matrix(N, K, 64, g, DEV), 64)
+    x = torch.randn(M, K, generator=g, device=DEV).bfloat16()
+    stream, weight = torch.randn(M, N, generator=g, device=DEV), torch.rand(N, generator=g, device=DEV) + 0.5
+    plain = stream.clone()
+    ops.gemm_w4(x, w4, out=plain, accumulate=True)
+    ops.forget_norm_handoff()
+    ops.expect_norm(stream, weight)
+    ops.gemm_w4(x, w4, out=stream, accumulate=True)
+    h = ops.norm_handoff(stream, weight)
+    assert torch.equal(stream, plain) and torch.equal(h.xg, (stream * weight).bfloat16())
+    want = stream.double().view(M, h.parts, -1).pow(2).sum(-1)
+    assert ((h.ssq[:M * h.parts].view(M, -1).double() - want).abs() <= 20 * 2.0 ** -24 * want).all()        # (squares and at most 16 sums of positive numbers)
+    ops.forget_norm_handoff()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [40, 200, 600])
+def test_long_sums_in_a_replayed_graph_and_on_two_streams(M):
+    from fellm_b200 import ops
+    g = torch.Generator(device=DEV).manual_seed(M)
+    w4 = ops.pack_w4(*w4_util.random_matrix(1536, 8192, 64, g, DEV), 64)
+    xs = [torch.randn(M, 8192, generator=g, device=DEV).bfloat16() for _ in range(4)]
+    want = [ops.gemm_w4(x, w4) for x in xs]
+    held, y, side = xs[0].clone(), torch.empty(M, 1536, device=DEV, dtype=torch.bfloat16), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.gemm_w4(held, w4, out=y)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.gemm_w4(held, w4, out=y)
+    for i in range(4):
+        held.copy_(xs[i])
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = [ops.gemm_w4(x, w4) for x in xs]
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[i]) and all(torch.equal(a, b) for a, b in zip(beside, want))
+    ops.check_umma_status(DEV)
