@@ -2036,7 +2036,7 @@ def _w4_room(N: int, K: int, group: int, device):
     """Levels [slabs, chunks, 128] and scales [slabs, groups, 8], each with room behind it that a kernel may read ahead into."""
     if group not in W4_GROUPS:
         raise KernelError(f"a group of {group}: four-bit matrices have groups of {', '.join(map(str, W4_GROUPS))}")
-    if N < 1 or K < 1 or N > 2 ** 30 or K > 2 ** 20:           # (a bfloat16 result's K is one sum in tensor memory: its error grows with it)
+    if N < 1 or K < 1 or N > 2 ** 30 or K > 2 ** 20:           # (sums are tested up to that K)
         raise KernelError(f"a matrix of {N} x {K} cannot be held in four bits")
     slabs, chunks = -(-N // 16), -(-K // 64)
     return (torch.empty((slabs * chunks + W4_READ_AHEAD) * 128, dtype=torch.int32, device=device),
